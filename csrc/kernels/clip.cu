@@ -1,0 +1,246 @@
+// Norm of all gradients of a step and their clipping, over any number of tensors.
+//
+//   norm = |scale| sqrt(sum g^2)      coef = norm <= max ? 1 : max / norm      out = coef * scale * g
+//
+// Bound by memory: every gradient is read for the norm and, where clipped gradients are wanted, again for the product (out of L2 as far as
+// they fit), or by the optimizer, which takes the coefficient along. A launch knows its tensors from its parameters, CLIP_TENSORS of
+// them, cut into chunks of CLIP_CHUNK values; nothing is kept between calls.
+//
+// Squares are summed in f32 over eight values, those sums in f64, in an order that the sizes give: the same bits every time.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "ono_kernels.h"
+
+namespace ono {
+void set_error(const char* fmt, const char* a, long long b, long long c);
+
+constexpr int CLIP_TENSORS = 256, CLIP_CHUNK = 4096, CLIP_THREADS = 256, CLIP_MAX_BLOCKS = 8 * 148;
+
+// A tensor's values are counted from the 8 values' boundary in front of the first (`phase` before it), so that groups of eight
+// that begin at a multiple of eight are aligned.
+struct ClipBatch {
+  const void* g[CLIP_TENSORS];
+  void* out[CLIP_TENSORS];
+  long long n[CLIP_TENSORS];
+  unsigned int end[CLIP_TENSORS];        // chunks up to and with this tensor's
+  unsigned char phase[CLIP_TENSORS], type[CLIP_TENSORS];      // type: that of g, and of out times four
+  int count;
+};
+
+__device__ __forceinline__ float clip_load(const void* p, int type, long long i) {
+  if (type == 0) return reinterpret_cast<const float*>(p)[i];
+  if (type == 1) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void clip_store(void* p, int type, long long i, float v) {
+  if (type == 0) reinterpret_cast<float*>(p)[i] = v;
+  else if (type == 1) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+// Eight values from i on, zeros outside [0, n); whole groups by 16-byte loads.
+__device__ __forceinline__ void clip_load8(const void* p, int type, long long i, long long n, float (&v)[8]) {
+  if (i >= 0 && i + 8 <= n) {
+    if (type == 0) {
+      const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+      const float4 a = q[0], b = q[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = type == 1 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[k])) : __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+        v[2 * k] = f.x; v[2 * k + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = i + k >= 0 && i + k < n ? clip_load(p, type, i + k) : 0.0f;
+  }
+}
+__device__ __forceinline__ void clip_store8(void* p, int type, long long i, long long n, bool aligned, const float (&v)[8]) {
+  if (aligned && i >= 0 && i + 8 <= n) {
+    if (type == 0) {
+      float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i);
+      q[0] = make_float4(v[0], v[1], v[2], v[3]);
+      q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (type == 1) { const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]); u[k] = *reinterpret_cast<const uint32_t*>(&h); }
+        else { const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]); u[k] = *reinterpret_cast<const uint32_t*>(&h); }
+      }
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) if (i + k >= 0 && i + k < n) clip_store(p, type, i + k, v[k]);
+  }
+}
+
+// The tensor that chunk c belongs to.
+__device__ __forceinline__ int clip_find(const ClipBatch& b, unsigned int c) {
+  int lo = 0, hi = b.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (b.end[mid] > c) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
+// The sum of eight squares. In f32 unless one of them is out of its range (above 2^62 in size, or below 2^-48 all of them).
+__device__ __forceinline__ double squares8(const float (&v)[8]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s = fmaf(v[k], v[k], s);
+  if (s > 2e37f || s < 1e-28f) {
+    double t = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += (double)v[k] * (double)v[k];
+    return t;
+  }
+  return (double)s;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int w = 0; w < CLIP_THREADS / 32; ++w) v += s[w];
+  return v;
+}
+
+// part[block] (+)= the squares of the block's chunks.
+__global__ void __launch_bounds__(CLIP_THREADS) clip_norm_kernel(const __grid_constant__ ClipBatch b, double* part, int first) {
+  __shared__ double s[CLIP_THREADS / 32];
+  double acc = 0.0;
+  for (unsigned int c = blockIdx.x; c < b.end[b.count - 1]; c += gridDim.x) {
+    const int t = clip_find(b, c);
+    const long long at = (long long)(c - (t ? b.end[t - 1] : 0)) * CLIP_CHUNK - b.phase[t];
+#pragma unroll
+    for (int k = 0; k < CLIP_CHUNK / CLIP_THREADS / 8; ++k) {
+      float v[8];
+      clip_load8(b.g[t], b.type[t] & 3, at + 8 * (k * CLIP_THREADS + (int)threadIdx.x), b.n[t], v);
+      acc += squares8(v);
+    }
+  }
+  acc = block_sum(acc, s);
+  if (threadIdx.x == 0) part[blockIdx.x] = first ? acc : part[blockIdx.x] + acc;
+}
+
+// Norm and coefficient from the blocks' sums; every block that calls it gets the same ones.
+__device__ __forceinline__ double clip_coef(const double* part, int parts, float scale, float max_norm, float* norm_out, float* coef_out, double* s) {
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < parts; i += CLIP_THREADS) sum += part[i];
+  sum = block_sum(sum, s);
+  const double norm = fabs((double)scale) * sqrt(sum), coef = norm <= (double)max_norm ? 1.0 : (double)max_norm / norm;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (norm_out) *norm_out = (float)norm;
+    if (coef_out) *coef_out = (float)coef;
+  }
+  return coef;
+}
+
+__global__ void __launch_bounds__(CLIP_THREADS) clip_finish_kernel(const double* part, int parts, float scale, float max_norm, float* norm, float* coef) {
+  __shared__ double s[CLIP_THREADS / 32];
+  clip_coef(part, parts, scale, max_norm, norm, coef, s);
+}
+
+__global__ void __launch_bounds__(CLIP_THREADS) clip_write_kernel(const __grid_constant__ ClipBatch b, const double* part, int parts, float scale, float max_norm,
+                                                                  float* norm, float* coef) {
+  __shared__ double s[CLIP_THREADS / 32];
+  const float f = (float)(clip_coef(part, parts, scale, max_norm, norm, coef, s) * (double)scale);
+  for (unsigned int c = blockIdx.x; c < b.end[b.count - 1]; c += gridDim.x) {
+    const int t = clip_find(b, c), type = b.type[t] & 3, otype = b.type[t] >> 2;
+    if (f == 1.0f && b.out[t] == b.g[t]) continue;
+    const long long at = (long long)(c - (t ? b.end[t - 1] : 0)) * CLIP_CHUNK - b.phase[t];
+    const bool aligned = (((uintptr_t)b.out[t] / (otype ? 2 : 4)) & 7) == b.phase[t];
+#pragma unroll
+    for (int k = 0; k < CLIP_CHUNK / CLIP_THREADS / 8; ++k) {
+      const long long i = at + 8 * (k * CLIP_THREADS + (int)threadIdx.x);
+      if (i >= b.n[t]) break;
+      float v[8];
+      clip_load8(b.g[t], type, i, b.n[t], v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] *= f;
+      clip_store8(b.out[t], otype, i, b.n[t], aligned, v);
+    }
+  }
+}
+}  // namespace ono
+
+using namespace ono;
+
+extern "C" long long ono_clip_scratch(void) { return CLIP_MAX_BLOCKS * 8; }
+
+extern "C" int ono_clip(const OnoClip* c, ono_stream_t stream) {
+  if (!c || c->n_tensors < 0 || (c->n_tensors && !c->t) || !c->scratch || c->scratch_bytes < ono_clip_scratch() || ((uintptr_t)c->scratch & 7)) {
+    set_error("bad clip args%s", "", 0, 0);
+    return -1;
+  }
+  if (!(c->max_norm > 0.0f) || !isfinite(c->scale)) { set_error("clip: max_norm must be positive and scale finite%s", "", 0, 0); return -1; }
+  for (int k = 0; k < c->n_tensors; ++k) {
+    const OnoClipTensor& t = c->t[k];
+    if (t.n < 0 || (unsigned)t.g_dtype > 2u || (c->write && (unsigned)t.out_dtype > 2u) || (t.n && (!t.g || (c->write && !t.out))) ||
+        ((uintptr_t)t.g & (t.g_dtype ? 1 : 3)) || (c->write && ((uintptr_t)t.out & (t.out_dtype ? 1 : 3)))) {
+      set_error("bad clip tensor %s%lld", "", k, 0);
+      return -1;
+    }
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  double* part = reinterpret_cast<double*>(c->scratch);
+  ClipBatch b;
+  int next = 0;
+  // The tensors from `next` on that a launch takes; false where none are left.
+  auto fill = [&]() {
+    b.count = 0;
+    unsigned int end = 0;
+    for (; next < c->n_tensors && b.count < CLIP_TENSORS; ++next) {
+      const OnoClipTensor& t = c->t[next];
+      if (t.n == 0) continue;
+      const int k = b.count, esz = t.g_dtype ? 2 : 4;
+      const int phase = (int)(((uintptr_t)t.g / esz) & 7);
+      const long long chunks = (t.n + phase + CLIP_CHUNK - 1) / CLIP_CHUNK;
+      if (end + chunks >= (1ll << 31)) break;
+      b.g[k] = t.g; b.out[k] = t.out; b.n[k] = t.n;
+      b.phase[k] = (unsigned char)phase;
+      b.type[k] = (unsigned char)(t.g_dtype | (c->write ? t.out_dtype : 0) << 2);
+      b.end[k] = end += (unsigned)chunks;
+      ++b.count;
+    }
+    return b.count > 0;
+  };
+  int parts = 0;
+  while (fill()) {
+    const int grid = (int)std::min<long long>(b.end[b.count - 1], std::min(CLIP_MAX_BLOCKS, 8 * ono_num_sms()));
+    // later launches of a call add to the sums of the first ones; blocks that it had not start theirs
+    if (grid > parts && parts) {
+      const cudaError_t e = cudaMemsetAsync(part + parts, 0, (size_t)(grid - parts) * 8, st);
+      if (e != cudaSuccess) { set_error("clip: %s", cudaGetErrorString(e), 0, 0); return -7; }
+    }
+    clip_norm_kernel<<<grid, CLIP_THREADS, 0, st>>>(b, part, parts == 0);
+    parts = std::max(parts, grid);
+  }
+  if (!c->write || parts == 0) {
+    clip_finish_kernel<<<1, CLIP_THREADS, 0, st>>>(part, parts, c->scale, c->max_norm, c->norm, c->coef);
+  } else {
+    next = 0;
+    while (fill()) {
+      const int grid = (int)std::min<long long>(b.end[b.count - 1], 8 * ono_num_sms());
+      clip_write_kernel<<<grid, CLIP_THREADS, 0, st>>>(b, part, parts, c->scale, c->max_norm, c->norm, c->coef);
+    }
+  }
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) { set_error("clip launch: %s", cudaGetErrorString(e), 0, 0); return -7; }
+  return 0;
+}

@@ -854,6 +854,12 @@ extern "C" int ono_sizeof(int which) {
     case 12: return (int)sizeof(OnoConvDgrad);
     case 13: return (int)sizeof(OnoConvFprop);
     case 10: return (int)sizeof(OnoColsum);
+    case 14: return (int)sizeof(OnoEmbedding);
+    case 15: return (int)sizeof(OnoEmbeddingGrad);
+    case 16: return (int)sizeof(OnoTokens);
+    case 17: return (int)sizeof(OnoTokensGrad);
+    case 18: return (int)sizeof(OnoClipTensor);
+    case 19: return (int)sizeof(OnoClip);
     default: return -1;
   }
 }

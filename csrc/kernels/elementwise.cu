@@ -456,7 +456,7 @@ __device__ __forceinline__ float optim_one(int kind, const OptimScalars& s, floa
 }
 
 __global__ void optim_kernel(const OnoOptim o) {
-  OptimScalars s{o.lr, o.mu, o.b1, o.b2, o.eps, o.grad_scale, 0.0f};
+  OptimScalars s{o.lr, o.mu, o.b1, o.b2, o.eps, o.grad_coef ? o.grad_scale * *o.grad_coef : o.grad_scale, 0.0f};
   if (o.kind == 2) {
     const float b1t = o.adam_pows[0], b2t = o.adam_pows[1];
     s.adam_step = o.lr * sqrtf(1.0f - b2t) / (1.0f - b1t);

@@ -188,6 +188,7 @@ typedef struct OnoOptim {
   const float* adam_pows;// device float[2] = {b1^t, b2^t} after this step's tick
   void* p_bf16;          // optional bf16 shadow of p
   int zero_grad;         // 1: g is zeroed after use (g must be writable)
+  const float* grad_coef;// optional device scalar that g is multiplied by as well (a clipping coefficient, ono_clip)
 } OnoOptim;
 int ono_optim(const OnoOptim* o, ono_stream_t stream);
 int ono_adam_tick(float* pows, float b1, float b2, ono_stream_t stream);  // pows *= {b1, b2}
@@ -476,6 +477,88 @@ int ono_sparse_lift(float* acc, long long n, const unsigned int* idx, const void
 int ono_sparse_lift_range(float* acc, long long begin, long long end, const unsigned int* idx, const void* val_f16,
                           const unsigned int* count, unsigned int capacity, const void* dense16, int dense_f16,
                           unsigned long long* bytes, ono_stream_t st);
+
+// ---------------------------------------------------------------------------------------------
+// Rows of a table by token (embedding.cu). ids: int32, or int64 with ids64; an id equal to padding_id stands for no token, any other outside
+// [0, vocab) likewise, and *status (optional) is set to ONO_ERR_BAD_ARG for those. dtypes: 0 f32, 1 bf16. Leading dimensions in elements.
+// ---------------------------------------------------------------------------------------------
+typedef struct OnoEmbedding {
+  const void* table;         // [vocab, ld_table]
+  const void* ids;           // [n]
+  void* out;                 // [n, ld_out]: out[i] = scale * table[ids[i]], zeros where there is no token
+  long long n, ld_table, ld_out, padding_id;
+  int vocab, width, table_bf16, out_bf16, ids64;
+  float scale;
+  int* status;
+} OnoEmbedding;
+int ono_embedding(const OnoEmbedding* e, ono_stream_t stream);
+// grad[v] = (accumulate ? grad[v] : 0) + scale * sum of d[i] over the i with ids[i] == v, in ascending order of i whatever the launch
+// looks like (the same bits every time). scratch: ono_embedding_grad_scratch bytes, 16-byte aligned; calls that overlap on the device need one each.
+typedef struct OnoEmbeddingGrad {
+  const void* d;             // [n, ld_d]
+  const void* ids;           // [n]
+  float* grad;               // [vocab, ld_grad]
+  long long n, ld_d, ld_grad, padding_id;
+  int vocab, width, d_bf16, ids64, accumulate;
+  float scale;
+  int* status;
+  void* scratch;
+  long long scratch_bytes;
+} OnoEmbeddingGrad;
+long long ono_embedding_grad_scratch(long long n, int vocab, int width);
+int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream);
+
+// ---------------------------------------------------------------------------------------------
+// Softmax over a vocabulary with one given token per row (token_loss.cu). With m = max x, z = sum exp(x - m):
+//   lse = m + ln z,  logp = (x[target] - m) - ln z,  entropy = ln z - sum exp(x - m) (x - m) / z,  top: the largest logits, ties to the
+//   lowest index. A logit of -inf has probability zero; a row of nothing else has logp = lse = -inf, entropy 0 and a gradient of zeros. A row
+//   with a NaN or +inf has NaN for all of them. A row whose target is ignore_id (or outside [0, V), which sets *status to ONO_ERR_BAD_ARG)
+//   is not read: zeros, and no alternatives. Places that have no alternative: id -1, log probability -inf.
+// ---------------------------------------------------------------------------------------------
+#define ONO_TOP_MAX 32
+typedef struct OnoTokens {
+  const void* x;             // [R, ld] logits
+  const void* targets;       // [R], optional (every row is read then, and logp, out are not to be had)
+  long long R, ld, ld_out, ignore_id;
+  int V, x_bf16, targets64, top;
+  float *logp, *lse, *entropy;       // [R], each optional
+  float* top_logp; int* top_id;      // [R, top], both or none
+  // Optional, the token loss -scale * sum_r weight[r] logp[r]: its gradient scale * weight[r] * (p - 1[target]). `out` may be x (same type).
+  void* out; int out_bf16;
+  const float* weight;       // [R], optional (ones)
+  float scale;
+  int* status;
+} OnoTokens;
+int ono_tokens(const OnoTokens* t, ono_stream_t stream);
+// out = d_logp (1[target] - p) - d_entropy p (ln p + entropy): the logits' gradient from those of ono_tokens' results.
+typedef struct OnoTokensGrad {
+  const void* x;             // [R, ld]
+  const void* targets;       // [R], optional (only d_entropy then)
+  long long R, ld, ld_out, ignore_id;
+  int V, x_bf16, targets64;
+  const float *lse, *entropy, *d_logp, *d_entropy;   // [R]; d_logp optional; entropy and d_entropy both or none
+  void* out; int out_bf16;   // [R, ld_out], may be x (same type)
+  int* status;
+} OnoTokensGrad;
+int ono_tokens_grad(const OnoTokensGrad* t, ono_stream_t stream);
+
+// ---------------------------------------------------------------------------------------------
+// Norm of all gradients and clipping (clip.cu). `t` lists the tensors (contiguous, any alignment of their type; dtypes 0 f32, 1 bf16, 2 f16).
+//   norm = |scale| sqrt(sum over all tensors of g^2);  coef = norm <= max_norm ? 1 : max_norm / norm (NaN for a NaN)
+//   out = coef * scale * g where out is given (it may be g itself, of the same type).
+// scratch: ono_clip_scratch bytes, 8-byte aligned; calls that overlap on the device need one each.
+// ---------------------------------------------------------------------------------------------
+typedef struct OnoClipTensor { const void* g; void* out; long long n; int g_dtype, out_dtype; } OnoClipTensor;
+typedef struct OnoClip {
+  const OnoClipTensor* t;    // host memory
+  int n_tensors;
+  float scale, max_norm;
+  float* norm; float* coef;  // device, each optional
+  int write;                 // 1: out is written
+  void* scratch; long long scratch_bytes;
+} OnoClip;
+long long ono_clip_scratch(void);
+int ono_clip(const OnoClip* c, ono_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -93,6 +93,11 @@ def _declare(lib) -> None:
         "ono_stage_pull": [C.POINTER(OnoStagePull), vp],
         "ono_stage_signal": [C.POINTER(vp), ci, ci, ci, vp, vp],
         "ono_stage_tick": [vp, vp],
+        "ono_embedding": [C.POINTER(OnoEmbedding), vp],
+        "ono_embedding_grad": [C.POINTER(OnoEmbeddingGrad), vp],
+        "ono_tokens": [C.POINTER(OnoTokens), vp],
+        "ono_tokens_grad": [C.POINTER(OnoTokensGrad), vp],
+        "ono_clip": [C.POINTER(OnoClip), vp],
     }
     for name, args in sigs.items():
         fn = getattr(lib, name)
@@ -101,7 +106,12 @@ def _declare(lib) -> None:
     lib.ono_num_sms.restype = ci
     lib.ono_sizeof.argtypes = [ci]
     lib.ono_sizeof.restype = ci
+    lib.ono_embedding_grad_scratch.argtypes = [ll, ci, ci]
+    lib.ono_embedding_grad_scratch.restype = lib.ono_clip_scratch.restype = ll
     for i, st in enumerate((OnoGemm, OnoLoss, OnoOptim, OnoRows, OnoSync, OnoPsAsync, OnoRing, OnoStagePull, OnoRingEmu, OnoFeed, OnoColsum, OnoDenseStep)):
+        if lib.ono_sizeof(i) != C.sizeof(st):
+            raise RuntimeError(f"ABI mismatch for {st.__name__}: C {lib.ono_sizeof(i)} vs ctypes {C.sizeof(st)}")
+    for i, st in enumerate((OnoEmbedding, OnoEmbeddingGrad, OnoTokens, OnoTokensGrad, OnoClipTensor, OnoClip), 14):
         if lib.ono_sizeof(i) != C.sizeof(st):
             raise RuntimeError(f"ABI mismatch for {st.__name__}: C {lib.ono_sizeof(i)} vs ctypes {C.sizeof(st)}")
 
@@ -117,6 +127,52 @@ def stream_ptr(stream=None) -> int:
 
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+def one_device(first, *others) -> None:
+    """All on one GPU (None among them does not count)."""
+    if not first.is_cuda:
+        raise RuntimeError("this op runs on CUDA only (no CPU fallback on this path)")
+    at = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"tensors on different devices: cuda:{at} and {t.device}")
+
+
+def pitch(t) -> int:
+    """Elements from one row of a matrix to the next."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def status_ptr(t) -> int | None:
+    import torch
+
+    if t is not None and (t.dtype != torch.int32 or t.numel() < 1):
+        raise TypeError("status must be int32")
+    return None if t is None else t.data_ptr()
+
+
+def scratch(t, nbytes: int, stream):
+    """Memory for one call that launches on ``stream`` (None: the current one) of the GPU of ``t``: the allocator gives it to nobody else
+    before what that stream holds now has run."""
+    import torch
+
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=t.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=t.device)
+
+
+def launch(t, stream, name: str, args) -> None:
+    """``name(args, stream)`` with the GPU of ``t`` as the current device, on ``stream`` (None: the one that is current there)."""
+    import torch
+
+    fn = getattr(load(), name)
+    if t.get_device() == torch.cuda.current_device():
+        check(fn(args, stream_ptr(stream)), name)
+    else:
+        with torch.cuda.device(t.device):
+            check(fn(args, stream_ptr(stream)), name)
 
 
 # --------------------------------------------------------------------------------------------
@@ -171,7 +227,56 @@ class OnoOptim(C.Structure):
         ("n", C.c_longlong), ("kind", C.c_int),
         ("lr", C.c_float), ("mu", C.c_float), ("b1", C.c_float), ("b2", C.c_float), ("eps", C.c_float),
         ("grad_scale", C.c_float), ("adam_pows", C.c_void_p), ("p_bf16", C.c_void_p),
-        ("zero_grad", C.c_int),
+        ("zero_grad", C.c_int), ("grad_coef", C.c_void_p),
+    ]
+
+
+class OnoEmbedding(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p), ("ids", C.c_void_p), ("out", C.c_void_p),
+        ("n", C.c_longlong), ("ld_table", C.c_longlong), ("ld_out", C.c_longlong), ("padding_id", C.c_longlong),
+        ("vocab", C.c_int), ("width", C.c_int), ("table_bf16", C.c_int), ("out_bf16", C.c_int), ("ids64", C.c_int),
+        ("scale", C.c_float), ("status", C.c_void_p),
+    ]
+
+
+class OnoEmbeddingGrad(C.Structure):
+    _fields_ = [
+        ("d", C.c_void_p), ("ids", C.c_void_p), ("grad", C.c_void_p),
+        ("n", C.c_longlong), ("ld_d", C.c_longlong), ("ld_grad", C.c_longlong), ("padding_id", C.c_longlong),
+        ("vocab", C.c_int), ("width", C.c_int), ("d_bf16", C.c_int), ("ids64", C.c_int), ("accumulate", C.c_int),
+        ("scale", C.c_float), ("status", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_longlong),
+    ]
+
+
+class OnoTokens(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("targets", C.c_void_p),
+        ("R", C.c_longlong), ("ld", C.c_longlong), ("ld_out", C.c_longlong), ("ignore_id", C.c_longlong),
+        ("V", C.c_int), ("x_bf16", C.c_int), ("targets64", C.c_int), ("top", C.c_int),
+        ("logp", C.c_void_p), ("lse", C.c_void_p), ("entropy", C.c_void_p), ("top_logp", C.c_void_p), ("top_id", C.c_void_p),
+        ("out", C.c_void_p), ("out_bf16", C.c_int), ("weight", C.c_void_p), ("scale", C.c_float), ("status", C.c_void_p),
+    ]
+
+
+class OnoTokensGrad(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("targets", C.c_void_p),
+        ("R", C.c_longlong), ("ld", C.c_longlong), ("ld_out", C.c_longlong), ("ignore_id", C.c_longlong),
+        ("V", C.c_int), ("x_bf16", C.c_int), ("targets64", C.c_int),
+        ("lse", C.c_void_p), ("entropy", C.c_void_p), ("d_logp", C.c_void_p), ("d_entropy", C.c_void_p),
+        ("out", C.c_void_p), ("out_bf16", C.c_int), ("status", C.c_void_p),
+    ]
+
+
+class OnoClipTensor(C.Structure):
+    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("n", C.c_longlong), ("g_dtype", C.c_int), ("out_dtype", C.c_int)]
+
+
+class OnoClip(C.Structure):
+    _fields_ = [
+        ("t", C.POINTER(OnoClipTensor)), ("n_tensors", C.c_int), ("scale", C.c_float), ("max_norm", C.c_float),
+        ("norm", C.c_void_p), ("coef", C.c_void_p), ("write", C.c_int), ("scratch", C.c_void_p), ("scratch_bytes", C.c_longlong),
     ]
 
 

@@ -148,9 +148,12 @@ def optim_step(p: torch.Tensor, g: torch.Tensor, *, kind: str, lr: float, mu: fl
                b2: float = 0.999, eps: float = 1e-8, m: torch.Tensor | None = None,
                v: torch.Tensor | None = None, adam_pows: torch.Tensor | None = None,
                grad_scale: float = 1.0, p_bf16: torch.Tensor | None = None, zero_grad: bool = False,
-               stream=None) -> None:
-    """SGD / momentum / Adam on a flat f32 buffer (one kernel)."""
+               grad_coef: torch.Tensor | None = None, stream=None) -> None:
+    """SGD / momentum / Adam on a flat f32 buffer (one kernel). ``grad_coef``: one f32 on the device that the gradient is multiplied by beside
+    ``grad_scale`` (``clip.grad_norm``'s coefficient for gradients scaled by ``grad_scale``)."""
     _need_cuda(p)
+    if grad_coef is not None and (grad_coef.dtype != torch.float32 or grad_coef.numel() != 1 or grad_coef.device != p.device):
+        raise ValueError("grad_coef must be one float32 on the parameters' device")
     lib = _lib.load()
     o = _lib.OnoOptim()
     o.p, o.g, o.m, o.v = p.data_ptr(), g.data_ptr(), _p(m), _p(v)
@@ -161,6 +164,7 @@ def optim_step(p: torch.Tensor, g: torch.Tensor, *, kind: str, lr: float, mu: fl
     o.adam_pows = _p(adam_pows)
     o.p_bf16 = _p(p_bf16)
     o.zero_grad = int(zero_grad)
+    o.grad_coef = _p(grad_coef)
     _lib.check(lib.ono_optim(C.byref(o), _lib.stream_ptr(stream)), "ono_optim")
 
 

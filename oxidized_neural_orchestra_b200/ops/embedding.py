@@ -1,0 +1,84 @@
+"""Python entries to the rows-by-token kernels (``csrc/kernels/embedding.cu``): a table's rows looked up by token, and its gradient.
+
+Like the other ops each call launches on the current (or given) stream, can be captured into a graph and returns nothing. Tables and
+rows are 2-D with unit inner stride, f32 or bf16; ids are int32 or int64, of any shape."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+NO_PADDING = -(2**63)
+
+
+def _rows(t: torch.Tensor, what: str, dtypes=(torch.float32, torch.bfloat16)) -> None:
+    if t.dtype not in dtypes:
+        raise TypeError(f"{what} must be {' or '.join(str(d)[6:] for d in dtypes)}")
+    if t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < t.shape[1] and t.shape[0] > 1:
+        raise ValueError(f"{what} must be 2-D rows with unit inner stride")
+
+
+def _ids(ids: torch.Tensor, n: int) -> None:
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("ids must be int32 or int64")
+    if not ids.is_contiguous() or ids.numel() != n:
+        raise ValueError(f"ids must be contiguous, one for each of the {n} rows")
+
+
+def embedding(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, *, scale: float = 1.0, padding_id: int | None = -1,
+              status: torch.Tensor | None = None, stream=None) -> None:
+    """``out[i] = scale * table[ids[i]]`` (the product in f32, rounded once to the type of ``out``).
+
+    An id equal to ``padding_id`` (None: there is none) stands for no token: its row is zeros. So is that of any other id
+    outside the table, and then ``status`` (int32[1]) becomes non-zero."""
+    _rows(table, "table")
+    _rows(out, "out")
+    n, width = out.shape
+    _ids(ids, n)
+    if table.shape[1] != width:
+        raise ValueError(f"table rows have {table.shape[1]} values, out rows {width}")
+    _lib.one_device(table, ids, out, status)
+    if n == 0 or width == 0:
+        return
+    e = _lib.OnoEmbedding(table.data_ptr(), ids.data_ptr(), out.data_ptr(), n, _lib.pitch(table), _lib.pitch(out),
+                          NO_PADDING if padding_id is None else padding_id, table.shape[0], width, table.dtype == torch.bfloat16,
+                          out.dtype == torch.bfloat16, ids.dtype == torch.int64, scale, _lib.status_ptr(status))
+    _lib.launch(table, stream, "ono_embedding", C.byref(e))
+
+
+def embedding_grad_scratch(n: int, vocab: int, width: int) -> int:
+    """Bytes of scratch that ``embedding_grad`` wants for ``n`` tokens."""
+    return _lib.load().ono_embedding_grad_scratch(n, vocab, width)
+
+
+def embedding_grad(d: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, *, scale: float = 1.0, accumulate: bool = False,
+                   padding_id: int | None = -1, scratch: torch.Tensor | None = None, status: torch.Tensor | None = None,
+                   stream=None) -> None:
+    """Gradient of the table behind ``embedding``: ``grad[v]`` (f32) becomes ``scale`` times the sum of the ``d[i]`` with ``ids[i] == v``,
+    zeros for tokens that do not occur; with ``accumulate`` the sums are added to what is there and the other rows stay as they are. ``padding_id``
+    and ``status`` as for ``embedding``.
+
+    Sums are f32 and go over the tokens in one order that depends on the ids alone: the same bits every time. ``scratch``: a
+    contiguous tensor of at least ``embedding_grad_scratch`` bytes that no overlapping call uses (None: allocated for this call)."""
+    _rows(d, "d")
+    _rows(grad, "grad", (torch.float32,))
+    n, width = d.shape
+    vocab = grad.shape[0]
+    _ids(ids, n)
+    if grad.shape[1] != width:
+        raise ValueError(f"d rows have {width} values, grad rows {grad.shape[1]}")
+    if scratch is not None and not scratch.is_contiguous():
+        raise ValueError("scratch must be contiguous")
+    _lib.one_device(d, ids, grad, status, scratch)
+    if vocab == 0 or width == 0:
+        return
+    need = embedding_grad_scratch(n, vocab, width)
+    if scratch is None:
+        scratch = _lib.scratch(grad, need, stream)
+    e = _lib.OnoEmbeddingGrad(d.data_ptr(), ids.data_ptr(), grad.data_ptr(), n, _lib.pitch(d), _lib.pitch(grad),
+                              NO_PADDING if padding_id is None else padding_id, vocab, width, d.dtype == torch.bfloat16,
+                              ids.dtype == torch.int64, accumulate, scale, _lib.status_ptr(status), scratch.data_ptr(),
+                              scratch.numel() * scratch.element_size())
+    _lib.launch(grad, stream, "ono_embedding_grad", C.byref(e))

@@ -1,0 +1,116 @@
+"""What the operators on tokens and gradients refuse, before anything is launched."""
+import math
+
+import pytest
+import torch
+
+
+def _e():
+    return torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 8)
+
+
+def test_embedding():
+    from oxidized_neural_orchestra_b200.ops.embedding import embedding, embedding_grad
+
+    t, i, o = _e()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        embedding(t, i, o)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        embedding_grad(o, i, t)
+    for call in (embedding, lambda a, b, c: embedding_grad(c, b, a)):
+        with pytest.raises(TypeError):
+            call(t, i.float(), o)
+        with pytest.raises(TypeError):
+            call(t, i.to(torch.int16), o)
+        with pytest.raises(ValueError):
+            call(t, i[:2], o)
+        with pytest.raises(ValueError):
+            call(t, torch.zeros(6, dtype=torch.int64)[::2], o)
+        with pytest.raises(ValueError):
+            call(t, i, o[:, :7])
+        with pytest.raises(ValueError):
+            call(t.t().contiguous().t(), i, o)
+        with pytest.raises(ValueError):
+            call(t, i, o[0].expand(3, 8))
+        with pytest.raises(TypeError):
+            call(t.double(), i, o)
+        with pytest.raises(TypeError):
+            call(t, i, o.half())
+    with pytest.raises(TypeError):
+        embedding_grad(o, i, t.bfloat16())
+    with pytest.raises(ValueError):
+        embedding_grad(o, i, t, scratch=torch.zeros(100, 2)[:, 0])
+
+
+def test_tokens():
+    from oxidized_neural_orchestra_b200.ops.token_loss import token_logprobs, token_logprobs_grad, token_loss
+
+    x, t, v = torch.zeros(3, 9), torch.zeros(3, dtype=torch.int64), torch.zeros(3)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        token_logprobs(x, t, logp=v)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        token_loss(x, t, out=torch.zeros(3, 9))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        token_logprobs_grad(x, t, lse=v, d_logp=v, out=x)
+    for bad in (dict(logp=torch.zeros(4)), dict(logp=v.double()), dict(logp=torch.zeros(6)[::2]), dict(lse=torch.zeros(3, 1)), dict(entropy=v.bfloat16()),
+                dict(top_logp=torch.zeros(3, 10), top_id=torch.zeros(3, 10, dtype=torch.int32)), dict(top_logp=torch.zeros(2, 2), top_id=torch.zeros(2, 2, dtype=torch.int32)),
+                dict(top_logp=torch.zeros(3, 2), top_id=torch.zeros(3, 3, dtype=torch.int32))):
+        with pytest.raises((ValueError, RuntimeError)):
+            token_logprobs(x, t, **bad)
+    with pytest.raises(ValueError):
+        token_logprobs(torch.zeros(3, 90), t, top_logp=torch.zeros(3, 33), top_id=torch.zeros(3, 33, dtype=torch.int32))
+    for bad in (dict(top_logp=torch.zeros(3, 2)), dict(top_id=torch.zeros(3, 2, dtype=torch.int32)), dict(top_logp=torch.zeros(3, 2), top_id=torch.zeros(3, 2, dtype=torch.int64))):
+        with pytest.raises(TypeError):
+            token_logprobs(x, t, **bad)
+    for targets, err in ((t.float(), TypeError), (t[:2], ValueError), (t.unsqueeze(1), ValueError), (torch.zeros(6, dtype=torch.int64)[::2], ValueError)):
+        with pytest.raises(err):
+            token_logprobs(x, targets, lse=v)
+    with pytest.raises(ValueError):
+        token_logprobs(x, None, logp=v)
+    with pytest.raises(ValueError):
+        token_loss(x, None, out=x)
+    for logits, err in ((x.half(), TypeError), (x.t(), ValueError), (x[0], ValueError), (x[0].expand(3, 9), ValueError)):
+        with pytest.raises(err):
+            token_logprobs(logits, t, lse=v)
+    for out, err in ((torch.zeros(3, 8), ValueError), (torch.zeros(3, 9).half(), TypeError), (torch.zeros(9, 3).t(), ValueError), (x.view(torch.bfloat16)[:, :9], ValueError)):
+        with pytest.raises(err):
+            token_loss(x, t, out=out)
+        with pytest.raises(err):
+            token_logprobs_grad(x, t, lse=v, d_logp=v, out=out)
+    with pytest.raises(ValueError):
+        token_logprobs_grad(x, t, lse=v, out=x)
+    with pytest.raises(ValueError):
+        token_logprobs_grad(x, None, lse=v, d_logp=v, out=x)
+    with pytest.raises(ValueError):
+        token_logprobs_grad(x, t, lse=v, d_entropy=v, out=x)
+    with pytest.raises(ValueError):
+        token_logprobs_grad(x, t, lse=v, d_logp=v, entropy=v, out=x)
+    with pytest.raises(TypeError, match="status"):
+        from oxidized_neural_orchestra_b200.ops import _lib
+        _lib.status_ptr(v)
+
+
+def test_clip():
+    from oxidized_neural_orchestra_b200.ops.clip import clip_grads, grad_norm
+
+    g, n = [torch.zeros(4), torch.zeros(2, 3)], torch.zeros(1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        grad_norm(g, n)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        clip_grads(g, 1.0)
+    for max_norm in (0.0, -1.0, math.nan):
+        with pytest.raises(ValueError):
+            clip_grads(g, max_norm)
+    for scale in (math.nan, math.inf):
+        with pytest.raises(ValueError):
+            grad_norm(g, n, scale=scale)
+    for bad, err in (([torch.zeros(4, 4).t()], ValueError), ([torch.zeros(8)[::2]], ValueError), ([torch.zeros(4).double()], TypeError), ([torch.zeros(4).int()], TypeError)):
+        with pytest.raises(err):
+            grad_norm(bad, n)
+    with pytest.raises(TypeError):
+        grad_norm(torch.zeros(4), n)
+    for out in ([torch.zeros(4)], [torch.zeros(4), torch.zeros(3, 2)], [g[0].view(torch.bfloat16)[:4], torch.zeros(2, 3)]):
+        with pytest.raises(ValueError):
+            clip_grads(g, 1.0, out=out)
+    with pytest.raises(ValueError, match="one place"):
+        clip_grads([g[0], g[0]], 1.0)
