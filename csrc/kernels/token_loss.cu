@@ -6,8 +6,10 @@
 //
 // All of it is f32 whatever the logits' type; x - m before the multiplication by log2 e, so that logits of any size keep their distances.
 //
-// Bound by memory, so a row is read once: it lies in the shared memory of one warp, one CTA or a cluster of up to eight while it is gone through
-// for its maximum, its sum, its alternatives and its gradient, and the next row is on its way meanwhile (asynchronous copies).
+// Bound by memory, so a row is read once, by a warp, a CTA or a cluster of up to eight: a thread keeps a running maximum and sum of what it has seen,
+// the warps hand theirs to each other, and for the loss's gradient the row waits in shared memory meanwhile. Instructions are the next
+// bound (16 bits a logit leave 11 issue slots each at the memory's rate): two logits go into one instruction where there is one, nothing is
+// looked at logit by logit that can be decided for a thread, and what a row costs beside its logits is spread over many of them a thread.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -29,7 +31,7 @@ enum TokMode : int { TOK_LOGP, TOK_ENTROPY, TOK_TOP, TOK_LOSS, TOK_GRAD };
 struct TokDev {
   const void* x; const void* targets;
   long long R, ld, ld_out, ignore_id;
-  int V, targets64, top, per, stages;      // per: 16-byte groups of a row that a CTA takes
+  int V, targets64, top, per, staged;      // per: 16-byte groups of a row that a CTA takes; staged: they are kept in shared memory
   float *logp, *lse, *entropy, *top_logp;
   int* top_id;
   void* out;
@@ -44,11 +46,44 @@ struct TokDev {
 constexpr float LSE_EXACT = 128.0f;
 constexpr int TOK_CTAS = 8;      // of a cluster, at most
 
-__device__ __forceinline__ float exp_of(float d) {      // exp(d)
+// 2^t
+__device__ __forceinline__ float exp2_of(float t) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+__device__ __forceinline__ float exp_of(float d) { return exp2_of(d * LOG2E); }
+// Two values an instruction.
+__device__ __forceinline__ float2 fma_2(float2 a, float2 b, float2 c) {
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 z, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(a.x), "=f"(a.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return a;
+}
+__device__ __forceinline__ float2 mul_2(float2 a, float2 b) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(a.x), "=f"(a.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return a;
+}
+__device__ __forceinline__ float2 add_2(float2 a, float2 b) {
+  add_f32x2(a.x, a.y, b.x, b.y);
+  return a;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// A maximum beyond this in size, times log2 e, is rounded by more than a few hundredths (and may leave f32): such a row is gone through again.
+constexpr float TOK_FAR = 1e6f;
+// What exponents are taken relative to, in units of log2: the maximum's, of any size, rounded; a logit is then one multiply-add, and its error
+// that of the difference. Zero where there is nothing but far negative ones (all exponentials are zero then).
+__device__ __forceinline__ float shift_of(float m) { return m < -TOK_FAR ? 0.0f : m * LOG2E; }
+
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 __device__ __forceinline__ void cp_async16(void* smem, const void* g) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(g) : "memory");
 }
@@ -68,7 +103,13 @@ template <> struct TokVec<float> {
   static __device__ __forceinline__ void get(const uint4& w, float (&v)[4]) {
     v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
   }
-  static __device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
+  static constexpr uint32_t NINF = 0xff800000u;      // a word of logits that are -inf
+  static __device__ __forceinline__ float most(const uint4 (&w)[4]) {
+    float m = __int_as_float(0xff800000);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(w[k].x), __uint_as_float(w[k].y))), fmaxf(__uint_as_float(w[k].z), __uint_as_float(w[k].w)));
+    return m;
+  }
 };
 template <> struct TokVec<__nv_bfloat16> {
   static constexpr int E = 8;
@@ -77,58 +118,80 @@ template <> struct TokVec<__nv_bfloat16> {
 #pragma unroll
     for (int k = 0; k < 4; ++k) { v[2 * k] = __uint_as_float(u[k] << 16); v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
   }
-  static __device__ __forceinline__ __nv_bfloat16 ninf() { return __ushort_as_bfloat16(0xff80); }
+  static constexpr uint32_t NINF = 0xff80ff80u;
+  static __device__ __forceinline__ float most(const uint4 (&w)[4]) {
+    __nv_bfloat162 m[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w[k]);
+      m[k] = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    }
+    m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    return fmaxf(__low2float(m[0]), __high2float(m[0]));
+  }
 };
 
-template <int GW>
+template <int W>
 __device__ __forceinline__ void group_sync() {
-  if (GW == 1) __syncwarp(); else __syncthreads();
+  if (W == 1) __syncwarp(); else __syncthreads();
 }
 
-// GW warps to a row; a group of one warp has CAP places for candidates, a CTA more.
-template <int GW> struct TokShared {
-  static constexpr int CAP = GW == 1 ? 256 : 512;
-  float top[GW];
-  unsigned int cut[GW];
-  float2 sum[GW];
-  unsigned int count, tally[2];
+// W warps to a row; CAP: places for candidates.
+template <int W> struct TokShared {
+  static constexpr int CAP = W == 1 ? 256 : 512;
+  unsigned int count, threads, tally[W];
+  unsigned short who[W * 32];
 };
-struct TokPeers {      // what the CTAs of a cluster tell each other, for this row and the next
-  float4 part[2][TOK_CTAS];
-  unsigned long long key[2][TOK_CTAS][ONO_TOP_MAX];
+// What the warps of a row's CTAs tell each other, for this row and the next: maximum, sum, sum times exponent, bound of the alternatives.
+template <bool TOP> struct TokPeers {
+  float4 part[2][TOK_CTAS * 4];
+  unsigned long long key[2][TOP ? TOK_CTAS : 1][ONO_TOP_MAX];
 };
 
 // The group's sum of a whole number.
-template <int GW>
+template <int W>
 __device__ __forceinline__ unsigned int group_count(unsigned int v, unsigned int* s_warp, int gt) {
   v = __reduce_add_sync(0xffffffffu, v);
-  if (GW == 1) return v;
+  if (W == 1) return v;
   __syncthreads();
   if ((gt & 31) == 0) s_warp[gt >> 5] = v;
   __syncthreads();
   v = 0;
 #pragma unroll
-  for (int w = 0; w < GW; ++w) v += s_warp[w];
+  for (int w = 0; w < W; ++w) v += s_warp[w];
   return v;
 }
 
-// The candidates for the `top` largest logits of n groups of 16 bytes, group 0 being group v0 of the row, exactly: where so many logits are
-// as large as the bound that there is no room for them (equal ones, mostly). The K-th largest value is found bit by bit, then come
-// all that are above it, and of those equal to it the first ones.
-template <typename T, int GW>
-__device__ __noinline__ void exact_candidates(const uint4* buf, int n, int v0, int ph, int K, unsigned long long* cand, TokShared<GW>& s, int gt) {
-  constexpr int E = TokVec<T>::E, GT = GW * 32, BITS = 8 * (int)sizeof(T);
-  auto for_all = [&](auto f) {
-    for (int v = gt; v < n; v += GT) {
-      float x[E];
-      TokVec<T>::get(buf[v], x);
+// A group of 16 bytes of a row that begins `ph` logits into group 0; -inf outside of the row.
+template <typename T>
+__device__ __forceinline__ void tok_group(const T* x, int ph, int V, int v, float (&o)[TokVec<T>::E]) {
+  constexpr int E = TokVec<T>::E;
+  if (v * E >= ph && (v + 1) * E <= ph + V) {
+    TokVec<T>::get(load16(x + (v * E - ph)), o);
+  } else {
 #pragma unroll
-      for (int k = 0; k < E; ++k) if (x[k] > __int_as_float(0xff800000)) f(order_of(x[k]) >> (32 - BITS), x[k], (v0 + v) * E + k - ph);
+    for (int k = 0; k < E; ++k) { const int j = v * E + k - ph; o[k] = j >= 0 && j < V ? to_f32(x[j]) : __int_as_float(0xff800000); }
+  }
+}
+
+// The candidates for the K largest logits of the groups v0 to v1 of a row, exactly: where so many logits are as large as the bound that there
+// is no room for them (equal ones, mostly). The K-th largest value is found bit by bit, then come all that are above it, and of those
+// equal to it the first ones.
+template <typename T, int W>
+__device__ __noinline__ void exact_candidates(const T* x, int ph, int V, int v0, int v1, int K, unsigned long long* cand, TokShared<W>& s, int gt) {
+  constexpr int E = TokVec<T>::E, GT = W * 32, BITS = 8 * (int)sizeof(T);
+  const float ninf = __int_as_float(0xff800000);
+  auto for_all = [&](auto f) {
+    for (int v = v0 + gt; v < v1; v += GT) {
+      float q[E];
+      tok_group(x, ph, V, v, q);
+#pragma unroll
+      for (int k = 0; k < E; ++k) if (q[k] > ninf) f(order_of(q[k]) >> (32 - BITS), q[k], v * E + k - ph);
     }
   };
   unsigned int valid = 0;
   for_all([&](unsigned int, float, int) { ++valid; });
-  valid = group_count<GW>(valid, s.cut, gt);
+  valid = group_count<W>(valid, s.tally, gt);
   const unsigned int want = min((unsigned int)K, valid);
   unsigned int value = 0;      // the largest with at least `want` logits not below it
   if (want) {
@@ -136,71 +199,127 @@ __device__ __noinline__ void exact_candidates(const uint4* buf, int n, int v0, i
       const unsigned int t = value | 1u << b;
       unsigned int c = 0;
       for_all([&](unsigned int o, float, int) { c += o >= t; });
-      if (group_count<GW>(c, s.cut, gt) >= want) value = t;
+      if (group_count<W>(c, s.tally, gt) >= want) value = t;
     }
   }
   unsigned int above = 0;
   for_all([&](unsigned int o, float, int) { above += o > value; });
-  above = group_count<GW>(above, s.cut, gt);
-  group_sync<GW>();
+  above = group_count<W>(above, s.tally, gt);
+  group_sync<W>();
   if (gt == 0) s.count = 0;
-  group_sync<GW>();
-  if (want) for_all([&](unsigned int o, float x, int j) { if (o > value) cand[atomicAdd(&s.count, 1u)] = top_key(x, j); });
+  group_sync<W>();
+  if (want) for_all([&](unsigned int o, float q, int j) { if (o > value) cand[atomicAdd(&s.count, 1u)] = top_key(q, j); });
   unsigned int missing = want - above;      // of the equal ones, in the order of their places
-  for (int at = 0; at < n && missing; at += GT) {
+  for (int at = v0; at < v1 && missing; at += GT) {
     const int v = at + gt;
-    float x[E];
+    float q[E];
     unsigned int mine = 0;
-    if (v < n) {
-      TokVec<T>::get(buf[v], x);
+    if (v < v1) {
+      tok_group(x, ph, V, v, q);
 #pragma unroll
-      for (int k = 0; k < E; ++k) mine += x[k] > __int_as_float(0xff800000) && (order_of(x[k]) >> (32 - BITS)) == value;
+      for (int k = 0; k < E; ++k) mine += q[k] > ninf && (order_of(q[k]) >> (32 - BITS)) == value;
     }
     unsigned int before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const unsigned int w = __shfl_up_sync(0xffffffffu, before, o); if ((gt & 31) >= o) before += w; }
     unsigned int total = __shfl_sync(0xffffffffu, before, 31);
     before -= mine;
-    if (GW > 1) {
+    if (W > 1) {
       __syncthreads();
-      if ((gt & 31) == 0) s.cut[gt >> 5] = total;
+      if ((gt & 31) == 0) s.tally[gt >> 5] = total;
       __syncthreads();
       total = 0;
 #pragma unroll
-      for (int w = 0; w < GW; ++w) { if (w < (gt >> 5)) before += s.cut[w]; total += s.cut[w]; }
+      for (int w = 0; w < W; ++w) { if (w < (gt >> 5)) before += s.tally[w]; total += s.tally[w]; }
     }
     if (mine && before < missing) {
 #pragma unroll
       for (int k = 0; k < E; ++k)
-        if (x[k] > __int_as_float(0xff800000) && (order_of(x[k]) >> (32 - BITS)) == value && before++ < missing)
-          cand[atomicAdd(&s.count, 1u)] = top_key(x[k], (v0 + v) * E + k - ph);
+        if (q[k] > ninf && (order_of(q[k]) >> (32 - BITS)) == value && before++ < missing) cand[atomicAdd(&s.count, 1u)] = top_key(q[k], v * E + k - ph);
     }
     missing -= min(missing, total);
   }
-  group_sync<GW>();
+  group_sync<W>();
 }
 
-template <typename T, typename O, int MODE, int GW, int NT>
+// Maximum and sums of some logits: z = sum 2^(x log2 e - shift), u = sum 2^q q of those exponents q, shift = shift_of(m).
+struct TokSums { float m, z, u; };
+// The sum over the warp's lanes; every lane gets it.
+template <bool ENT>
+__device__ __forceinline__ TokSums tok_join(TokSums s) {
+  const float m = of_order(__reduce_max_sync(0xffffffffu, order_of(s.m))), by = shift_of(s.m) - shift_of(m), f = exp2_of(by);
+  if (ENT) s.u = s.z == 0.0f ? 0.0f : f * (s.u + fmaxf(by, -1e4f) * s.z);      // (zero times a number, far below)
+  s.z = s.z == 0.0f ? 0.0f : f * s.z;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { s.z += __shfl_xor_sync(0xffffffffu, s.z, o); if (ENT) s.u += __shfl_xor_sync(0xffffffffu, s.u, o); }
+  s.m = m;
+  return s;
+}
+
+// Rows out of the ordinary, out of line.
+// Sums of the groups v0 to v1 relative to the row's maximum m, differences first.
+template <typename T, int W>
+__device__ __noinline__ TokSums far_sums(const T* x, int ph, int V, int v0, int v1, float m, int gt) {
+  constexpr int E = TokVec<T>::E;
+  TokSums s = {m, 0.0f, 0.0f};
+  for (int v = v0 + gt; v < v1; v += W * 32) {
+    float o[E];
+    tok_group(x, ph, V, v, o);
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const float q = (o[k] - m) * LOG2E, e = exp2_of(q);
+      s.z += e;
+      s.u = fmaf(e, fmaxf(q, -1e4f), s.u);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { s.z += __shfl_xor_sync(0xffffffffu, s.z, o); s.u += __shfl_xor_sync(0xffffffffu, s.u, o); }
+  return s;
+}
+// d = p (f + h ln p) with ln p = (x - m) - log_z, `hit` added at t.
+template <typename T, typename O, int W>
+__device__ __noinline__ void far_write(const T* x, O* d, int j0, int j1, float m, float log_z, float f, float h, int t, float hit, int gt) {
+  for (int j = j0 + gt; j < j1; j += W * 32) {
+    const float lp = (to_f32(x[j]) - m) - log_z, v = exp_of(lp) * (f + h * fmaxf(lp, -1e4f));
+    d[j] = from_f32<O>(j == t ? v + hit : v);
+  }
+}
+template <typename O, int W>
+__device__ __noinline__ void zero_write(O* d, int j0, int j1, int gt) {
+  constexpr int N = 16 / (int)sizeof(O);
+  const int first = min(j1, j0 + (int)((N - (uintptr_t)(d + j0) / sizeof(O)) & (N - 1))), last = first + (max(j1 - first, 0) & ~(N - 1));
+  if (gt < first - j0) d[j0 + gt] = from_f32<O>(0.0f);
+  for (int j = first + gt * N; j < last; j += W * 32 * N) *reinterpret_cast<uint4*>(d + j) = make_uint4(0, 0, 0, 0);
+  if (gt < j1 - last) d[last + gt] = from_f32<O>(0.0f);
+}
+
+template <typename T, typename O, int MODE, int W, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constant__ TokDev a) {
-  constexpr int E = TokVec<T>::E, GT = GW * 32, NG = NT / GT, CAP = TokShared<GW>::CAP;
+  constexpr int E = TokVec<T>::E, GT = W * 32, NG = NT / GT, CAP = TokShared<W>::CAP;
   constexpr bool TOP = MODE == TOK_TOP, ENT = MODE == TOK_ENTROPY || MODE == TOK_TOP, FWD = MODE <= TOK_TOP;
+  static_assert(W == 1 || NG == 1, "a CTA takes one row, or a row a warp");
   const float ninf = __int_as_float(0xff800000);
   extern __shared__ __align__(16) unsigned char tok_smem[];
-  __shared__ TokShared<GW> s_all[NG];
-  __shared__ TokPeers s_peers;
+  __shared__ TokShared<W> s_all[TOP ? NG : 1];
+  __shared__ TokPeers<TOP> s_peers;
+  static_assert(W <= 4, "a lane for each warp of a cluster");
   const int grp = threadIdx.x / GT, gt = threadIdx.x % GT, lane = threadIdx.x & 31, warp = gt >> 5;
-  TokShared<GW>& s = s_all[grp];
+  TokShared<W>& s = s_all[TOP ? grp : 0];
   int C = 1, rank = 0;
-  if (GW > 1) {
+  if (W > 1) {
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(C));
     rank = (int)cluster_ctarank();
   }
-  uint4* const bufs = reinterpret_cast<uint4*>(tok_smem) + (size_t)grp * a.stages * a.per;
-  unsigned long long* const cand = reinterpret_cast<unsigned long long*>(tok_smem + (size_t)NG * a.stages * a.per * 16) + (size_t)grp * (CAP + ONO_TOP_MAX);
+  uint4* const kept = reinterpret_cast<uint4*>(tok_smem) + (size_t)grp * a.per;      // (staged)
+  unsigned long long* const cand = reinterpret_cast<unsigned long long*>(tok_smem) + (size_t)grp * (CAP + ONO_TOP_MAX);      // (TOP)
   unsigned long long* const list = cand + CAP;
   const long long stride = (long long)(gridDim.x / C) * NG;
   const int K = TOP ? a.top : 1;
-
+  auto sync_row = [&]() {      // all that share the row
+    if (W == 1) __syncwarp();
+    else if (C == 1) __syncthreads();
+    else cluster_sync_all();
+  };
   auto raw_target = [&](long long r) -> long long {
     if (!a.targets) return 0;
     if (r >= a.R) return a.ignore_id;
@@ -212,46 +331,55 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
     if (a.status && gt == 0) atomicExch(a.status, ONO_ERR_BAD_ARG);
     return -1;
   };
-  auto phase_of = [&](const T* x) { return (int)(((uintptr_t)x / sizeof(T)) & (E - 1)); };
-  auto load = [&](long long r, uint4* buf) {
-    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ld;
-    const int ph = phase_of(x), nv = (ph + a.V + E - 1) / E, v0 = rank * a.per, v1 = min(nv, v0 + a.per);
-    for (int v = v0 + gt; v < v1; v += GT) {
-      if (v * E >= ph && (v + 1) * E <= ph + a.V) {
-        cp_async16(buf + (v - v0), x + (v * E - ph));
-      } else {      // an end of the row: -inf beyond it
-        T* o = reinterpret_cast<T*>(buf + (v - v0));
-#pragma unroll
-        for (int k = 0; k < E; ++k) { const int j = v * E + k - ph; o[k] = j >= 0 && j < a.V ? x[j] : TokVec<T>::ninf(); }
-      }
-    }
+
+  const bool staged = MODE == TOK_LOSS && a.staged;
+  // A row that is kept: on its way into shared memory from when the one before it has left. A thread fetches what it will read itself.
+  auto fetch = [&](long long r) {
+    const T* const x = reinterpret_cast<const T*>(a.x) + r * a.ld;
+    const int ph = (int)(((uintptr_t)x / sizeof(T)) & (E - 1)), va = max(rank * a.per, ph ? 1 : 0), vb = min(rank * a.per + a.per, (ph + a.V) / E);
+    const T* src = x + ((va + gt) * E - ph);
+    uint4* dst = kept + gt;
+#pragma unroll 4
+    for (int v = va + gt; v < vb; v += GT, src += GT * E, dst += GT) cp_async16(dst, src);
   };
-  // f(value) of every logit of the CTA's share to the output, g(value, result) where the target is
-  auto write = [&](long long r, const uint4* buf, int t, auto f, auto g) {
-    const T* x = reinterpret_cast<const T*>(a.x) + r * a.ld;
-    O* d = reinterpret_cast<O*>(a.out) + r * a.ld_out;
-    const int ph = phase_of(x), nv = (ph + a.V + E - 1) / E, v0 = rank * a.per, v1 = min(nv, v0 + a.per);
-    if ((((uintptr_t)d / sizeof(O) - ph) & (E - 1)) == 0) {
-      const int vt = t < 0 ? -1 : (t + ph) / E;
-      for (int v = v0 + gt; v < v1; v += GT) {
-        float w[E];
-        if (buf) {
-          TokVec<T>::get(buf[v - v0], w);
-          float q[E];
+
+  if (W > 1 && C > 1) cluster_sync_all();      // every CTA of the cluster runs: its shared memory may be written to
+  long long r = (long long)(blockIdx.x / C) * NG + grp;
+  long long raw_next = raw_target(r);
+  if (staged && r < a.R && target(raw_next) >= 0) fetch(r);
+  int live = 0;
+  for (; r < a.R; r += stride) {
+    const int t = target(raw_next);
+    raw_next = raw_target(r + stride);
+    const T* const x = reinterpret_cast<const T*>(a.x) + r * a.ld;
+    // The row in groups of 16 bytes: whole ones from va to vb are this CTA's, and of the first and last one, if they are not whole, a logit a thread.
+    const int ph = (int)(((uintptr_t)x / sizeof(T)) & (E - 1)), nv = (ph + a.V + E - 1) / E, v0 = rank * a.per, v1 = min(nv, v0 + a.per);
+    const int va = max(v0, ph ? 1 : 0), vb = min(v1, (ph + a.V) / E);
+    const int jh = gt - ph, jt = (nv - 1) * E + gt - ph;
+    const bool has_h = gt < E && v0 == 0 && ph && jh >= 0 && jh < a.V, has_t = gt < E && nv - 1 >= v0 && nv - 1 < v1 && nv - 1 >= vb && (nv > 1 || !ph) && jt < a.V;
+    O* const d = FWD ? nullptr : reinterpret_cast<O*>(a.out) + r * a.ld_out;
+    const int j0 = max(v0 * E - ph, 0), j1 = min(v1 * E - ph, a.V);      // the CTA's logits
+    // f(two logits) of them to the output, `hit` added where the target is
+    auto write = [&](float xh, float xt, float hit, auto f) {
+      auto one = [&](int j, float v) {
+        float q = f(make_float2(v, v)).x;
+        if (j == t) q += hit;
+        d[j] = from_f32<O>(q);
+      };
+      if (has_h) one(jh, xh);
+      if (has_t) one(jt, xt);
+      if ((((uintptr_t)d / sizeof(O) - ph) & (E - 1)) == 0) {
+        const int vt = t < 0 ? -1 : (t + ph) / E;
+        auto put = [&](int v, const uint4& w4) {
+          float w[E];
+          TokVec<T>::get(w4, w);
 #pragma unroll
-          for (int k = 0; k < E; ++k) q[k] = f(w[k]);
+          for (int k = 0; k < E; k += 2) { const float2 p = f(make_float2(w[k], w[k + 1])); w[k] = p.x; w[k + 1] = p.y; }
           if (v == vt) {
 #pragma unroll
-            for (int k = 0; k < E; ++k) if (v * E + k - ph == t) q[k] = g(w[k], q[k]);
+            for (int k = 0; k < E; ++k) if (v * E + k - ph == t) w[k] += hit;
           }
-#pragma unroll
-          for (int k = 0; k < E; ++k) w[k] = q[k];
-        } else {
-#pragma unroll
-          for (int k = 0; k < E; ++k) w[k] = 0.0f;
-        }
-        O* o = d + (v * E - ph);
-        if (v * E >= ph && (v + 1) * E <= ph + a.V) {
+          O* o = d + (v * E - ph);
           if constexpr (sizeof(O) == 4) {
 #pragma unroll
             for (int k = 0; k < E; k += 4) *reinterpret_cast<float4*>(o + k) = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
@@ -265,204 +393,217 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
             if constexpr (E == 4) *reinterpret_cast<uint2*>(o) = make_uint2(u[0], u[1]);
             else *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[E / 2 - 2], u[E / 2 - 1]);
           }
-        } else {
+        };
+        int v = va + gt;
+        for (; v + 3 * GT < vb; v += 4 * GT) {
+          uint4 w4[4];
 #pragma unroll
-          for (int k = 0; k < E; ++k) { const int j = v * E + k - ph; if (j >= 0 && j < a.V) o[k] = from_f32<O>(w[k]); }
+          for (int q = 0; q < 4; ++q) w4[q] = staged ? kept[v + q * GT - va] : load16(x + ((v + q * GT) * E - ph));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) put(v + q * GT, w4[q]);
         }
+        if (v < vb) {
+          uint4 w4[3];
+#pragma unroll
+          for (int q = 0; q < 3; ++q) if (v + q * GT < vb) w4[q] = staged ? kept[v + q * GT - va] : load16(x + ((v + q * GT) * E - ph));
+#pragma unroll
+          for (int q = 0; q < 3; ++q) if (v + q * GT < vb) put(v + q * GT, w4[q]);
+        }
+      } else {      // the output's rows are aligned another way: value by value
+        group_sync<W>();      // (here a thread reads what others have kept)
+        for (int i = va * E + gt; i < vb * E; i += GT) one(i - ph, to_f32(staged ? reinterpret_cast<const T*>(kept)[i - va * E] : x[i - ph]));
+        group_sync<W>();
       }
-    } else {      // the output's rows are aligned another way: value by value
-      const T* b = reinterpret_cast<const T*>(buf);
-      for (int i = max(v0 * E, ph) + gt; i < min(v1 * E, ph + a.V); i += GT) {
-        float q = 0.0f;
-        if (buf) { const float w = to_f32(b[i - v0 * E]); q = f(w); if (i - ph == t) q = g(w, q); }
-        d[i - ph] = from_f32<O>(q);
-      }
-    }
-  };
-
-  if (GW > 1 && C > 1) cluster_sync_all();      // every CTA of the cluster runs: its shared memory may be written to
-  long long r = (long long)(blockIdx.x / C) * NG + grp;
-  int t = target(raw_target(r)), t_next = target(raw_target(r + stride));
-  int it = 0, live = 0;
-  if (t >= 0 && r < a.R) load(r, bufs);
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  float x_t = 0.0f, in0 = 0.0f, in1 = 0.0f, in2 = 0.0f, in3 = 0.0f;
-  auto inputs = [&](long long q, int tq) {
-    if (tq < 0 || q >= a.R) return;
-    if ((FWD || MODE == TOK_LOSS) && gt == 0) x_t = to_f32(reinterpret_cast<const T*>(a.x)[q * a.ld + tq]);
-    if (MODE == TOK_LOSS) in0 = a.weight ? __ldg(a.weight + q) : 1.0f;
-    if (MODE == TOK_GRAD) {
-      in0 = __ldg(a.lse_in + q);
-      in1 = a.d_logp ? __ldg(a.d_logp + q) : 0.0f;
-      if (a.d_entropy) { in2 = __ldg(a.d_entropy + q); in3 = __ldg(a.entropy_in + q); }
-    }
-  };
-  inputs(r, t);
-  for (; r < a.R; r += stride, ++it) {
-    const long long raw_after = raw_target(r + 2 * stride);
-    const uint4* buf = bufs + (a.stages == 2 ? (size_t)(it & 1) * a.per : 0);
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    group_sync<GW>();
-    const float my_xt = x_t, i0 = in0, i1 = in1, i2 = in2, i3 = in3;
-    if (a.stages == 2) {
-      if (t_next >= 0 && r + stride < a.R) load(r + stride, bufs + (size_t)((it + 1) & 1) * a.per);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    inputs(r + stride, t_next);
+    };
     if (t < 0) {
-      if (rank == 0) {
-        if (FWD || MODE == TOK_LOSS) {
-          if (gt == 0) {
-            if (a.logp) a.logp[r] = 0.0f;
-            if (a.lse) a.lse[r] = 0.0f;
-            if (ENT && a.entropy) a.entropy[r] = 0.0f;
+      if (rank == 0 && MODE != TOK_GRAD) {
+        if (gt == 0) {
+          if (a.logp) a.logp[r] = 0.0f;
+          if (a.lse) a.lse[r] = 0.0f;
+          if (ENT && a.entropy) a.entropy[r] = 0.0f;
+        }
+        if (TOP && gt < K) { a.top_logp[r * K + gt] = ninf; a.top_id[r * K + gt] = -1; }
+      }
+      if (!FWD) zero_write<O, W>(d, j0, j1, gt);
+      if (staged && r + stride < a.R && target(raw_next) >= 0) fetch(r + stride);
+      continue;
+    }
+    float x_t = 0.0f, i0 = 1.0f, i1 = 0.0f, i2 = 0.0f, i3 = 0.0f;
+    if (MODE != TOK_GRAD && gt == 0 && a.targets) x_t = to_f32(x[t]);
+    if (MODE == TOK_LOSS && a.weight) i0 = __ldg(a.weight + r);
+    if (MODE == TOK_GRAD) {
+      i0 = __ldg(a.lse_in + r);
+      if (a.d_logp) i1 = __ldg(a.d_logp + r);
+      if (a.d_entropy) { i2 = __ldg(a.d_entropy + r); i3 = __ldg(a.entropy_in + r); }
+    }
+    const float xh = has_h ? to_f32(x[jh]) : ninf, xt = has_t ? to_f32(x[jt]) : ninf;
+    TokSums g = {0.0f, 1.0f, 0.0f};
+    float log_z = 0.0f;      // ln of the row's sum relative to its maximum
+    bool far = false;
+    if (MODE != TOK_GRAD || fabsf(i0) > LSE_EXACT) {
+      TokSums mine = {ninf, 0.0f, 0.0f};
+      float2 z2[2] = {both(0.0f), both(0.0f)}, u2[2] = {both(0.0f), both(0.0f)};
+      float shift = 0.0f;
+      if (staged) asm volatile("cp.async.wait_all;" ::: "memory");
+      auto raise = [&](float m) {
+        if (m > mine.m) {
+          const float to = shift_of(m), by = mine.m < -TOK_FAR ? 0.0f : shift - to;      // (what was too far below has left nothing)
+          const float2 f = both(exp2_of(by));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (ENT) u2[k] = mul_2(f, fma_2(both(fmaxf(by, -1e4f)), z2[k], u2[k]));
+            z2[k] = mul_2(z2[k], f);
           }
-          if (TOP && gt < K) { a.top_logp[r * K + gt] = ninf; a.top_id[r * K + gt] = -1; }
+          mine.m = m;
+          shift = to;
+        }
+      };
+      auto take = [&](int k, float2 v) {
+        const float2 q = fma_2(v, both(LOG2E), both(-shift)), e = make_float2(exp2_of(q.x), exp2_of(q.y));
+        z2[k] = add_2(z2[k], e);
+        if (ENT) u2[k] = fma_2(e, make_float2(fmaxf(q.x, -1e4f), fmaxf(q.y, -1e4f)), u2[k]);
+      };
+      auto take4 = [&](const uint4& w) {
+        float o[E];
+        TokVec<T>::get(w, o);
+#pragma unroll
+        for (int k = 0; k < E; k += 2) take(k / 2 % 2, make_float2(o[k], o[k + 1]));
+      };
+      int v = va + gt;
+      for (; v + 3 * GT < vb; v += 4 * GT) {
+        uint4 w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = staged ? kept[v + q * GT - va] : load16(x + ((v + q * GT) * E - ph));
+        raise(TokVec<T>::most(w));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) take4(w[q]);
+      }
+      if (v < vb) {
+        uint4 w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          w[q] = make_uint4(TokVec<T>::NINF, TokVec<T>::NINF, TokVec<T>::NINF, TokVec<T>::NINF);
+          if (q < 3 && v + q * GT < vb) w[q] = staged ? kept[v + q * GT - va] : load16(x + ((v + q * GT) * E - ph));
+        }
+        raise(TokVec<T>::most(w));
+#pragma unroll
+        for (int q = 0; q < 3; ++q) if (v + q * GT < vb) take4(w[q]);
+      }
+      if (has_h || has_t) {
+        raise(fmaxf(xh, xt));
+        take(0, make_float2(xh, xt));
+      }
+      z2[0] = add_2(z2[0], z2[1]);
+      mine.z = z2[0].x + z2[0].y;
+      if (ENT) { u2[0] = add_2(u2[0], u2[1]); mine.u = u2[0].x + u2[0].y; }
+      const float tm = mine.m;
+      float cut = ninf;
+      if (TOP) {
+        // the warp's J-th largest of its lanes' maxima; the smallest of the warps' bounds: W * J >= K logits are not below it
+        unsigned int rest = order_of(tm), best = __reduce_max_sync(0xffffffffu, rest);
+        for (int q = 1; q < (K + W - 1) / W; ++q) {
+          const unsigned int who = __ballot_sync(0xffffffffu, rest == best);
+          if (lane == __ffs(who) - 1) rest = 0;
+          best = __reduce_max_sync(0xffffffffu, rest);
+        }
+        cut = best ? of_order(best) : ninf;
+        if (gt == 0) s.count = s.threads = 0;
+        if (gt < K) list[gt] = 0;
+      }
+      g = tok_join<ENT>(mine);
+      const int par = live & 1, lead = live % C;
+      const float4* const part = s_peers.part[par];
+      if (W > 1) {
+        const float4 told = make_float4(g.m, g.z, g.u, cut);
+        if (C == 1) { if (lane == 0) s_peers.part[par][warp] = told; }
+        else if (lane < C) st_cluster_v4(mapa_shared(smem_u32(&s_peers.part[par][rank * W + warp]), (uint32_t)lane), told);
+        sync_row();
+        auto of = [&](int i) { return i < C * W ? TokSums{part[i].x, part[i].y, part[i].z} : TokSums{ninf, 0.0f, 0.0f}; };
+        g = tok_join<ENT>(of(lane));
+        if (TOP) {
+#pragma unroll
+          for (int w = 0; w < W; ++w) { const float c = part[rank * W + w].w; cut = w ? fminf(cut, c) : c; }
         }
       }
-      if (!FWD) write(r, nullptr, -1, [](float) { return 0.0f; }, [](float, float q) { return q; });
-    } else {
-      const T* x = reinterpret_cast<const T*>(a.x) + r * a.ld;
-      const int ph = phase_of(x), v0 = rank * a.per, n = min((ph + a.V + E - 1) / E - v0, a.per);
-      float m = 0.0f, z = 1.0f, u = 0.0f, log_z = 0.0f;
-      const bool sums = MODE != TOK_GRAD || fabsf(i0) > LSE_EXACT;
-      if (sums) {
-        // the maximum; for the alternatives a bound that at least K logits reach
-        float tm = ninf;
-        if constexpr (E == 8) {
-          __nv_bfloat162 m2 = __halves2bfloat162(TokVec<T>::ninf(), TokVec<T>::ninf());
-          for (int v = gt; v < n; v += GT) {
-            const uint4 w = buf[v];
-            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-            m2 = __hmax2(m2, __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+      if (TOP && W == 1) __syncwarp();
+      far = fabsf(g.m) > TOK_FAR && g.m > ninf;
+      if (far) {
+        // logits of a size that log2 e takes out of f32: differences first. (A second exchange, by all that share the row.)
+        mine = far_sums<T, W>(x, ph, a.V, v0, v1, g.m, gt);
+        if (W > 1) {
+          sync_row();      // the first sums have been read
+          const float4 told = make_float4(0.0f, mine.z, mine.u, 0.0f);
+          if (C == 1) { if (lane == 0) s_peers.part[par][warp] = told; }
+          else if (lane < C) st_cluster_v4(mapa_shared(smem_u32(&s_peers.part[par][rank * W + warp]), (uint32_t)lane), told);
+          sync_row();
+          mine.z = mine.u = 0.0f;
+          for (int i = 0; i < C * W; ++i) { mine.z += part[i].y; mine.u += part[i].z; }
+        }
+        g.z = mine.z;
+        g.u = mine.u;
+      }
+      const bool empty = g.z == 0.0f;
+      const float log2_z = empty ? 0.0f : log2f(g.z), at = shift_of(g.m);
+      // (the sum is relative to the shift, which is the maximum times log2 e rounded)
+      log_z = (fabsf(g.m) <= TOK_FAR ? log2_z - fmaf(g.m, LOG2E, -at) : log2_z) * LN2;
+      // ln p of a logit
+      auto lp = [&](float v) { return far || fabsf(v) > TOK_FAR ? (v - g.m) - log_z : (fmaf(v, LOG2E, -at) - log2_z) * LN2; };
+      if (MODE != TOK_GRAD && gt == 0 && rank == 0) {
+        if (a.lse) a.lse[r] = empty ? ninf : far ? g.m + log_z : (at + log2_z) * LN2;
+        if (a.logp) a.logp[r] = empty ? ninf : lp(x_t);
+        if (ENT && a.entropy) a.entropy[r] = empty ? 0.0f : (log2_z - g.u / g.z) * LN2;
+      }
+      if (TOP) {
+        auto offer = [&](float v, int j) {
+          if (v >= cut && v > ninf) {
+            const unsigned int at_c = atomicAdd(&s.count, 1u);
+            if (at_c < CAP) cand[at_c] = top_key(v, j);
           }
-          tm = fmaxf(__low2float(m2), __high2float(m2));
+        };
+        // the threads that have seen a logit that reaches the bound; what they have seen is read again, by all
+        if (tm >= cut && tm > ninf) s.who[atomicAdd(&s.threads, 1u)] = (unsigned short)gt;
+        group_sync<W>();
+        const int each = (vb - va + GT - 1) / GT, items = max(0, each) * (int)s.threads;
+        for (int i = gt; i < items; i += GT) {
+          const int v = va + s.who[i / each] + i % each * GT;
+          if (v < vb) {
+            float o[E];
+            TokVec<T>::get(load16(x + (v * E - ph)), o);
+#pragma unroll
+            for (int k = 0; k < E; ++k) offer(o[k], v * E + k - ph);
+          }
+        }
+        if (has_h) offer(xh, jh);
+        if (has_t) offer(xt, jt);
+        group_sync<W>();
+        int have = (int)s.count;
+        if (have > CAP) {
+          group_sync<W>();
+          exact_candidates<T, W>(x, ph, a.V, v0, v1, K, cand, s, gt);
+          have = (int)s.count;
+        }
+        for (int i = gt; i < have; i += GT) {
+          const unsigned long long key = cand[i];
+          int above = 0;
+          for (int q = 0; q < have; ++q) above += cand[q] > key;
+          if (above < K) list[above] = key;
+        }
+        group_sync<W>();
+        auto put = [&](int k, unsigned long long key) {
+          a.top_logp[r * K + k] = key ? lp(of_order((unsigned int)(key >> 32))) : ninf;
+          a.top_id[r * K + k] = key ? (int)(0xffffffffu - (unsigned int)key) : -1;
+        };
+        if (W == 1 || C == 1) {
+          if (gt < K) put(gt, list[gt]);
+          group_sync<W>();
         } else {
-          for (int v = gt; v < n; v += GT) {
-            float w[E];
-            TokVec<T>::get(buf[v], w);
-#pragma unroll
-            for (int k = 0; k < E; ++k) tm = fmaxf(tm, w[k]);
+          if (gt < K) {
+            const uint32_t to = mapa_shared(smem_u32(&s_peers.key[par][rank][gt]), (uint32_t)lead);
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(list[gt]) : "memory");
           }
-        }
-        const unsigned int mine = order_of(tm);
-        unsigned int wm = __reduce_max_sync(0xffffffffu, mine), cut = wm;
-        if (TOP) {
-          // every warp's J-th largest of its lanes' maxima; the smallest of these: GW * J >= K logits are not below it
-          unsigned int rest = mine;
-          for (int q = 1; q < (K + GW - 1) / GW; ++q) {
-            const unsigned int who = __ballot_sync(0xffffffffu, rest == cut);
-            if (lane == __ffs(who) - 1) rest = 0;
-            cut = __reduce_max_sync(0xffffffffu, rest);
-          }
-        }
-        m = of_order(wm);
-        if (GW > 1) {
-          if (lane == 0) { s.top[warp] = m; s.cut[warp] = cut; }
-          if (TOP && gt == 0) s.count = 0;
-          if (TOP && gt < K) list[gt] = 0;
-          __syncthreads();
-#pragma unroll
-          for (int w = 0; w < GW; ++w) { m = fmaxf(m, s.top[w]); if (TOP) cut = min(cut, s.cut[w]); }
-        } else if (TOP) {
-          if (gt == 0) s.count = 0;
-          if (gt < K) list[gt] = 0;
-          __syncwarp();
-        }
-        const float base = m == ninf ? 0.0f : m;      // (a row of -inf alone sums to zero, one with NaN to NaN)
-        for (int careful = 0; careful < 2; ++careful) {
-          z = u = 0.0f;
-          for (int v = gt; v < n; v += GT) {
-            float w[E];
-            TokVec<T>::get(buf[v], w);
-            float e[E];
-#pragma unroll
-            for (int k = 0; k < E; ++k) { w[k] -= base; e[k] = exp_of(w[k]); }
-#pragma unroll
-            for (int k = 0; k < E; ++k) z += e[k];
-            if (ENT) {
-#pragma unroll
-              for (int k = 0; k < E; ++k) u = fmaf(e[k], careful ? fmaxf(w[k], -1e4f) : w[k], u);
-            }
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) { z += __shfl_xor_sync(0xffffffffu, z, o); if (ENT) u += __shfl_xor_sync(0xffffffffu, u, o); }
-          if (GW > 1) {
-            if (careful) __syncthreads();
-            if (lane == 0) s.sum[warp] = make_float2(z, u);
-            __syncthreads();
-            z = u = 0.0f;
-#pragma unroll
-            for (int w = 0; w < GW; ++w) { z += s.sum[w].x; u += s.sum[w].y; }
-          }
-          if (!ENT || u == u || z != z) break;      // zero times -inf among the terms: once more, with zero times a number
-        }
-        if (TOP) {
-          const float bound = of_order(cut);
-          if (tm >= bound && tm > ninf) {
-            for (int v = gt; v < n; v += GT) {
-              float w[E];
-              TokVec<T>::get(buf[v], w);
-#pragma unroll
-              for (int k = 0; k < E; ++k)
-                if (w[k] >= bound && w[k] > ninf) {
-                  const unsigned int at = atomicAdd(&s.count, 1u);
-                  if (at < CAP) cand[at] = top_key(w[k], (v0 + v) * E + k - ph);
-                }
-            }
-          }
-          group_sync<GW>();
-          int have = (int)s.count;
-          if (have > CAP) {
-            group_sync<GW>();
-            exact_candidates<T, GW>(buf, n, v0, ph, K, cand, s, gt);
-            have = (int)s.count;
-          }
-          for (int i = gt; i < have; i += GT) {
-            const unsigned long long key = cand[i];
-            int above = 0;
-            for (int q = 0; q < have; ++q) above += cand[q] > key;
-            if (above < K) list[above] = key;
-          }
-          group_sync<GW>();
-        }
-        const int lead = GW > 1 ? live % C : 0;
-        if (GW > 1 && C > 1) {
-          const int par = live & 1;
-          if (gt < C) st_cluster_v4(mapa_shared(smem_u32(&s_peers.part[par][rank]), (uint32_t)gt), make_float4(m, z, u, 0.0f));
-          if (TOP && gt < K)
-            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&s_peers.key[par][rank][gt]), (uint32_t)lead)), "l"(list[gt]) : "memory");
           cluster_sync_all();
-          m = ninf;
-          for (int q = 0; q < C; ++q) m = fmaxf(m, s_peers.part[par][q].x);
-          z = u = 0.0f;
-          for (int q = 0; q < C; ++q) {
-            const float4 w = s_peers.part[par][q];
-            if (w.y == 0.0f) continue;
-            const float f = exp_of(w.x - m);
-            z = fmaf(w.y, f, z);
-            u += f * (w.z + fmaxf(w.x - m, -1e4f) * w.y);      // (zero times a number, far below)
-          }
-        }
-        const bool empty = z == 0.0f;
-        log_z = empty ? 0.0f : logf(z);
-        if ((FWD || MODE == TOK_LOSS) && gt == 0 && rank == 0) {
-          if (a.lse) a.lse[r] = empty ? ninf : m + log_z;
-          if (a.logp) a.logp[r] = empty ? ninf : (my_xt - m) - log_z;
-          if (ENT && a.entropy) a.entropy[r] = empty ? 0.0f : log_z - u / z;
-        }
-        if (TOP && rank == lead) {
-          float* tl = a.top_logp + r * K;
-          int* ti = a.top_id + r * K;
-          auto put = [&](int k, unsigned long long key) {
-            tl[k] = key ? (of_order((unsigned int)(key >> 32)) - m) - log_z : ninf;
-            ti[k] = key ? (int)(0xffffffffu - (unsigned int)key) : -1;
-          };
-          if (GW == 1 || C == 1) {
-            if (gt < K) put(gt, list[gt]);
-          } else {
-            const unsigned long long(*keys)[ONO_TOP_MAX] = s_peers.key[live & 1];
-            int there = 0;
+          if (rank == lead) {
+            const unsigned long long(*keys)[ONO_TOP_MAX] = s_peers.key[par];
             for (int i = gt; i < C * K; i += GT) {
               const unsigned long long key = keys[i / K][i % K];
               int above = 0;
@@ -471,73 +612,74 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
               if (key && above < K) put(above, key);
             }
             if (gt < K) {
+              int there = 0;
               for (int q = 0; q < C; ++q) for (int k = 0; k < K; ++k) there += keys[q][k] != 0;
               if (gt >= there) put(gt, 0);
             }
           }
         }
-        ++live;
       }
-      if (MODE == TOK_LOSS) {
-        const bool empty = z == 0.0f;
-        const float base = empty ? 0.0f : m, w = a.scale * i0, f = empty ? 0.0f : w / z;
-        write(r, empty ? nullptr : buf, t, [&](float v) { return exp_of(v - base) * f; }, [&](float, float q) { return q - w; });
+      ++live;
+      if (W == 1) __syncwarp();      // (out may be x: what was wanted of the row has been read; a CTA has met above)
+    }
+    const bool empty = MODE == TOK_GRAD ? i0 == ninf : g.z == 0.0f;
+    if (!FWD && empty) {
+      zero_write<O, W>(d, j0, j1, gt);
+    } else if (MODE == TOK_LOSS) {
+      const float w = a.scale * i0;
+      if (far) {
+        far_write<T, O, W>(x, d, j0, j1, g.m, log_z, w, 0.0f, t, -w, gt);
+      } else {
+        const float2 off = both(-shift_of(g.m)), fs = both(w / g.z);
+        write(xh, xt, -w, [&](float2 v) { const float2 q = fma_2(v, both(LOG2E), off); return mul_2(make_float2(exp2_of(q.x), exp2_of(q.y)), fs); });
       }
-      if (MODE == TOK_GRAD) {
-        if (!sums) log_z = i0;
-        if (!sums) m = 0.0f;
-        const bool empty = i0 == ninf;
+    } else if (MODE == TOK_GRAD) {
+      if (fabsf(i0) <= LSE_EXACT) {
+        // -p (g + h (ln p + H)) with ln p = ln 2 (q - off): q = x log2 e - c, c the product lse log2 e rounded, off what that took off
+        const float c = i0 * LOG2E, off = fmaf(i0, LOG2E, -c), f = -exp2_of(-off);
+        const float2 at = both(-c), A = both(f * (i1 + i2 * (i3 - LN2 * off))), B = both(f * LN2 * i2);
         if (a.d_entropy)
-          write(r, empty ? nullptr : buf, t,
-                [&](float v) { const float lp = (v - m) - log_z; return -exp_of(lp) * (i1 + i2 * (fmaxf(lp, -1e4f) + i3)); }, [&](float, float q) { return q + i1; });
+          write(xh, xt, i1, [&](float2 v) {
+            float2 q = fma_2(v, both(LOG2E), at);
+            q = make_float2(fmaxf(q.x, -1e4f), fmaxf(q.y, -1e4f));      // (zero times a number; no NaN comes here)
+            return mul_2(make_float2(exp2_of(q.x), exp2_of(q.y)), fma_2(q, B, A));
+          });
         else
-          write(r, empty ? nullptr : buf, t, [&](float v) { return -exp_of((v - m) - log_z) * i1; }, [&](float, float q) { return q + i1; });
+          write(xh, xt, i1, [&](float2 v) { const float2 q = fma_2(v, both(LOG2E), at); return mul_2(make_float2(exp2_of(q.x), exp2_of(q.y)), A); });
+      } else {      // as for a NaN, which is in lse then
+        far_write<T, O, W>(x, d, j0, j1, isnan(i0) ? i0 : g.m, log_z, -(i1 + i2 * i3), -i2, t, i1, gt);
       }
     }
-    if (a.stages == 1) {
-      group_sync<GW>();      // the row has been read by all
-      if (t_next >= 0 && r + stride < a.R) load(r + stride, bufs);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    t = t_next;
-    t_next = target(raw_after);
+    if (staged && r + stride < a.R && target(raw_next) >= 0) fetch(r + stride);
   }
 }
 
 // How a launch is laid out.
-struct TokShape { int warps, ctas, per, stages; size_t smem; };
+struct TokShape { int warps, ctas, per, staged; size_t smem; };
 
-constexpr int TOK_WARP_ROW = 4096, TOK_SMALL_ROW = 16384, TOK_SLICE = 32768, TOK_SMEM = 225 * 1024;
+constexpr int TOK_WARP_ROW = 8192, TOK_SLICE = 32768;
 
-static TokShape tok_shape(long long rows, int V, int esz, bool top) {
+static TokShape tok_shape(long long rows, int V, int esz, int mode) {
   const int E = 16 / esz;
   const long long groups = ((long long)V + 2 * E - 2) / E, bytes = groups * 16;      // of a row that begins anywhere
   TokShape s = {};
-  auto smem = [&](int warps, int groups_in_cta) {
-    const size_t cand = top ? (size_t)(8 * ((warps == 1 ? 256 : 512) + ONO_TOP_MAX)) * groups_in_cta : 0;
-    return (size_t)s.per * 16 * s.stages * groups_in_cta + cand;
-  };
   s.ctas = 1;
-  s.stages = 2;
-  if (bytes <= TOK_WARP_ROW) {
-    s.warps = 1;
-    s.per = (int)groups;
-    s.smem = smem(1, 4);
-    return s;
+  s.warps = bytes <= TOK_WARP_ROW ? 1 : 4;
+  if (s.warps > 1) {
+    while (s.ctas < TOK_CTAS && ((mode == TOK_LOSS && bytes > (long long)TOK_SLICE * s.ctas) || (rows * s.ctas * 2 <= ono_num_sms() && bytes > 4096ll * s.ctas))) s.ctas *= 2;
   }
-  s.warps = bytes <= TOK_SMALL_ROW ? 4 : 8;
-  while (s.ctas < TOK_CTAS && (bytes > (long long)TOK_SLICE * s.ctas || (rows * s.ctas * 2 <= ono_num_sms() && bytes > 4096ll * s.ctas))) s.ctas *= 2;
-  if (s.ctas > 1) s.warps = 8;
   s.per = (int)((groups + s.ctas - 1) / s.ctas);
-  if (s.per * 16 > TOK_SLICE) s.stages = 1;
-  s.smem = smem(s.warps, 1);
+  const int rows_of_cta = s.warps == 1 ? 4 : 1;
+  s.staged = mode == TOK_LOSS && s.per * 16 <= 100 * 1024;
+  if (s.staged) s.smem = (size_t)s.per * 16 * rows_of_cta;
+  if (mode == TOK_TOP) s.smem = (size_t)(8 * ((s.warps == 1 ? 256 : 512) + ONO_TOP_MAX)) * rows_of_cta;
   return s;
 }
 
 template <typename T, typename O, int MODE, int GW, int NT>
 static cudaError_t tok_go(const TokDev& d, const TokShape& s, cudaStream_t st) {
   auto kern = tok_kernel<T, O, MODE, GW, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.smem);
+  cudaError_t e = s.smem > 32768 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.smem) : cudaSuccess;
   if (e != cudaSuccess) return e;
   const long long units = (d.R + NT / (GW * 32) - 1) / (NT / (GW * 32));      // of a CTA, or a cluster
   cudaLaunchConfig_t cfg = {};
@@ -554,7 +696,7 @@ static cudaError_t tok_go(const TokDev& d, const TokShape& s, cudaStream_t st) {
   static std::atomic<unsigned long long> known[4];
   std::atomic<unsigned long long>& k = known[s.ctas == 8 ? 3 : s.ctas >> 1];
   unsigned long long v = k.load();
-  if ((v >> 16) != s.smem) {
+  if (v == 0 || (v >> 16) != s.smem) {
     int resident = 0;
     if ((e = cudaOccupancyMaxActiveClusters(&resident, kern, &cfg)) != cudaSuccess) return e;
     v = (unsigned long long)s.smem << 16 | (unsigned)std::max(1, std::min(resident, 65535));
@@ -566,11 +708,10 @@ static cudaError_t tok_go(const TokDev& d, const TokShape& s, cudaStream_t st) {
 
 template <typename T, typename O, int MODE>
 static int tok_run(TokDev& d, cudaStream_t st) {
-  const TokShape s = tok_shape(d.R, d.V, sizeof(T), MODE == TOK_TOP);
-  if (s.smem > (size_t)TOK_SMEM) { set_error("tokens: a row of %s%lld logits is more than a cluster's shared memory holds", "", d.V, 0); return -1; }
+  const TokShape s = tok_shape(d.R, d.V, sizeof(T), MODE);
   d.per = s.per;
-  d.stages = s.stages;
-  const cudaError_t e = s.warps == 1 ? tok_go<T, O, MODE, 1, 128>(d, s, st) : s.warps == 4 ? tok_go<T, O, MODE, 4, 128>(d, s, st) : tok_go<T, O, MODE, 8, 256>(d, s, st);
+  d.staged = s.staged;
+  const cudaError_t e = s.warps == 1 ? tok_go<T, O, MODE, 1, 128>(d, s, st) : tok_go<T, O, MODE, 4, 128>(d, s, st);
   if (e != cudaSuccess) { set_error("tokens launch: %s", cudaGetErrorString(e), 0, 0); return -7; }
   return 0;
 }
