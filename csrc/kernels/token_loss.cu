@@ -104,10 +104,13 @@ template <> struct TokVec<float> {
     v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
   }
   static constexpr uint32_t NINF = 0xff800000u;      // a word of logits that are -inf
+  static __device__ __forceinline__ float most(const uint4& w) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
   static __device__ __forceinline__ float most(const uint4 (&w)[4]) {
     float m = __int_as_float(0xff800000);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(w[k].x), __uint_as_float(w[k].y))), fmaxf(__uint_as_float(w[k].z), __uint_as_float(w[k].w)));
+    for (int k = 0; k < 4; ++k) m = fmaxf(m, most(w[k]));
     return m;
   }
 };
@@ -119,15 +122,17 @@ template <> struct TokVec<__nv_bfloat16> {
     for (int k = 0; k < 4; ++k) { v[2 * k] = __uint_as_float(u[k] << 16); v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
   }
   static constexpr uint32_t NINF = 0xff80ff80u;
+  static __device__ __forceinline__ __nv_bfloat162 most2(const uint4& w) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  }
+  static __device__ __forceinline__ float most(const uint4& w) {
+    const __nv_bfloat162 m = most2(w);
+    return fmaxf(__low2float(m), __high2float(m));
+  }
   static __device__ __forceinline__ float most(const uint4 (&w)[4]) {
-    __nv_bfloat162 m[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w[k]);
-      m[k] = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    }
-    m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
-    return fmaxf(__low2float(m[0]), __high2float(m[0]));
+    const __nv_bfloat162 m = __hmax2(__hmax2(most2(w[0]), most2(w[1])), __hmax2(most2(w[2]), most2(w[3])));
+    return fmaxf(__low2float(m), __high2float(m));
   }
 };
 
@@ -144,7 +149,7 @@ template <int W> struct TokShared {
 };
 // What the warps of a row's CTAs tell each other, for this row and the next: maximum, sum, sum times exponent, bound of the alternatives.
 template <bool TOP> struct TokPeers {
-  float4 part[2][TOK_CTAS * 4];
+  float4 part[2][TOK_CTAS * 8];
   unsigned long long key[2][TOP ? TOK_CTAS : 1][ONO_TOP_MAX];
 };
 
@@ -293,8 +298,24 @@ __device__ __noinline__ void zero_write(O* d, int j0, int j1, int gt) {
   if (gt < j1 - last) d[last + gt] = from_f32<O>(0.0f);
 }
 
+// CTAs of an SM that the registers have to allow: 64 registers a thread, a few more where a row is gone through twice in one form or another (us, 1024
+// threads to an SM against this: loss of 4096 x 50257 bf16 175.4 -> 165.9, gradient of 4096 x 128256 362.6 -> 357.6).
+constexpr int tok_resident(int mode, int warps, int threads) {
+  return (warps == 1 || mode <= TOK_TOP ? 1024 : mode == TOK_LOSS ? 896 : 768) / threads;
+}
+
+// Two together.
+template <bool ENT>
+__device__ __forceinline__ TokSums tok_two(const TokSums& a, const TokSums& b) {
+  TokSums s = {fmaxf(a.m, b.m), 0.0f, 0.0f};
+  const float at = shift_of(s.m), fa = shift_of(a.m) - at, fb = shift_of(b.m) - at, ea = exp2_of(fa), eb = exp2_of(fb);
+  if (a.z != 0.0f) { s.z = ea * a.z; if (ENT) s.u = ea * (a.u + fmaxf(fa, -1e4f) * a.z); }
+  if (b.z != 0.0f) { s.z += eb * b.z; if (ENT) s.u += eb * (b.u + fmaxf(fb, -1e4f) * b.z); }
+  return s;
+}
+
 template <typename T, typename O, int MODE, int W, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constant__ TokDev a) {
+__global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(const __grid_constant__ TokDev a) {
   constexpr int E = TokVec<T>::E, GT = W * 32, NG = NT / GT, CAP = TokShared<W>::CAP;
   constexpr bool TOP = MODE == TOK_TOP, ENT = MODE == TOK_ENTROPY || MODE == TOK_TOP, FWD = MODE <= TOK_TOP;
   static_assert(W == 1 || NG == 1, "a CTA takes one row, or a row a warp");
@@ -302,7 +323,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
   extern __shared__ __align__(16) unsigned char tok_smem[];
   __shared__ TokShared<W> s_all[TOP ? NG : 1];
   __shared__ TokPeers<TOP> s_peers;
-  static_assert(W <= 4, "a lane for each warp of a cluster");
   const int grp = threadIdx.x / GT, gt = threadIdx.x % GT, lane = threadIdx.x & 31, warp = gt >> 5;
   TokShared<W>& s = s_all[TOP ? grp : 0];
   int C = 1, rank = 0;
@@ -343,7 +363,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
     for (int v = va + gt; v < vb; v += GT, src += GT * E, dst += GT) cp_async16(dst, src);
   };
 
-  if (W > 1 && C > 1) cluster_sync_all();      // every CTA of the cluster runs: its shared memory may be written to
+  // A CTA's shared memory may be written to once it runs: said here, waited for ahead of the first word to another.
+  bool met = W == 1 || C == 1;
+  if (!met) cluster_arrive();
+  auto meet = [&]() { if (!met) { cluster_wait(); met = true; } };
   long long r = (long long)(blockIdx.x / C) * NG + grp;
   long long raw_next = raw_target(r);
   if (staged && r < a.R && target(raw_next) >= 0) fetch(r);
@@ -511,15 +534,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
         if (gt < K) list[gt] = 0;
       }
       g = tok_join<ENT>(mine);
-      const int par = live & 1, lead = live % C;
+      const int par = live & 1;
       const float4* const part = s_peers.part[par];
       if (W > 1) {
         const float4 told = make_float4(g.m, g.z, g.u, cut);
         if (C == 1) { if (lane == 0) s_peers.part[par][warp] = told; }
-        else if (lane < C) st_cluster_v4(mapa_shared(smem_u32(&s_peers.part[par][rank * W + warp]), (uint32_t)lane), told);
+        else {
+          meet();
+          if (lane < C) st_cluster_v4(mapa_shared(smem_u32(&s_peers.part[par][rank * W + warp]), (uint32_t)lane), told);
+        }
         sync_row();
         auto of = [&](int i) { return i < C * W ? TokSums{part[i].x, part[i].y, part[i].z} : TokSums{ninf, 0.0f, 0.0f}; };
-        g = tok_join<ENT>(of(lane));
+        g = tok_join<ENT>(W == 8 && C > 4 ? tok_two<ENT>(of(lane), of(32 + lane)) : of(lane));
         if (TOP) {
 #pragma unroll
           for (int w = 0; w < W; ++w) { const float c = part[rank * W + w].w; cut = w ? fminf(cut, c) : c; }
@@ -563,14 +589,23 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
         // the threads that have seen a logit that reaches the bound; what they have seen is read again, by all
         if (tm >= cut && tm > ninf) s.who[atomicAdd(&s.threads, 1u)] = (unsigned short)gt;
         group_sync<W>();
-        const int each = (vb - va + GT - 1) / GT, items = max(0, each) * (int)s.threads;
-        for (int i = gt; i < items; i += GT) {
-          const int v = va + s.who[i / each] + i % each * GT;
-          if (v < vb) {
-            float o[E];
-            TokVec<T>::get(load16(x + (v * E - ph)), o);
+        const unsigned int each = max(vb - va + GT - 1, 0) / GT, items = each * s.threads;
+        for (unsigned int i = gt; i < items; i += 4 * GT) {
+          int v[4];
+          uint4 w[4];
 #pragma unroll
-            for (int k = 0; k < E; ++k) offer(o[k], v * E + k - ph);
+          for (int q = 0; q < 4; ++q) {
+            const unsigned int iq = i + q * GT;
+            v[q] = iq < items ? va + s.who[iq / each] + (int)(iq % each) * GT : vb;
+            if (v[q] < vb) w[q] = load16(x + (v[q] * E - ph));
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (v[q] >= vb || !(TokVec<T>::most(w[q]) >= cut)) continue;
+            float o[E];
+            TokVec<T>::get(w[q], o);
+#pragma unroll
+            for (int k = 0; k < E; ++k) offer(o[k], v[q] * E + k - ph);
           }
         }
         if (has_h) offer(xh, jh);
@@ -585,6 +620,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
         for (int i = gt; i < have; i += GT) {
           const unsigned long long key = cand[i];
           int above = 0;
+#pragma unroll 8
           for (int q = 0; q < have; ++q) above += cand[q] > key;
           if (above < K) list[above] = key;
         }
@@ -597,26 +633,31 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
           if (gt < K) put(gt, list[gt]);
           group_sync<W>();
         } else {
-          if (gt < K) {
-            const uint32_t to = mapa_shared(smem_u32(&s_peers.key[par][rank][gt]), (uint32_t)lead);
-            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(list[gt]) : "memory");
+          for (int i = gt; i < K * C; i += GT) {
+            const uint32_t to = mapa_shared(smem_u32(&s_peers.key[par][rank][i / C]), (uint32_t)(i % C));
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(list[i / C]) : "memory");
           }
           cluster_sync_all();
-          if (rank == lead) {
-            const unsigned long long(*keys)[ONO_TOP_MAX] = s_peers.key[par];
-            for (int i = gt; i < C * K; i += GT) {
-              const unsigned long long key = keys[i / K][i % K];
-              int above = 0;
-              for (int q = 0; q < C; ++q)
-                for (int k = 0; k < K; ++k) above += keys[q][k] > key;
-              if (key && above < K) put(above, key);
-            }
-            if (gt < K) {
-              int there = 0;
-              for (int q = 0; q < C; ++q) for (int k = 0; k < K; ++k) there += keys[q][k] != 0;
-              if (gt >= there) put(gt, 0);
-            }
+          // every CTA finds its own keys' places among all, a warp a key
+          unsigned long long all[TOK_CTAS * ONO_TOP_MAX / 32];
+          unsigned int there = 0;
+#pragma unroll
+          for (int q = 0; q < TOK_CTAS * ONO_TOP_MAX / 32; ++q) {
+            const int i = q * 32 + lane;
+            all[q] = i < C * K ? s_peers.key[par][i / K][i % K] : 0;
+            there += all[q] != 0;
           }
+          for (int k = warp; k < K; k += W) {
+            const unsigned long long key = list[k];
+            unsigned int above = 0;
+#pragma unroll
+            for (int q = 0; q < TOK_CTAS * ONO_TOP_MAX / 32; ++q) above += all[q] > key;
+            above = __reduce_add_sync(0xffffffffu, above);
+            if (lane == 0 && key && above < (unsigned)K) put((int)above, key);
+          }
+          there = __reduce_add_sync(0xffffffffu, there);
+          if (rank == 0 && gt < K && gt >= (int)there) put(gt, 0);
+          group_sync<W>();      // (the list has been read)
         }
       }
       ++live;
@@ -652,6 +693,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) tok_kernel(const __grid_constan
     }
     if (staged && r + stride < a.R && target(raw_next) >= 0) fetch(r + stride);
   }
+  meet();
 }
 
 // How a launch is laid out.
@@ -666,8 +708,9 @@ static TokShape tok_shape(long long rows, int V, int esz, int mode) {
   s.ctas = 1;
   s.warps = bytes <= TOK_WARP_ROW ? 1 : 4;
   if (s.warps > 1) {
-    while (s.ctas < TOK_CTAS && ((mode == TOK_LOSS && bytes > (long long)TOK_SLICE * s.ctas) || (rows * s.ctas * 2 <= ono_num_sms() && bytes > 4096ll * s.ctas))) s.ctas *= 2;
+    while (s.ctas < TOK_CTAS && ((mode == TOK_LOSS && bytes > (long long)TOK_SLICE * s.ctas) || (rows * s.ctas <= 4 * ono_num_sms() && bytes > 8192ll * s.ctas))) s.ctas *= 2;
   }
+  if (s.warps > 1 && mode != TOK_LOSS && rows * s.ctas <= 2 * ono_num_sms()) s.warps = 8;
   s.per = (int)((groups + s.ctas - 1) / s.ctas);
   const int rows_of_cta = s.warps == 1 ? 4 : 1;
   s.staged = mode == TOK_LOSS && s.per * 16 <= 100 * 1024;
@@ -711,7 +754,9 @@ static int tok_run(TokDev& d, cudaStream_t st) {
   const TokShape s = tok_shape(d.R, d.V, sizeof(T), MODE);
   d.per = s.per;
   d.staged = s.staged;
-  const cudaError_t e = s.warps == 1 ? tok_go<T, O, MODE, 1, 128>(d, s, st) : tok_go<T, O, MODE, 4, 128>(d, s, st);
+  cudaError_t e;
+  if constexpr (MODE == TOK_LOSS) e = s.warps == 1 ? tok_go<T, O, MODE, 1, 128>(d, s, st) : tok_go<T, O, MODE, 4, 128>(d, s, st);
+  else e = s.warps == 1 ? tok_go<T, O, MODE, 1, 128>(d, s, st) : s.warps == 4 ? tok_go<T, O, MODE, 4, 128>(d, s, st) : tok_go<T, O, MODE, 8, 256>(d, s, st);
   if (e != cudaSuccess) { set_error("tokens launch: %s", cudaGetErrorString(e), 0, 0); return -7; }
   return 0;
 }
