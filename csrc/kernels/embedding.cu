@@ -103,11 +103,15 @@ struct SortShared {
   unsigned int warp_sum[SORT_WARPS];
 };
 
+constexpr int SORT_BATCH = 16;      // keys that a lane has in registers: their loads are in flight together
+
 struct GradDev {
   OnoEmbeddingGrad e;
   unsigned int *key[2], *place[2];     // ping, pong
-  float* part;                         // [chunks][2][width]
-  int passes, bits, chunk, sorted;     // sorted: which of the two holds the result
+  unsigned int* runs;                  // number of long runs, then their first and last chunks
+  float* part;                         // [chunks][2][pitch]
+  int passes, bits, sorted;            // sorted: which of the two holds the result
+  int chunk, pitch;
 };
 
 template <typename I>
@@ -119,35 +123,52 @@ __device__ void sort_places(const GradDev& p, SortShared& s) {
   const unsigned long long first64 = (unsigned long long)per * (unsigned)(rank * SORT_WARPS + warp);
   const unsigned int first = (unsigned int)min((unsigned long long)n, first64), last = (unsigned int)min((unsigned long long)n, first64 + per);
   const unsigned int below = (1u << lane) - 1u;
+  if (n && rank == 0 && tid == 0) *p.runs = 0;
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.bits, radix = 1 << p.bits;
     const unsigned int* kin = p.key[(pass + 1) & 1];
     const unsigned int* pin = p.place[(pass + 1) & 1];
     unsigned int* kout = p.key[pass & 1];
     unsigned int* pout = p.place[pass & 1];
-    auto key_at = [&](unsigned int j) -> unsigned int {
-      if (pass) return __ldcg(kin + j);      // written by other SMs since this one may have read the place
-      const long long r = token_row(reinterpret_cast<const I*>(e.ids)[j], e.vocab, e.padding_id, e.status);
-      return r < 0 ? (unsigned int)e.vocab : (unsigned int)r;      // no token: behind all of them
+    unsigned int key[SORT_BATCH];
+    auto keys_from = [&](unsigned int j0) {
+#pragma unroll
+      for (int b = 0; b < SORT_BATCH; ++b) {
+        const unsigned int j = j0 + 32 * b + lane;
+        if (j >= last) continue;
+        if (pass) {
+          key[b] = __ldcg(kin + j);      // written by other SMs since this one may have read the place
+        } else {
+          const long long r = token_row(__ldg(reinterpret_cast<const I*>(e.ids) + j), e.vocab, e.padding_id, e.status);
+          key[b] = r < 0 ? (unsigned int)e.vocab : (unsigned int)r;      // no token: behind all of them
+        }
+      }
     };
     for (int k = lane; k < radix; k += 32) s.count[warp][k] = 0;
     __syncwarp();
-    for (unsigned int j0 = first; j0 < last; j0 += 32) {
-      const unsigned int j = j0 + lane;
-      const unsigned int digit = j < last ? (key_at(j) >> shift) & (radix - 1) : 0xffffffffu;
-      const unsigned int peers = __match_any_sync(0xffffffffu, digit);
-      if (j < last && (peers & below) == 0) s.count[warp][digit] += __popc(peers);
-      __syncwarp();
+    for (unsigned int j0 = first; j0 < last; j0 += 32 * SORT_BATCH) {
+      keys_from(j0);
+#pragma unroll
+      for (int b = 0; b < SORT_BATCH; ++b) {
+        const unsigned int j = j0 + 32 * b + lane;
+        if (j0 + 32 * b >= last) break;
+        const unsigned int digit = j < last ? (key[b] >> shift) & (radix - 1) : 0xffffffffu;
+        const unsigned int peers = __match_any_sync(0xffffffffu, digit);
+        if (j < last && (peers & below) == 0) s.count[warp][digit] += __popc(peers);
+        __syncwarp();
+      }
     }
     __syncthreads();
     if (tid < radix) {
       unsigned int sum = 0;
+#pragma unroll 8
       for (int w = 0; w < SORT_WARPS; ++w) { const unsigned int c = s.count[w][tid]; s.count[w][tid] = sum; sum += c; }
       s.total[tid] = sum;
     }
     cluster_sync_all();
     unsigned int before = 0, all = 0;
     if (tid < radix) {
+#pragma unroll
       for (int q = 0; q < SORT_CTAS; ++q) {
         unsigned int v;
         asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(&s.total[tid]), (uint32_t)q)) : "memory");
@@ -166,20 +187,30 @@ __device__ void sort_places(const GradDev& p, SortShared& s) {
       s.base[tid] = lower + run - all + before;
     }
     __syncthreads();
-    for (unsigned int j0 = first; j0 < last; j0 += 32) {
-      const unsigned int j = j0 + lane;
-      const unsigned int key = j < last ? key_at(j) : 0u;
-      const unsigned int digit = j < last ? (key >> shift) & (radix - 1) : 0xffffffffu;
-      const unsigned int peers = __match_any_sync(0xffffffffu, digit);
-      unsigned int at = 0;
-      if (j < last) at = s.base[digit] + s.count[warp][digit] + __popc(peers & below);
-      __syncwarp();
-      if (j < last) {
-        if ((peers & below) == 0) s.count[warp][digit] += __popc(peers);
-        kout[at] = key;
-        pout[at] = pass ? __ldcg(pin + j) : j;
+    for (unsigned int j0 = first; j0 < last; j0 += 32 * SORT_BATCH) {
+      unsigned int from[SORT_BATCH];
+      if (last - first > 32 * SORT_BATCH) keys_from(j0);      // (else they are still here)
+#pragma unroll
+      for (int b = 0; b < SORT_BATCH; ++b) {
+        const unsigned int j = j0 + 32 * b + lane;
+        if (j < last) from[b] = pass ? __ldcg(pin + j) : j;
       }
-      __syncwarp();
+#pragma unroll
+      for (int b = 0; b < SORT_BATCH; ++b) {
+        const unsigned int j = j0 + 32 * b + lane;
+        if (j0 + 32 * b >= last) break;
+        const unsigned int digit = j < last ? (key[b] >> shift) & (radix - 1) : 0xffffffffu;
+        const unsigned int peers = __match_any_sync(0xffffffffu, digit);
+        unsigned int at = 0;
+        if (j < last) at = s.base[digit] + s.count[warp][digit] + __popc(peers & below);
+        __syncwarp();
+        if (j < last) {
+          if ((peers & below) == 0) s.count[warp][digit] += __popc(peers);
+          kout[at] = key[b];
+          pout[at] = from[b];
+        }
+        __syncwarp();
+      }
     }
     cluster_sync_all();
   }
@@ -206,120 +237,214 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const __gr
 }
 
 // Second launch: a warp adds up the rows of a chunk of `chunk` sorted places, 32 * VEC columns of them. A run of equal tokens belongs to
-// the chunk it starts in, whose warp follows it into the next chunk if it ends there. A run that is longer is summed chunk by chunk:
-// part[c][1] has the sum of what starts in c, part[c][0] of what comes from before; the third launch adds them in order.
-// `runs_on`: whether the run that place b - 1 belongs to (which starts in the chunk before b) is one of the long ones.
+// the chunk it starts in, whose warp follows it into the next chunk if it ends there. A longer run is summed chunk by chunk: part[c][1]
+// has the sum of what starts in c, part[c][0] of what comes from before; the third launch adds them in order.
+// Whether the run of token k that starts in the chunk before place b and reaches it is one of the long ones.
 __device__ __forceinline__ bool long_run(const unsigned int* key, unsigned int n, unsigned int b, unsigned int chunk, unsigned int k) {
   return b + chunk <= n && key[b + chunk - 1] == k;
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void add_row(float (&acc)[VEC], const T* row, int left) {      // left: columns from here on
-  if constexpr (VEC == 1) {
-    if (left > 0) acc[0] += to_f32(*row);
-  } else {
-    if (left >= VEC) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(row));
-      add_piece<T, VEC>(acc, w);
+template <int VEC>
+struct GradVec {      // what a lane has of an f32 row: 16-byte accesses where the row is aligned and the lane's columns are all there
+  static __device__ __forceinline__ void load(float (&v)[VEC], const float* p, int left, bool aligned) {
+    if (VEC > 1 && aligned && left >= VEC) {
+#pragma unroll
+      for (int k = 0; k < VEC; k += 4) { const float4 w = *reinterpret_cast<const float4*>(p + k); v[k] = w.x; v[(k + 1) % VEC] = w.y; v[(k + 2) % VEC] = w.z; v[(k + 3) % VEC] = w.w; }
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) if (k < left) acc[k] += to_f32(row[k]);
+      for (int k = 0; k < VEC; ++k) v[k] = k < left ? p[k] : 0.0f;
     }
   }
-}
+  static __device__ __forceinline__ void store(float* p, const float (&v)[VEC], int left, bool aligned) {
+    if (VEC > 1 && aligned && left >= VEC) {
+#pragma unroll
+      for (int k = 0; k < VEC; k += 4) *reinterpret_cast<float4*>(p + k) = make_float4(v[k], v[(k + 1) % VEC], v[(k + 2) % VEC], v[(k + 3) % VEC]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) if (k < left) p[k] = v[k];
+    }
+  }
+};
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool ACC>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constant__ GradDev p, int tiles) {
+  constexpr int U = ACC ? 4 : 8;      // rows in flight
   const OnoEmbeddingGrad& e = p.e;
   const unsigned int n = (unsigned int)e.n, L = (unsigned int)p.chunk, none = (unsigned int)e.vocab;
-  const unsigned int* key = p.key[p.sorted];
-  const unsigned int* place = p.place[p.sorted];
+  const unsigned int* const key = p.key[p.sorted];
+  const unsigned int* const place = p.place[p.sorted];
   const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const unsigned int c = (unsigned int)(item / tiles);
-  const int col = ((int)(item - (long long)c * tiles) * 32 + lane) * VEC, left = e.width - col;
-  const unsigned int s = c * L;
-  if (s >= n) return;
-  unsigned int end = min(n, s + L);
-  const unsigned int k0 = key[s], kl = key[end - 1];
+  const int tile = (int)(item - (long long)c * tiles), col = (tile * 32 + lane) * VEC, left = e.width - col;
+  const bool aligned = (((uintptr_t)e.grad | (uintptr_t)(e.ld_grad * 4)) & 15) == 0;
+  if ((unsigned long long)c * L >= n) return;
+  const unsigned int s = c * L, own = min(n, s + L);
+  unsigned int end = own;
+  const unsigned int k0 = key[s], kl = key[own - 1], kb = s > 0 ? key[s - 1] : none, ke = own < n ? key[own] : none;
   if (k0 == none) return;
-  // what comes from the chunk before, and what goes on into the next
-  const bool from_before = s > 0 && key[s - 1] == k0;
-  const bool starts_before = from_before && (s == L || key[s - L] != k0 || key[s - L - 1] != k0);      // in the chunk just before
-  const bool skip_head = from_before && starts_before && !long_run(key, n, s, L, k0);
-  const bool goes_on = end < n && key[end] == kl;
-  const bool all_one = from_before && kl == k0;                  // one run, from before to the end at least
-  bool tail_long = false;
-  if (goes_on && !all_one) {
-    tail_long = long_run(key, n, end, L, kl);
-    if (!tail_long) end = min(n, end + L);                       // this warp finishes it; it stops at the next token
-  }
-  const unsigned int own_end = min(n, s + L);
-  float acc[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-  unsigned int cur = k0;
-  bool head = from_before;
-  auto flush = [&](bool tail) {
-    if (cur != none && !(head && skip_head) && left > 0) {
-      if (head || (tail && tail_long)) {
-        float* o = p.part + ((long long)c * 2 + (head ? 0 : 1)) * e.width + col;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) if (k < left) o[k] = acc[k];
-      } else {
-        float* o = e.grad + (long long)cur * e.ld_grad + col;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k)
-          if (k < left) o[k] = e.accumulate ? o[k] + e.scale * acc[k] : e.scale * acc[k];
+  const bool from_before = s > 0 && kb == k0, goes_on = own < n && ke == kl;
+  unsigned int at = s;
+  if (from_before) {
+    const bool just_before = s == L || key[s - L] != k0 || key[s - L - 1] != k0;      // it starts in the chunk before
+    if (just_before && !long_run(key, n, s, L, k0)) {                                 // whose warp finishes it
+      if (kl == k0) return;
+      for (bool found = false; !found; ) {
+        const unsigned int j = at + lane;
+        const unsigned int other = __ballot_sync(0xffffffffu, j < own && key[min(j, own - 1)] != k0);
+        found = other != 0;
+        at += found ? __ffs(other) - 1 : 32;
       }
     }
+  }
+  const bool head = from_before && at == s;      // a piece of a run that started earlier
+  bool tail_long = false;
+  if (goes_on && !(head && kl == k0) && kl != none) {
+    tail_long = long_run(key, n, own, L, kl);
+    if (!tail_long) {
+      end = min(n, own + L);      // this warp finishes it; it stops at the next token
+    } else if (tile == 0) {       // where it ends: the last place of token kl, 32 probes at a time
+      unsigned int lo = own + L - 1, hi = n;      // key[lo] == kl, key[hi] != kl or hi == n
+      while (hi - lo > 1) {
+        const unsigned int step = (hi - lo + 31) / 32, j = lo + step * (lane + 1);
+        const unsigned int same = __popc(__ballot_sync(0xffffffffu, j < hi && key[min(j, n - 1)] == kl));
+        const unsigned int was = lo;
+        lo = was + step * same;
+        hi = min(hi, was + step * (same + 1));
+      }
+      if (lane == 0) {
+        const unsigned int slot = atomicAdd(p.runs, 1u);
+        p.runs[2 + 2 * slot] = c;
+        p.runs[3 + 2 * slot] = lo / L;
+      }
+    }
+  }
+  float acc[VEC], old[VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-    head = false;
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+  unsigned int cur = none;
+  bool piece = head;
+  auto flush = [&](bool tail) {
+    if (cur == none || left <= 0) return;
+    if (piece || (tail && tail_long)) {
+      GradVec<VEC>::store(p.part + ((long long)c * 2 + (piece ? 0 : 1)) * p.pitch + col, acc, left, true);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] = ACC ? old[k] + e.scale * acc[k] : e.scale * acc[k];
+      GradVec<VEC>::store(e.grad + (long long)cur * e.ld_grad + col, acc, left, aligned);
+    }
   };
-  for (unsigned int j0 = s; j0 < end; j0 += 32) {
+  for (unsigned int j0 = at; j0 < end; j0 += 32) {
     const unsigned int j = j0 + lane;
     const unsigned int kj = j < end ? key[j] : none, pj = j < end ? place[j] : 0u;
     const int m = (int)min(32u, end - j0);
-    for (int q = 0; q < m; ++q) {
-      const unsigned int k = __shfl_sync(0xffffffffu, kj, q), at = __shfl_sync(0xffffffffu, pj, q);
-      if (k != cur) {
-        flush(false);
-        if (k == none || j0 + q >= own_end) return;              // (beyond the chunk only its last run goes on)
-        cur = k;
+    for (int q0 = 0; q0 < m; q0 += U) {
+      uint4 w[U];
+      float f[U][1];
+      float was[ACC ? U : 1][VEC];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int q = q0 + u;
+        const unsigned int k = __shfl_sync(0xffffffffu, kj, q & 31), from = __shfl_sync(0xffffffffu, pj, q & 31);
+        const unsigned int kp = __shfl_sync(0xffffffffu, kj, (q - 1) & 31);
+        if (q < m && k != none && left > 0) {
+          const T* row = reinterpret_cast<const T*>(e.d) + (long long)from * e.ld_d + col;
+          if constexpr (VEC == 1) {
+            f[u][0] = to_f32(*row);
+          } else if (left >= VEC) {
+            w[u] = __ldg(reinterpret_cast<const uint4*>(row));
+          } else {
+            T* t = reinterpret_cast<T*>(&w[u]);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) t[i] = i < left ? row[i] : from_f32<T>(0.0f);
+          }
+          if (ACC && (q == 0 || kp != k)) GradVec<VEC>::load(was[ACC ? u : 0], e.grad + (long long)k * e.ld_grad + col, left, aligned);
+        }
       }
-      if (!(head && skip_head)) add_row<T, VEC>(acc, reinterpret_cast<const T*>(e.d) + (long long)at * e.ld_d + col, left);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int q = q0 + u;
+        const unsigned int k = __shfl_sync(0xffffffffu, kj, q & 31);
+        if (q >= m) break;
+        if (k != cur) {
+          flush(false);
+          if (cur != none) piece = false;
+          if (k == none || j0 + q >= own) return;              // (beyond the chunk only its last run goes on)
+          cur = k;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) { acc[i] = 0.0f; if (ACC) old[i] = was[ACC ? u : 0][i]; }
+        }
+        if (left > 0) {
+          if constexpr (VEC == 1) acc[0] += f[u][0];
+          else add_piece<T, VEC>(acc, w[u]);
+        }
+      }
     }
   }
   flush(true);
 }
 
-// Third launch: a block takes 256 columns of the long run that starts in chunk c, if one does.
+// Third launch: a block takes a long run's sums, 32 * VEC columns of them; its warps every eighth, then one adds up theirs.
+template <int VEC>
 __global__ void __launch_bounds__(256) embedding_join_kernel(const __grid_constant__ GradDev p, int tiles) {
+  __shared__ float s_sum[8][32 * VEC];
   const OnoEmbeddingGrad& e = p.e;
-  const unsigned int n = (unsigned int)e.n, L = (unsigned int)p.chunk;
-  const unsigned int* key = p.key[p.sorted];
-  const unsigned int c = blockIdx.x / tiles, s = c * L, end = s + L;
-  if (end >= n) return;
-  const unsigned int k = key[end - 1];
-  if (k == (unsigned int)e.vocab || key[end] != k || !long_run(key, n, end, L, k)) return;
-  if (s > 0 && key[s] == k && key[s - 1] == k) return;            // it started before
-  const int col = (int)(blockIdx.x - c * tiles) * 256 + threadIdx.x;
-  if (col >= e.width) return;
-  float acc = p.part[((long long)c * 2 + 1) * e.width + col];
-  for (unsigned int q = c + 1; (unsigned long long)q * L < n && key[q * L] == k; ++q) acc += p.part[(long long)q * 2 * e.width + col];
-  float* o = e.grad + (long long)k * e.ld_grad + col;
-  *o = e.accumulate ? *o + e.scale * acc : e.scale * acc;
+  const unsigned int L = (unsigned int)p.chunk, runs = *p.runs;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool aligned = (((uintptr_t)e.grad | (uintptr_t)(e.ld_grad * 4)) & 15) == 0;
+  for (unsigned long long item = blockIdx.x; item < (unsigned long long)runs * tiles; item += gridDim.x) {
+    const unsigned int run = (unsigned int)(item / tiles), c = p.runs[2 + 2 * run], c1 = p.runs[3 + 2 * run];
+    const int col = ((int)(item - (unsigned long long)run * tiles) * 32 + lane) * VEC, left = e.width - col;
+    float acc[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+    if (left > 0) {
+#pragma unroll 4
+      for (unsigned int q = c + warp; q <= c1; q += 8) {
+        float v[VEC];
+        GradVec<VEC>::load(v, p.part + ((long long)q * 2 + (q == c ? 1 : 0)) * p.pitch + col, left, true);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s_sum[warp][lane * VEC + k] = acc[k];
+    __syncthreads();
+    if (warp == 0 && left > 0) {
+      float* g = e.grad + (long long)p.key[p.sorted][c * L + L - 1] * e.ld_grad + col;
+      float old[VEC];
+      if (e.accumulate) GradVec<VEC>::load(old, g, left, aligned);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        float t = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += s_sum[w][lane * VEC + k];
+        acc[k] = e.accumulate ? old[k] + e.scale * t : e.scale * t;
+      }
+      GradVec<VEC>::store(g, acc, left, aligned);
+    }
+    __syncthreads();
+  }
 }
 
-constexpr int GRAD_CHUNK = 64;
+// Places to a chunk: as many as leave enough warps to fill the GPU (a lane has U rows in flight whatever the chunk).
+static int grad_chunk(long long n, int width) {
+  const long long tiles = (width + 127) / 128;
+  int L = 512;
+  while (L > 8 && n / L * tiles < 32ll * 148) L >>= 1;
+  return L;
+}
 
-struct GradScratch { long long key, part, bytes; };
+struct GradScratch { long long key, runs, part, bytes; int chunk, pitch; };
 static GradScratch grad_scratch(long long n, int width) {
   GradScratch g;
+  g.chunk = grad_chunk(n, width);
+  g.pitch = (width + 3) / 4 * 4;
+  const long long chunks = (n + g.chunk - 1) / g.chunk;
   g.key = (n * 4 + 15) / 16 * 16;
-  g.part = 4 * g.key;
-  g.bytes = g.part + (n + GRAD_CHUNK - 1) / GRAD_CHUNK * 2 * width * 4;
+  g.runs = 4 * g.key;
+  g.part = g.runs + ((2 + 2 * chunks) * 4 + 15) / 16 * 16;
+  g.bytes = g.part + chunks * 2 * g.pitch * 4;
   return g;
 }
 
@@ -379,11 +504,13 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
     p.key[k] = reinterpret_cast<unsigned int*>(at + k * g.key);
     p.place[k] = reinterpret_cast<unsigned int*>(at + (2 + k) * g.key);
   }
+  p.runs = reinterpret_cast<unsigned int*>(at + g.runs);
   p.part = reinterpret_cast<float*>(at + g.part);
+  p.chunk = g.chunk;
+  p.pitch = g.pitch;
   const int need = 32 - __builtin_clz((unsigned)e->vocab);      // tokens, and `vocab` for none
   p.passes = (need + SORT_BITS - 1) / SORT_BITS;
   p.bits = (need + p.passes - 1) / p.passes;
-  p.chunk = GRAD_CHUNK;
   p.sorted = (p.passes - 1) & 1;
   int zero = 0;
   if (!e->accumulate) {
@@ -410,21 +537,22 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
   const int esz = e->d_bf16 ? 2 : 4;
   const bool vec = ((uintptr_t)e->d & 15) == 0 && e->ld_d * esz % 16 == 0;
   const int cols = 32 * (vec ? 16 / esz : 1), tiles = (e->width + cols - 1) / cols;
-  const long long chunks = (e->n + GRAD_CHUNK - 1) / GRAD_CHUNK, blocks = (chunks * tiles + 7) / 8;
+  const long long chunks = (e->n + g.chunk - 1) / g.chunk, blocks = (chunks * tiles + 7) / 8;
   if (blocks >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
   using B = __nv_bfloat16;
-  if (e->d_bf16) {
-    if (vec) embedding_sum_kernel<B, 8><<<(unsigned)blocks, 256, 0, st>>>(p, tiles);
-    else embedding_sum_kernel<B, 1><<<(unsigned)blocks, 256, 0, st>>>(p, tiles);
+  auto sum = [&](auto kern) { kern<<<(unsigned)blocks, 256, 0, st>>>(p, tiles); };
+  if (e->accumulate) {
+    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, true>); else sum(embedding_sum_kernel<B, 1, true>); }
+    else { if (vec) sum(embedding_sum_kernel<float, 4, true>); else sum(embedding_sum_kernel<float, 1, true>); }
   } else {
-    if (vec) embedding_sum_kernel<float, 4><<<(unsigned)blocks, 256, 0, st>>>(p, tiles);
-    else embedding_sum_kernel<float, 1><<<(unsigned)blocks, 256, 0, st>>>(p, tiles);
+    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, false>); else sum(embedding_sum_kernel<B, 1, false>); }
+    else { if (vec) sum(embedding_sum_kernel<float, 4, false>); else sum(embedding_sum_kernel<float, 1, false>); }
   }
   if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad sum: %s", cudaGetErrorString(r), 0, 0); return -7; }
-  if (e->n > 2 * GRAD_CHUNK) {      // shorter ones have no long run
-    const int jt = (e->width + 255) / 256;
-    if (chunks * jt >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
-    embedding_join_kernel<<<(unsigned)(chunks * jt), 256, 0, st>>>(p, jt);
+  if (e->n > g.chunk) {      // (a long run fills a whole chunk and begins ahead of it)
+    const int jt = (e->width + 127) / 128;
+    const unsigned grid = (unsigned)std::min<long long>(chunks * jt, 4ll * ono_num_sms());
+    embedding_join_kernel<4><<<grid, 256, 0, st>>>(p, jt);
     if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad join: %s", cudaGetErrorString(r), 0, 0); return -7; }
   }
   return 0;
