@@ -18,6 +18,19 @@
 namespace ono {
 void set_error(const char* fmt, const char* a, long long b, long long c);
 
+// The lanes whose digit is this one's, of `bits` bits; digits are below 2^bits, lanes without one give 2^bits.
+__device__ __forceinline__ unsigned int same_digit(unsigned int digit, int bits) {
+  unsigned int peers = 0xffffffffu;
+#pragma unroll
+  for (int b = 0; b < 10; ++b) {
+    if (b > bits) break;
+    const bool one = digit >> b & 1u;
+    const unsigned int ones = __ballot_sync(0xffffffffu, one);
+    peers &= one ? ones : ~ones;
+  }
+  return peers;
+}
+
 // The row an id stands for, -1 for none.
 template <typename I>
 __device__ __forceinline__ long long token_row(I id, int vocab, long long padding_id, int* status) {
@@ -28,22 +41,27 @@ __device__ __forceinline__ long long token_row(I id, int vocab, long long paddin
 }
 
 // ------------------------------------------------------------------------------------------------
-// Lookup: a warp takes EMB_SEG groups of a row, a lane up to four of them, VEC values each.
+// Lookup: a warp takes 32 * EMB_LOADS groups of VEC values of a row, or several rows where one has fewer groups than lanes.
 // ------------------------------------------------------------------------------------------------
-constexpr int EMB_SEG = 128;
+// Two loads to a lane; more leave fewer warps, each of which waits for its row's number first (131072 x 2048 bf16, us: one 174, two 134, four 161,
+// eight 387). Values that come one by one are four bytes or two, and then eight are in flight (100000 x 517 f32: two 123, four 85).
+template <int VEC> constexpr int EMB_LOADS = VEC == 1 ? 8 : 2;
 
 template <typename TI, typename TO, int VEC, typename I>
-__global__ void __launch_bounds__(256) embedding_kernel(const OnoEmbedding e, int groups, int segs) {
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const long long i = item / segs;
+__global__ void __launch_bounds__(256) embedding_kernel(const OnoEmbedding e, int groups, int segs, int lanes) {
+  constexpr int U = EMB_LOADS<VEC>;
+  const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  // lanes: log2 of those that a row takes
+  const long long i = lanes < 5 ? job * (32 >> lanes) + (lane >> lanes) : job / segs;
   if (i >= e.n) return;
-  const int lane = threadIdx.x & 31, g0 = (int)(item - i * segs) * EMB_SEG + lane;
+  const int g0 = lanes < 5 ? lane & ((1 << lanes) - 1) : (int)(job - i * segs) * 32 * U + lane;
   const long long row = token_row(reinterpret_cast<const I*>(e.ids)[i], e.vocab, e.padding_id, e.status);
   const TI* src = reinterpret_cast<const TI*>(e.table) + (row < 0 ? 0 : row) * e.ld_table;
   TO* dst = reinterpret_cast<TO*>(e.out) + i * e.ld_out;
-  float v[4][VEC];
+  float v[U][VEC];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int g = g0 + 32 * u;
     if (g >= groups) continue;
     if (VEC > 1 && (g + 1) * VEC <= e.width) {
@@ -62,7 +80,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const OnoEmbedding e, in
     }
   }
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int g = g0 + 32 * u;
     if (g >= groups) continue;
     if (row >= 0) {
@@ -89,150 +107,174 @@ __global__ void __launch_bounds__(256) embedding_kernel(const OnoEmbedding e, in
 }
 
 // ------------------------------------------------------------------------------------------------
-// Gradient. First launch: cluster 0 sorts the places by token, the other CTAs fill the table with zeros.
+// Gradient. The places are sorted by token (stable), while other CTAs of the same launches fill the table with zeros.
 // ------------------------------------------------------------------------------------------------
-// A radix sort, `bits` (at most 9) of the token a pass, stable. The places are dealt to the cluster's warps in runs; a warp goes through its
-// own 32 at a time, lanes of one digit finding each other by match. Counts per warp and digit are turned into positions by a sum over the
-// warps, one over the CTAs (distributed shared memory) and one over the digits. Keys and places go through memory between passes
-// (L2): the cluster barrier, release and acquire, orders them.
-constexpr int SORT_CTAS = 8, SORT_THREADS = 1024, SORT_WARPS = SORT_THREADS / 32, SORT_BITS = 9, SORT_RADIX = 1 << SORT_BITS;
-struct SortShared {
-  unsigned int count[SORT_WARPS][SORT_RADIX];
-  unsigned int total[SORT_RADIX];      // read by the other CTAs
-  unsigned int base[SORT_RADIX];
-  unsigned int warp_sum[SORT_WARPS];
-};
-
-constexpr int SORT_BATCH = 16;      // keys that a lane has in registers: their loads are in flight together
-
 struct GradDev {
   OnoEmbeddingGrad e;
-  unsigned int *key[2], *place[2];     // ping, pong
+  uint2* item[2];                      // token and place, ping and pong
+  unsigned int* hist;                  // [3][tiles][SORT_RADIX]: of a pass, the next and the one after it, in turn
   unsigned int* runs;                  // number of long runs, then their first and last chunks
   float* part;                         // [chunks][2][pitch]
-  int passes, bits, sorted;            // sorted: which of the two holds the result
+  int sorted;                          // which of `item` holds the result
   int chunk, pitch;
+  int bits, tile, tiles;               // radix sort: bits a pass, places of a CTA, CTAs
 };
 
-template <typename I>
-__device__ void sort_places(const GradDev& p, SortShared& s) {
-  const OnoEmbeddingGrad& e = p.e;
-  const unsigned int n = (unsigned int)e.n;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = (int)cluster_ctarank();
-  const unsigned int per = ((n + SORT_CTAS * SORT_WARPS - 1) / (SORT_CTAS * SORT_WARPS) + 31) / 32 * 32;
-  const unsigned long long first64 = (unsigned long long)per * (unsigned)(rank * SORT_WARPS + warp);
-  const unsigned int first = (unsigned int)min((unsigned long long)n, first64), last = (unsigned int)min((unsigned long long)n, first64 + per);
-  const unsigned int below = (1u << lane) - 1u;
-  if (n && rank == 0 && tid == 0) *p.runs = 0;
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const int shift = pass * p.bits, radix = 1 << p.bits;
-    const unsigned int* kin = p.key[(pass + 1) & 1];
-    const unsigned int* pin = p.place[(pass + 1) & 1];
-    unsigned int* kout = p.key[pass & 1];
-    unsigned int* pout = p.place[pass & 1];
-    unsigned int key[SORT_BATCH];
-    auto keys_from = [&](unsigned int j0) {
-#pragma unroll
-      for (int b = 0; b < SORT_BATCH; ++b) {
-        const unsigned int j = j0 + 32 * b + lane;
-        if (j >= last) continue;
-        if (pass) {
-          key[b] = __ldcg(kin + j);      // written by other SMs since this one may have read the place
-        } else {
-          const long long r = token_row(__ldg(reinterpret_cast<const I*>(e.ids) + j), e.vocab, e.padding_id, e.status);
-          key[b] = r < 0 ? (unsigned int)e.vocab : (unsigned int)r;      // no token: behind all of them
-        }
-      }
-    };
-    for (int k = lane; k < radix; k += 32) s.count[warp][k] = 0;
-    __syncwarp();
-    for (unsigned int j0 = first; j0 < last; j0 += 32 * SORT_BATCH) {
-      keys_from(j0);
-#pragma unroll
-      for (int b = 0; b < SORT_BATCH; ++b) {
-        const unsigned int j = j0 + 32 * b + lane;
-        if (j0 + 32 * b >= last) break;
-        const unsigned int digit = j < last ? (key[b] >> shift) & (radix - 1) : 0xffffffffu;
-        const unsigned int peers = __match_any_sync(0xffffffffu, digit);
-        if (j < last && (peers & below) == 0) s.count[warp][digit] += __popc(peers);
-        __syncwarp();
-      }
+// Zeros for the CTAs behind the first `from` of a launch: values [cta * ZERO_VALUES, ...) of the table, `cta` from `first` on.
+constexpr int ZERO_VALUES = 1 << 16;      // of a CTA (a multiple of 4)
+__device__ __forceinline__ void fill_zeros(const OnoEmbeddingGrad& e, long long cta) {
+  const int threads = (int)blockDim.x;
+  if (e.ld_grad == e.width && ((uintptr_t)e.grad & 15) == 0) {
+    const long long all = (long long)e.vocab * e.width, end = min(all, (cta + 1) * ZERO_VALUES);
+    for (long long i = cta * ZERO_VALUES + 4 * threadIdx.x; i < end; i += 4 * threads) {
+      if (i + 4 <= all) *reinterpret_cast<float4*>(e.grad + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+      else for (long long k = i; k < all; ++k) e.grad[k] = 0.0f;
     }
-    __syncthreads();
-    if (tid < radix) {
-      unsigned int sum = 0;
-#pragma unroll 8
-      for (int w = 0; w < SORT_WARPS; ++w) { const unsigned int c = s.count[w][tid]; s.count[w][tid] = sum; sum += c; }
-      s.total[tid] = sum;
-    }
-    cluster_sync_all();
-    unsigned int before = 0, all = 0;
-    if (tid < radix) {
-#pragma unroll
-      for (int q = 0; q < SORT_CTAS; ++q) {
-        unsigned int v;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(&s.total[tid]), (uint32_t)q)) : "memory");
-        if (q < rank) before += v;
-        all += v;
-      }
-    }
-    unsigned int run = all;                  // inclusive sum over the digits
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const unsigned int v = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += v; }
-    if (lane == 31) s.warp_sum[warp] = run;
-    __syncthreads();
-    if (tid < radix) {
-      unsigned int lower = 0;
-      for (int w = 0; w < warp; ++w) lower += s.warp_sum[w];
-      s.base[tid] = lower + run - all + before;
-    }
-    __syncthreads();
-    for (unsigned int j0 = first; j0 < last; j0 += 32 * SORT_BATCH) {
-      unsigned int from[SORT_BATCH];
-      if (last - first > 32 * SORT_BATCH) keys_from(j0);      // (else they are still here)
-#pragma unroll
-      for (int b = 0; b < SORT_BATCH; ++b) {
-        const unsigned int j = j0 + 32 * b + lane;
-        if (j < last) from[b] = pass ? __ldcg(pin + j) : j;
-      }
-#pragma unroll
-      for (int b = 0; b < SORT_BATCH; ++b) {
-        const unsigned int j = j0 + 32 * b + lane;
-        if (j0 + 32 * b >= last) break;
-        const unsigned int digit = j < last ? (key[b] >> shift) & (radix - 1) : 0xffffffffu;
-        const unsigned int peers = __match_any_sync(0xffffffffu, digit);
-        unsigned int at = 0;
-        if (j < last) at = s.base[digit] + s.count[warp][digit] + __popc(peers & below);
-        __syncwarp();
-        if (j < last) {
-          if ((peers & below) == 0) s.count[warp][digit] += __popc(peers);
-          kout[at] = key[b];
-          pout[at] = from[b];
-        }
-        __syncwarp();
-      }
-    }
-    cluster_sync_all();
+  } else {
+    const long long rows = (ZERO_VALUES + e.width - 1) / e.width, end = min((long long)e.vocab, (cta + 1) * rows);
+    for (long long v = cta * rows + (threadIdx.x >> 5); v < end; v += threads >> 5)
+      for (int k = threadIdx.x & 31; k < e.width; k += 32) e.grad[v * e.ld_grad + k] = 0.0f;
   }
+}
+static long long zero_ctas(const OnoEmbeddingGrad& e) {
+  if (e.accumulate) return 0;
+  if (e.ld_grad == e.width && ((uintptr_t)e.grad & 15) == 0) return ((long long)e.vocab * e.width + ZERO_VALUES - 1) / ZERO_VALUES;
+  const long long rows = (ZERO_VALUES + e.width - 1) / e.width;
+  return (e.vocab + rows - 1) / rows;
+}
+
+// The token of a place; `vocab`, behind all of them, where there is none.
+template <typename I>
+__device__ __forceinline__ unsigned int token_key(const OnoEmbeddingGrad& e, unsigned int j) {
+  const long long r = token_row(__ldg(reinterpret_cast<const I*>(e.ids) + j), e.vocab, e.padding_id, e.status);
+  return r < 0 ? (unsigned int)e.vocab : (unsigned int)r;
+}
+
+// Few places: each finds its rank by comparing with all of them, four threads a place. One launch, no pass waits for another.
+constexpr int RANK_MAX = 4096, RANK_PLACES = 64;
+template <typename I>
+__global__ void __launch_bounds__(4 * RANK_PLACES) embedding_rank_kernel(const __grid_constant__ GradDev p, int ctas) {
+  __shared__ __align__(16) unsigned int s_key[RANK_MAX];
+  const OnoEmbeddingGrad& e = p.e;
+  if ((int)blockIdx.x >= ctas) { fill_zeros(e, blockIdx.x - ctas); return; }
+  const int n = (int)e.n, nv = (n + 3) / 4;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
+  for (int j = threadIdx.x; j < 4 * nv; j += 4 * RANK_PLACES) s_key[j] = j < n ? token_key<I>(e, j) : 0xffffffffu;
+  __syncthreads();
+  const int i = blockIdx.x * RANK_PLACES + (threadIdx.x >> 2), part = threadIdx.x & 3;
+  const uint4* keys = reinterpret_cast<const uint4*>(s_key);
+  unsigned int rank = 0, key = 0;
+  if (i < n) {
+    key = s_key[i];
+    const int vi = i >> 2;
+#pragma unroll 4
+    for (int v = part; v < vi; v += 4) { const uint4 k = keys[v]; rank += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key); }
+#pragma unroll 4
+    for (int v = vi + 1 + part; v < nv; v += 4) { const uint4 k = keys[v]; rank += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key); }
+    const unsigned int k = s_key[4 * vi + part];
+    rank += k < key || (k == key && 4 * vi + part < i);
+  }
+  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+  rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+  if (i < n && part == 0) p.item[p.sorted][rank] = make_uint2(key, (unsigned int)i);
+}
+
+// Many: a radix sort, `bits` (at most 9) of the token a pass. A CTA has a tile of the places, its warps runs of it; a warp goes through its
+// own 32 at a time, lanes of one digit finding each other by a vote on every bit (match.any takes longer the more digits there are:
+// 131072 places 74 us, so 62). Positions are sums of counts: over the warps, over the tiles before (each CTA adds them up itself) and
+// over the digits. The first launch counts; every pass then counts for the next one where its places go to.
+constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_BITS = 9, SORT_RADIX = 1 << SORT_BITS, SORT_BATCH = 2;
+constexpr int SORT_TILE = SORT_THREADS * SORT_BATCH, SORT_TILES = 256;      // places of a CTA, or as many times that as leave SORT_TILES of them
+static_assert(SORT_THREADS == SORT_RADIX, "a thread for each digit");
+
+template <typename I>
+__global__ void __launch_bounds__(SORT_THREADS) embedding_count_kernel(const __grid_constant__ GradDev p, long long zero) {
+  __shared__ unsigned int s_count[SORT_RADIX];
+  const OnoEmbeddingGrad& e = p.e;
+  if ((int)blockIdx.x >= p.tiles) { fill_zeros(e, zero + blockIdx.x - p.tiles); return; }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
+  s_count[threadIdx.x] = 0;
+  unsigned int* const mine = p.hist + blockIdx.x * SORT_RADIX + threadIdx.x;
+  mine[p.tiles * SORT_RADIX] = 0;
+  __syncthreads();
+  const long long j0 = (long long)blockIdx.x * p.tile, end = min(e.n, j0 + p.tile);
+#pragma unroll 8
+  for (long long j = j0 + threadIdx.x; j < end; j += SORT_THREADS) atomicAdd(&s_count[token_key<I>(e, (unsigned int)j) & ((1u << p.bits) - 1)], 1u);
+  __syncthreads();
+  *mine = s_count[threadIdx.x];
 }
 
 template <typename I>
-__global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const __grid_constant__ GradDev p) {
-  extern __shared__ __align__(16) unsigned char sort_smem[];
-  if (blockIdx.x < SORT_CTAS) {
-    sort_places<I>(p, *reinterpret_cast<SortShared*>(sort_smem));
-    return;
-  }
+__global__ void __launch_bounds__(SORT_THREADS) embedding_scatter_kernel(const __grid_constant__ GradDev p, int pass, int last, long long zero) {
+  __shared__ unsigned int s_count[SORT_WARPS][SORT_RADIX], s_base[SORT_RADIX], s_sum[SORT_WARPS];
   const OnoEmbeddingGrad& e = p.e;
-  const long long t = (long long)(blockIdx.x - SORT_CTAS) * SORT_THREADS + threadIdx.x, nt = (long long)(gridDim.x - SORT_CTAS) * SORT_THREADS;
-  if (e.ld_grad == e.width && ((uintptr_t)e.grad & 15) == 0) {
-    const long long all = (long long)e.vocab * e.width, n4 = all >> 2;
-    float4* g = reinterpret_cast<float4*>(e.grad);
-    for (long long i = t; i < n4; i += nt) g[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (long long i = 4 * n4 + t; i < all; i += nt) e.grad[i] = 0.0f;
-  } else {
-    for (long long v = t >> 5; v < e.vocab; v += nt >> 5)
-      for (int k = threadIdx.x & 31; k < e.width; k += 32) e.grad[v * e.ld_grad + k] = 0.0f;
+  if ((int)blockIdx.x >= p.tiles) { fill_zeros(e, zero + blockIdx.x - p.tiles); return; }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int shift = pass * p.bits;
+  const unsigned int mask = (1u << p.bits) - 1, below = (1u << lane) - 1u;
+  const uint2* in = p.item[(pass + 1) & 1];
+  uint2* out = p.item[pass & 1];
+  const unsigned int* hist = p.hist + pass % 3 * p.tiles * SORT_RADIX;
+  unsigned int* next = p.hist + (pass + 1) % 3 * p.tiles * SORT_RADIX;
+  p.hist[((pass + 2) % 3 * p.tiles + blockIdx.x) * SORT_RADIX + tid] = 0;
+  const long long begin = (long long)blockIdx.x * p.tile + (long long)warp * (p.tile / SORT_WARPS);
+  const long long end = min(e.n, begin + p.tile / SORT_WARPS);
+  uint2 it[SORT_BATCH];
+  auto items_from = [&](long long j0) {
+#pragma unroll
+    for (int b = 0; b < SORT_BATCH; ++b) {
+      const long long j = j0 + 32 * b + lane;
+      if (j < end) it[b] = pass ? __ldg(in + j) : make_uint2(token_key<I>(e, (unsigned int)j), (unsigned int)j);
+    }
+  };
+  items_from(begin);
+  for (int k = lane; k < SORT_RADIX; k += 32) s_count[warp][k] = 0;
+  __syncwarp();
+  for (long long j0 = begin; j0 < end; j0 += 32 * SORT_BATCH) {
+    if (j0 != begin) items_from(j0);
+#pragma unroll
+    for (int b = 0; b < SORT_BATCH; ++b)
+      if (j0 + 32 * b + lane < end) atomicAdd(&s_count[warp][it[b].x >> shift & mask], 1u);
+  }
+  // a digit a thread: its places in the tiles before, and in all
+  unsigned int before = 0, all = 0;
+#pragma unroll 8
+  for (int t = 0; t < p.tiles; ++t) {
+    const unsigned int h = __ldg(hist + t * SORT_RADIX + tid);
+    if (t < (int)blockIdx.x) before += h;
+    all += h;
+  }
+  unsigned int run = all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const unsigned int v = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += v; }
+  if (lane == 31) s_sum[warp] = run;
+  __syncthreads();
+  unsigned int lower = 0;
+#pragma unroll
+  for (int w = 0; w < SORT_WARPS; ++w) if (w < warp) lower += s_sum[w];
+  s_base[tid] = lower + run - all + before;
+  unsigned int sum = 0;
+#pragma unroll
+  for (int w = 0; w < SORT_WARPS; ++w) { const unsigned int c = s_count[w][tid]; s_count[w][tid] = sum; sum += c; }
+  __syncthreads();
+  for (long long j0 = begin; j0 < end; j0 += 32 * SORT_BATCH) {
+    if (end - begin > 32 * SORT_BATCH) items_from(j0);      // (else they are still here)
+#pragma unroll
+    for (int b = 0; b < SORT_BATCH; ++b) {
+      const long long j = j0 + 32 * b + lane;
+      if (j0 + 32 * b >= end) break;
+      const unsigned int digit = j < end ? it[b].x >> shift & mask : mask + 1;
+      const unsigned int peers = same_digit(digit, p.bits);
+      unsigned int at = 0;
+      if (j < end) at = s_base[digit] + s_count[warp][digit] + __popc(peers & below);
+      __syncwarp();
+      if (j < end) {
+        if ((peers & below) == 0) s_count[warp][digit] += __popc(peers);
+        out[at] = it[b];      // (token and place in one store: scattered ones take a cycle a place)
+        if (!last) atomicAdd(&next[at / (unsigned int)p.tile * SORT_RADIX + (it[b].x >> (shift + p.bits) & mask)], 1u);
+      }
+      __syncwarp();
+    }
   }
 }
 
@@ -240,8 +282,8 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const __gr
 // the chunk it starts in, whose warp follows it into the next chunk if it ends there. A longer run is summed chunk by chunk: part[c][1]
 // has the sum of what starts in c, part[c][0] of what comes from before; the third launch adds them in order.
 // Whether the run of token k that starts in the chunk before place b and reaches it is one of the long ones.
-__device__ __forceinline__ bool long_run(const unsigned int* key, unsigned int n, unsigned int b, unsigned int chunk, unsigned int k) {
-  return b + chunk <= n && key[b + chunk - 1] == k;
+__device__ __forceinline__ bool long_run(const uint2* item, unsigned int n, unsigned int b, unsigned int chunk, unsigned int k) {
+  return b + chunk <= n && item[b + chunk - 1].x == k;
 }
 
 template <int VEC>
@@ -266,32 +308,31 @@ struct GradVec {      // what a lane has of an f32 row: 16-byte accesses where t
   }
 };
 
-template <typename T, int VEC, bool ACC>
+// U rows are in flight; with ACC those of the table that they are added to as well.
+template <typename T, int VEC, bool ACC, int U>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constant__ GradDev p, int tiles) {
-  constexpr int U = ACC ? 4 : 8;      // rows in flight
   const OnoEmbeddingGrad& e = p.e;
   const unsigned int n = (unsigned int)e.n, L = (unsigned int)p.chunk, none = (unsigned int)e.vocab;
-  const unsigned int* const key = p.key[p.sorted];
-  const unsigned int* const place = p.place[p.sorted];
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint2* const item = p.item[p.sorted];
+  const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  const unsigned int c = (unsigned int)(item / tiles);
-  const int tile = (int)(item - (long long)c * tiles), col = (tile * 32 + lane) * VEC, left = e.width - col;
+  const unsigned int c = (unsigned int)(job / tiles);
+  const int tile = (int)(job - (long long)c * tiles), col = (tile * 32 + lane) * VEC, left = e.width - col;
   const bool aligned = (((uintptr_t)e.grad | (uintptr_t)(e.ld_grad * 4)) & 15) == 0;
   if ((unsigned long long)c * L >= n) return;
   const unsigned int s = c * L, own = min(n, s + L);
   unsigned int end = own;
-  const unsigned int k0 = key[s], kl = key[own - 1], kb = s > 0 ? key[s - 1] : none, ke = own < n ? key[own] : none;
+  const unsigned int k0 = item[s].x, kl = item[own - 1].x, kb = s > 0 ? item[s - 1].x : none, ke = own < n ? item[own].x : none;
   if (k0 == none) return;
   const bool from_before = s > 0 && kb == k0, goes_on = own < n && ke == kl;
   unsigned int at = s;
   if (from_before) {
-    const bool just_before = s == L || key[s - L] != k0 || key[s - L - 1] != k0;      // it starts in the chunk before
-    if (just_before && !long_run(key, n, s, L, k0)) {                                 // whose warp finishes it
+    const bool just_before = s == L || item[s - L].x != k0 || item[s - L - 1].x != k0;      // it starts in the chunk before
+    if (just_before && !long_run(item, n, s, L, k0)) {                                 // whose warp finishes it
       if (kl == k0) return;
       for (bool found = false; !found; ) {
         const unsigned int j = at + lane;
-        const unsigned int other = __ballot_sync(0xffffffffu, j < own && key[min(j, own - 1)] != k0);
+        const unsigned int other = __ballot_sync(0xffffffffu, j < own && item[min(j, own - 1)].x != k0);
         found = other != 0;
         at += found ? __ffs(other) - 1 : 32;
       }
@@ -300,14 +341,14 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
   const bool head = from_before && at == s;      // a piece of a run that started earlier
   bool tail_long = false;
   if (goes_on && !(head && kl == k0) && kl != none) {
-    tail_long = long_run(key, n, own, L, kl);
+    tail_long = long_run(item, n, own, L, kl);
     if (!tail_long) {
       end = min(n, own + L);      // this warp finishes it; it stops at the next token
     } else if (tile == 0) {       // where it ends: the last place of token kl, 32 probes at a time
       unsigned int lo = own + L - 1, hi = n;      // key[lo] == kl, key[hi] != kl or hi == n
       while (hi - lo > 1) {
         const unsigned int step = (hi - lo + 31) / 32, j = lo + step * (lane + 1);
-        const unsigned int same = __popc(__ballot_sync(0xffffffffu, j < hi && key[min(j, n - 1)] == kl));
+        const unsigned int same = __popc(__ballot_sync(0xffffffffu, j < hi && item[min(j, n - 1)].x == kl));
         const unsigned int was = lo;
         lo = was + step * same;
         hi = min(hi, was + step * (same + 1));
@@ -336,7 +377,8 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
   };
   for (unsigned int j0 = at; j0 < end; j0 += 32) {
     const unsigned int j = j0 + lane;
-    const unsigned int kj = j < end ? key[j] : none, pj = j < end ? place[j] : 0u;
+    const uint2 ij = j < end ? item[j] : make_uint2(none, 0u);
+    const unsigned int kj = ij.x, pj = ij.y;
     const int m = (int)min(32u, end - j0);
     for (int q0 = 0; q0 < m; q0 += U) {
       uint4 w[U];
@@ -384,10 +426,112 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
   flush(true);
 }
 
-// Third launch: a block takes a long run's sums, 32 * VEC columns of them; its warps every eighth, then one adds up theirs.
+// Very few places: no sorting. A warp takes a place and 32 * VEC columns, looks for the place's token among all, and where the place is the
+// token's first adds up its rows, U in flight. The other CTAs fill the rows of the table that no token means with zeros. One launch.
+constexpr int FEW_MAX = 512, FEW_VALUES = 1 << 14;      // FEW_VALUES: zeros of a CTA
+template <typename T, int VEC, typename I>
+__global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGrad e, int tiles, int ctas) {
+  constexpr int U = 16, WORDS = FEW_MAX / 32;
+  __shared__ unsigned int s_word[8 * FEW_MAX / 2];      // rows with a token, or the warps' lists of 16 bits a place
+  static_assert(FEW_VALUES / 32 + 1 <= 8 * FEW_MAX / 2, "a bit for each of a CTA's rows");
+  const I* ids = reinterpret_cast<const I*>(e.ids);
+  const int n = (int)e.n, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool aligned = (((uintptr_t)e.grad | (uintptr_t)(e.ld_grad * 4)) & 15) == 0;
+  if ((int)blockIdx.x >= ctas) {
+    const long long cta = blockIdx.x - ctas;
+    const int rows = (FEW_VALUES + e.width - 1) / e.width;
+    const long long first = cta * rows;
+    const int mine = (int)min((long long)rows, e.vocab - first);
+    for (int k = threadIdx.x; k <= mine / 32; k += 256) s_word[k] = 0;
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += 256) {
+      const long long r = token_row(ids[j], e.vocab, e.padding_id, nullptr) - first;
+      if (r >= 0 && r < mine) atomicOr(&s_word[r >> 5], 1u << (r & 31));
+    }
+    __syncthreads();
+    auto met = [&](int r) { return s_word[r >> 5] >> (r & 31) & 1u; };
+    float* const g = e.grad + first * e.ld_grad;
+    if (e.width >= 64) {      // a warp a row
+      for (int r = warp; r < mine; r += 8) {
+        if (met(r)) continue;
+        float* const row = g + (long long)r * e.ld_grad;
+        const int head = min(e.width, (int)((16 - ((uintptr_t)row & 15)) & 15) / 4), body = head + ((e.width - head) & ~3);
+        if (lane < head) row[lane] = 0.0f;
+        for (int k = head + 4 * lane; k < body; k += 128) *reinterpret_cast<float4*>(row + k) = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane < e.width - body) row[body + lane] = 0.0f;
+      }
+    } else {      // a thread a value
+      for (int k = threadIdx.x; k < mine * e.width; k += 256) {
+        const int r = k / e.width;
+        if (!met(r)) g[(long long)r * e.ld_grad + k - r * e.width] = 0.0f;
+      }
+    }
+    return;
+  }
+  const long long job = (long long)blockIdx.x * 8 + warp;
+  const int i = (int)(job / tiles), col = ((int)(job - (long long)i * tiles) * 32 + lane) * VEC, left = e.width - col;
+  if (i >= n) return;
+  const I id = ids[i];
+  unsigned int same[WORDS];
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int j = 32 * w + lane;
+    const bool eq = j < n && ids[min(j, n - 1)] == id;
+    same[w] = 32 * w < n ? __ballot_sync(0xffffffffu, eq) : 0u;
+  }
+  const long long row = token_row(id, e.vocab, e.padding_id, e.status);
+  if (row < 0) return;
+  unsigned short* const list = reinterpret_cast<unsigned short*>(s_word) + warp * FEW_MAX;
+  int count = 0;
+  bool first = true;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    if (32 * w < i && (32 * w + 32 <= i ? same[w] : same[w] & ((1u << (i & 31)) - 1u))) first = false;
+    if (same[w] >> lane & 1u) list[count + __popc(same[w] & ((1u << lane) - 1u))] = (unsigned short)(32 * w + lane);
+    count += __popc(same[w]);
+  }
+  if (!first) return;
+  __syncwarp();
+  if (left <= 0) return;
+  float* const g = e.grad + row * e.ld_grad + col;
+  float acc[VEC], old[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+  if (e.accumulate) GradVec<VEC>::load(old, g, left, aligned);
+  for (int q0 = 0; q0 < count; q0 += U) {
+    uint4 w[U];
+    float f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (q0 + u >= count) continue;
+      const T* src = reinterpret_cast<const T*>(e.d) + (long long)list[q0 + u] * e.ld_d + col;
+      if (VEC == 1) {
+        f[u] = to_f32(*src);
+      } else if (left >= VEC) {
+        w[u] = __ldg(reinterpret_cast<const uint4*>(src));
+      } else {
+        T* t = reinterpret_cast<T*>(&w[u]);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) t[k] = k < left ? src[k] : from_f32<T>(0.0f);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (q0 + u >= count) break;
+      if constexpr (VEC == 1) acc[0] += f[u];
+      else add_piece<T, VEC>(acc, w[u]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = e.accumulate ? old[k] + e.scale * acc[k] : e.scale * acc[k];
+  GradVec<VEC>::store(g, acc, left, aligned);
+}
+
+// Third launch: a block takes a long run's sums, 32 * VEC columns of them; its warps every JOIN_WARPS-th, then one adds up theirs.
+constexpr int JOIN_WARPS = 16;
 template <int VEC>
-__global__ void __launch_bounds__(256) embedding_join_kernel(const __grid_constant__ GradDev p, int tiles) {
-  __shared__ float s_sum[8][32 * VEC];
+__global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const __grid_constant__ GradDev p, int tiles) {
+  __shared__ float s_sum[JOIN_WARPS][32 * VEC];
   const OnoEmbeddingGrad& e = p.e;
   const unsigned int L = (unsigned int)p.chunk, runs = *p.runs;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -399,8 +543,8 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const __grid_consta
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
     if (left > 0) {
-#pragma unroll 4
-      for (unsigned int q = c + warp; q <= c1; q += 8) {
+#pragma unroll 8
+      for (unsigned int q = c + warp; q <= c1; q += JOIN_WARPS) {
         float v[VEC];
         GradVec<VEC>::load(v, p.part + ((long long)q * 2 + (q == c ? 1 : 0)) * p.pitch + col, left, true);
 #pragma unroll
@@ -411,14 +555,14 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const __grid_consta
     for (int k = 0; k < VEC; ++k) s_sum[warp][lane * VEC + k] = acc[k];
     __syncthreads();
     if (warp == 0 && left > 0) {
-      float* g = e.grad + (long long)p.key[p.sorted][c * L + L - 1] * e.ld_grad + col;
+      float* g = e.grad + (long long)p.item[p.sorted][c * L + L - 1].x * e.ld_grad + col;
       float old[VEC];
       if (e.accumulate) GradVec<VEC>::load(old, g, left, aligned);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         float t = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) t += s_sum[w][lane * VEC + k];
+        for (int w = 0; w < JOIN_WARPS; ++w) t += s_sum[w][lane * VEC + k];
         acc[k] = e.accumulate ? old[k] + e.scale * t : e.scale * t;
       }
       GradVec<VEC>::store(g, acc, left, aligned);
@@ -431,31 +575,43 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const __grid_consta
 static int grad_chunk(long long n, int width) {
   const long long tiles = (width + 127) / 128;
   int L = 512;
-  while (L > 8 && n / L * tiles < 32ll * 148) L >>= 1;
+  while (L > 8 && n / L * tiles < (L > 64 ? 128ll : L > 32 ? 64 : 32) * 148) L >>= 1;
   return L;
 }
 
-struct GradScratch { long long key, runs, part, bytes; int chunk, pitch; };
+struct GradScratch { long long items, hist, runs, part, bytes; int chunk, pitch, tile, tiles; };
 static GradScratch grad_scratch(long long n, int width) {
   GradScratch g;
   g.chunk = grad_chunk(n, width);
   g.pitch = (width + 3) / 4 * 4;
   const long long chunks = (n + g.chunk - 1) / g.chunk;
-  g.key = (n * 4 + 15) / 16 * 16;
-  g.runs = 4 * g.key;
+  g.items = (n * 8 + 15) / 16 * 16;
+  g.tile = SORT_TILE * (int)((n + (long long)SORT_TILE * SORT_TILES - 1) / ((long long)SORT_TILE * SORT_TILES));
+  g.tiles = n > RANK_MAX ? (int)((n + g.tile - 1) / g.tile) : 0;
+  g.hist = 2 * g.items;
+  g.runs = g.hist + 3ll * g.tiles * SORT_RADIX * 4;
   g.part = g.runs + ((2 + 2 * chunks) * 4 + 15) / 16 * 16;
   g.bytes = g.part + chunks * 2 * g.pitch * 4;
   return g;
 }
 
-template <typename TI, typename TO, typename I>
-static cudaError_t embedding_go(const OnoEmbedding& e, bool vec, cudaStream_t st) {
+template <typename TI, typename TO, int VEC, typename I>
+static int embedding_go(const OnoEmbedding& e, cudaStream_t st) {
+  const int groups = (e.width + VEC - 1) / VEC, segs = (groups + 32 * EMB_LOADS<VEC> - 1) / (32 * EMB_LOADS<VEC>);
+  int lanes = 5;
+  while (lanes > 0 && groups <= 1 << (lanes - 1)) --lanes;
+  const long long jobs = lanes < 5 ? (e.n + (32 >> lanes) - 1) / (32 >> lanes) : e.n * segs, blocks = (jobs + 7) / 8;
+  if (blocks >= (1ll << 31)) { set_error("embedding: too many values%s", "", 0, 0); return -1; }
+  embedding_kernel<TI, TO, VEC, I><<<(unsigned)blocks, 256, 0, st>>>(e, groups, segs, lanes);
+  const cudaError_t r = cudaGetLastError();
+  if (r != cudaSuccess) { set_error("embedding launch: %s", cudaGetErrorString(r), 0, 0); return -7; }
+  return 0;
+}
+template <typename TI, typename TO>
+static int embedding_go(const OnoEmbedding& e, bool vec, cudaStream_t st) {
   constexpr int VEC = sizeof(TI) == 4 && sizeof(TO) == 4 ? 4 : 8;
-  const int groups = vec ? (e.width + VEC - 1) / VEC : e.width, segs = (groups + EMB_SEG - 1) / EMB_SEG;
-  const long long blocks = (e.n * segs + 7) / 8;
-  if (vec) embedding_kernel<TI, TO, VEC, I><<<(unsigned)blocks, 256, 0, st>>>(e, groups, segs);
-  else embedding_kernel<TI, TO, 1, I><<<(unsigned)blocks, 256, 0, st>>>(e, groups, segs);
-  return cudaGetLastError();
+  if (e.ids64) return vec ? embedding_go<TI, TO, VEC, long long>(e, st) : embedding_go<TI, TO, 1, long long>(e, st);
+  return vec ? embedding_go<TI, TO, VEC, int>(e, st) : embedding_go<TI, TO, 1, int>(e, st);
 }
 }  // namespace ono
 
@@ -466,93 +622,104 @@ extern "C" int ono_embedding(const OnoEmbedding* e, ono_stream_t stream) {
     set_error("bad embedding args%s", "", 0, 0);
     return -1;
   }
-  if (e->n * ((e->width + EMB_SEG - 1) / EMB_SEG) >= (8ll << 31)) { set_error("embedding: too many values%s", "", 0, 0); return -1; }
   if (e->n == 0) return 0;
   cudaStream_t st = (cudaStream_t)stream;
   const int ti = e->table_bf16 ? 2 : 4, to = e->out_bf16 ? 2 : 4;
   const bool vec = (((uintptr_t)e->table | (uintptr_t)e->out) & 15) == 0 && e->ld_table * ti % 16 == 0 && e->ld_out * to % 16 == 0;
   using B = __nv_bfloat16;
-  cudaError_t r;
-  if (e->ids64)
-    r = e->table_bf16 ? (e->out_bf16 ? embedding_go<B, B, long long>(*e, vec, st) : embedding_go<B, float, long long>(*e, vec, st))
-                      : (e->out_bf16 ? embedding_go<float, B, long long>(*e, vec, st) : embedding_go<float, float, long long>(*e, vec, st));
-  else
-    r = e->table_bf16 ? (e->out_bf16 ? embedding_go<B, B, int>(*e, vec, st) : embedding_go<B, float, int>(*e, vec, st))
-                      : (e->out_bf16 ? embedding_go<float, B, int>(*e, vec, st) : embedding_go<float, float, int>(*e, vec, st));
-  if (r != cudaSuccess) { set_error("embedding launch: %s", cudaGetErrorString(r), 0, 0); return -7; }
-  return 0;
+  if (e->table_bf16) return e->out_bf16 ? embedding_go<B, B>(*e, vec, st) : embedding_go<B, float>(*e, vec, st);
+  return e->out_bf16 ? embedding_go<float, B>(*e, vec, st) : embedding_go<float, float>(*e, vec, st);
 }
 
 extern "C" long long ono_embedding_grad_scratch(long long n, int vocab, int width) {
-  return n < 0 || vocab <= 0 || width <= 0 ? -1 : grad_scratch(n, width).bytes;
+  return n < 0 || vocab <= 0 || width <= 0 ? -1 : n <= FEW_MAX ? 0 : grad_scratch(n, width).bytes;
 }
 
 extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream) {
   if (!e || e->n < 0 || e->n > (1ll << 31) - 65536 || e->vocab <= 0 || e->width <= 0 || e->ld_d < e->width || e->ld_grad < e->width || !e->grad ||
-      (e->n && (!e->d || !e->ids || !e->scratch))) {
+      (e->n && (!e->d || !e->ids))) {
     set_error("bad embedding_grad args%s", "", 0, 0);
     return -1;
   }
   const GradScratch g = grad_scratch(e->n, e->width);
-  if (e->n && (e->scratch_bytes < g.bytes || ((uintptr_t)e->scratch & 15))) { set_error("embedding_grad: scratch of %s%lld bytes, 16-byte aligned", "", g.bytes, 0); return -1; }
+  if (e->n > FEW_MAX && (!e->scratch || e->scratch_bytes < g.bytes || ((uintptr_t)e->scratch & 15))) { set_error("embedding_grad: scratch of %s%lld bytes, 16-byte aligned", "", g.bytes, 0); return -1; }
   if (e->n == 0 && e->accumulate) return 0;
   cudaStream_t st = (cudaStream_t)stream;
-  GradDev p;
+  GradDev p = {};
   p.e = *e;
   char* at = reinterpret_cast<char*>(e->scratch);
-  for (int k = 0; k < 2; ++k) {
-    p.key[k] = reinterpret_cast<unsigned int*>(at + k * g.key);
-    p.place[k] = reinterpret_cast<unsigned int*>(at + (2 + k) * g.key);
-  }
+  for (int k = 0; k < 2; ++k) p.item[k] = reinterpret_cast<uint2*>(at + k * g.items);
+  p.hist = reinterpret_cast<unsigned int*>(at + g.hist);
   p.runs = reinterpret_cast<unsigned int*>(at + g.runs);
   p.part = reinterpret_cast<float*>(at + g.part);
   p.chunk = g.chunk;
   p.pitch = g.pitch;
-  const int need = 32 - __builtin_clz((unsigned)e->vocab);      // tokens, and `vocab` for none
-  p.passes = (need + SORT_BITS - 1) / SORT_BITS;
-  p.bits = (need + p.passes - 1) / p.passes;
-  p.sorted = (p.passes - 1) & 1;
-  int zero = 0;
-  if (!e->accumulate) {
-    const long long per = 4ll * SORT_THREADS * 4;                // a few stores a thread
-    zero = (int)std::min<long long>(2ll * ono_num_sms() / SORT_CTAS, ((long long)e->vocab * e->width + per * SORT_CTAS - 1) / (per * SORT_CTAS));
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(SORT_CTAS * (1 + zero)));
-  cfg.blockDim = dim3(SORT_THREADS);
-  cfg.dynamicSmemBytes = sizeof(SortShared);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = SORT_CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  auto sort = [&](auto kern) -> cudaError_t {
-    const cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared));
-    return r != cudaSuccess ? r : cudaLaunchKernelEx(&cfg, kern, p);
-  };
-  cudaError_t r = e->ids64 ? sort(embedding_sort_kernel<long long>) : sort(embedding_sort_kernel<int>);
-  if (r != cudaSuccess) { set_error("embedding_grad sort: %s", cudaGetErrorString(r), 0, 0); return -7; }
-  if (e->n == 0) return 0;
   const int esz = e->d_bf16 ? 2 : 4;
   const bool vec = ((uintptr_t)e->d & 15) == 0 && e->ld_d * esz % 16 == 0;
   const int cols = 32 * (vec ? 16 / esz : 1), tiles = (e->width + cols - 1) / cols;
   const long long chunks = (e->n + g.chunk - 1) / g.chunk, blocks = (chunks * tiles + 7) / 8;
   if (blocks >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
   using B = __nv_bfloat16;
+  cudaError_t r;
+  if (e->n <= FEW_MAX && e->n > 0) {
+    const long long ctas = (e->n * tiles + 7) / 8, rows = (FEW_VALUES + e->width - 1) / e->width, zero = e->accumulate ? 0 : (e->vocab + rows - 1) / rows;
+    auto few = [&](auto kern) { kern<<<(unsigned)(ctas + zero), 256, 0, st>>>(*e, tiles, (int)ctas); };
+    if (ctas + zero >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
+    if (e->ids64) {
+      if (e->d_bf16) { if (vec) few(embedding_few_kernel<B, 8, long long>); else few(embedding_few_kernel<B, 1, long long>); }
+      else { if (vec) few(embedding_few_kernel<float, 4, long long>); else few(embedding_few_kernel<float, 1, long long>); }
+    } else {
+      if (e->d_bf16) { if (vec) few(embedding_few_kernel<B, 8, int>); else few(embedding_few_kernel<B, 1, int>); }
+      else { if (vec) few(embedding_few_kernel<float, 4, int>); else few(embedding_few_kernel<float, 1, int>); }
+    }
+    if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad: %s", cudaGetErrorString(r), 0, 0); return -7; }
+    return 0;
+  }
+  const long long zeros = zero_ctas(*e);
+  if (zeros >= (1ll << 30)) { set_error("embedding_grad: too large a table%s", "", 0, 0); return -1; }
+  if (e->n <= RANK_MAX) {
+    const int ctas = (int)((e->n + RANK_PLACES - 1) / RANK_PLACES);
+    p.sorted = 0;
+    if (e->ids64) embedding_rank_kernel<long long><<<(unsigned)(ctas + zeros), 4 * RANK_PLACES, 0, st>>>(p, ctas);
+    else embedding_rank_kernel<int><<<(unsigned)(ctas + zeros), 4 * RANK_PLACES, 0, st>>>(p, ctas);
+    r = cudaGetLastError();
+  } else {
+    const int need = 32 - __builtin_clz((unsigned)e->vocab);      // tokens, and `vocab` for none
+    const int passes = (need + SORT_BITS - 1) / SORT_BITS;
+    p.bits = (need + passes - 1) / passes;
+    p.tile = g.tile;
+    p.tiles = g.tiles;
+    p.sorted = (passes - 1) & 1;
+    long long done = 0;
+    auto zeros_for = [&](int launch) { return zeros * (launch + 1) / (passes + 1) - done; };      // an even share of each launch
+    long long now = zeros_for(0);
+    if (e->ids64) embedding_count_kernel<long long><<<(unsigned)(g.tiles + now), SORT_THREADS, 0, st>>>(p, done);
+    else embedding_count_kernel<int><<<(unsigned)(g.tiles + now), SORT_THREADS, 0, st>>>(p, done);
+    r = cudaGetLastError();
+    done += now;
+    for (int pass = 0; pass < passes && r == cudaSuccess; ++pass) {
+      now = zeros_for(pass + 1);
+      if (e->ids64) embedding_scatter_kernel<long long><<<(unsigned)(g.tiles + now), SORT_THREADS, 0, st>>>(p, pass, pass == passes - 1, done);
+      else embedding_scatter_kernel<int><<<(unsigned)(g.tiles + now), SORT_THREADS, 0, st>>>(p, pass, pass == passes - 1, done);
+      r = cudaGetLastError();
+      done += now;
+    }
+  }
+  if (r != cudaSuccess) { set_error("embedding_grad sort: %s", cudaGetErrorString(r), 0, 0); return -7; }
+  if (e->n == 0) return 0;
   auto sum = [&](auto kern) { kern<<<(unsigned)blocks, 256, 0, st>>>(p, tiles); };
   if (e->accumulate) {
-    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, true>); else sum(embedding_sum_kernel<B, 1, true>); }
-    else { if (vec) sum(embedding_sum_kernel<float, 4, true>); else sum(embedding_sum_kernel<float, 1, true>); }
+    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, true, 4>); else sum(embedding_sum_kernel<B, 1, true, 8>); }
+    else { if (vec) sum(embedding_sum_kernel<float, 4, true, 4>); else sum(embedding_sum_kernel<float, 1, true, 8>); }
   } else {
-    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, false>); else sum(embedding_sum_kernel<B, 1, false>); }
-    else { if (vec) sum(embedding_sum_kernel<float, 4, false>); else sum(embedding_sum_kernel<float, 1, false>); }
+    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, false, 8>); else sum(embedding_sum_kernel<B, 1, false, 8>); }
+    else { if (vec) sum(embedding_sum_kernel<float, 4, false, 8>); else sum(embedding_sum_kernel<float, 1, false, 8>); }
   }
   if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad sum: %s", cudaGetErrorString(r), 0, 0); return -7; }
   if (e->n > g.chunk) {      // (a long run fills a whole chunk and begins ahead of it)
     const int jt = (e->width + 127) / 128;
     const unsigned grid = (unsigned)std::min<long long>(chunks * jt, 4ll * ono_num_sms());
-    embedding_join_kernel<4><<<grid, 256, 0, st>>>(p, jt);
+    embedding_join_kernel<4><<<grid, 32 * JOIN_WARPS, 0, st>>>(p, jt);
     if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad join: %s", cudaGetErrorString(r), 0, 0); return -7; }
   }
   return 0;

@@ -49,7 +49,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, *, scal
 
 
 def embedding_grad_scratch(n: int, vocab: int, width: int) -> int:
-    """Bytes of scratch that ``embedding_grad`` wants for ``n`` tokens."""
+    """Bytes of scratch that ``embedding_grad`` wants for ``n`` tokens (0 for few)."""
     return _lib.load().ono_embedding_grad_scratch(n, vocab, width)
 
 
@@ -74,11 +74,12 @@ def embedding_grad(d: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, *, sc
     _lib.one_device(d, ids, grad, status, scratch)
     if vocab == 0 or width == 0:
         return
-    need = embedding_grad_scratch(n, vocab, width)
     if scratch is None:
-        scratch = _lib.scratch(grad, need, stream)
+        need = embedding_grad_scratch(n, vocab, width)
+        if need:
+            scratch = _lib.scratch(grad, need, stream)
     e = _lib.OnoEmbeddingGrad(d.data_ptr(), ids.data_ptr(), grad.data_ptr(), n, _lib.pitch(d), _lib.pitch(grad),
                               NO_PADDING if padding_id is None else padding_id, vocab, width, d.dtype == torch.bfloat16,
-                              ids.dtype == torch.int64, accumulate, scale, _lib.status_ptr(status), scratch.data_ptr(),
-                              scratch.numel() * scratch.element_size())
+                              ids.dtype == torch.int64, accumulate, scale, _lib.status_ptr(status), None if scratch is None else scratch.data_ptr(),
+                              0 if scratch is None else scratch.numel() * scratch.element_size())
     _lib.launch(grad, stream, "ono_embedding_grad", C.byref(e))
