@@ -20,7 +20,7 @@
 namespace ono {
 void set_error(const char* fmt, const char* a, long long b, long long c);
 
-constexpr int CLIP_TENSORS = 256, CLIP_CHUNK = 4096, CLIP_THREADS = 256, CLIP_MAX_BLOCKS = 8 * 148;
+constexpr int CLIP_TENSORS = 256, CLIP_THREADS = 256, CLIP_GROUPS = 2, CLIP_CHUNK = 8 * CLIP_THREADS * CLIP_GROUPS, CLIP_MAX_BLOCKS = 8 * 148;
 
 // A tensor's values are counted from the 8 values' boundary in front of the first (`phase` before it), so that groups of eight
 // that begin at a multiple of eight are aligned.
@@ -127,12 +127,11 @@ __global__ void __launch_bounds__(CLIP_THREADS) clip_norm_kernel(const __grid_co
   for (unsigned int c = blockIdx.x; c < b.end[b.count - 1]; c += gridDim.x) {
     const int t = clip_find(b, c);
     const long long at = (long long)(c - (t ? b.end[t - 1] : 0)) * CLIP_CHUNK - b.phase[t];
+    float v[CLIP_GROUPS][8];
 #pragma unroll
-    for (int k = 0; k < CLIP_CHUNK / CLIP_THREADS / 8; ++k) {
-      float v[8];
-      clip_load8(b.g[t], b.type[t] & 3, at + 8 * (k * CLIP_THREADS + (int)threadIdx.x), b.n[t], v);
-      acc += squares8(v);
-    }
+    for (int k = 0; k < CLIP_GROUPS; ++k) clip_load8(b.g[t], b.type[t] & 3, at + 8 * (k * CLIP_THREADS + (int)threadIdx.x), b.n[t], v[k]);
+#pragma unroll
+    for (int k = 0; k < CLIP_GROUPS; ++k) acc += squares8(v[k]);
   }
   acc = block_sum(acc, s);
   if (threadIdx.x == 0) part[blockIdx.x] = first ? acc : part[blockIdx.x] + acc;
@@ -165,15 +164,16 @@ __global__ void __launch_bounds__(CLIP_THREADS) clip_write_kernel(const __grid_c
     if (f == 1.0f && b.out[t] == b.g[t]) continue;
     const long long at = (long long)(c - (t ? b.end[t - 1] : 0)) * CLIP_CHUNK - b.phase[t];
     const bool aligned = (((uintptr_t)b.out[t] / (otype ? 2 : 4)) & 7) == b.phase[t];
+    float v[CLIP_GROUPS][8];
 #pragma unroll
-    for (int k = 0; k < CLIP_CHUNK / CLIP_THREADS / 8; ++k) {
+    for (int k = 0; k < CLIP_GROUPS; ++k) clip_load8(b.g[t], type, at + 8 * (k * CLIP_THREADS + (int)threadIdx.x), b.n[t], v[k]);
+#pragma unroll
+    for (int k = 0; k < CLIP_GROUPS; ++k) {
       const long long i = at + 8 * (k * CLIP_THREADS + (int)threadIdx.x);
       if (i >= b.n[t]) break;
-      float v[8];
-      clip_load8(b.g[t], type, i, b.n[t], v);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] *= f;
-      clip_store8(b.out[t], otype, i, b.n[t], aligned, v);
+      for (int q = 0; q < 8; ++q) v[k][q] *= f;
+      clip_store8(b.out[t], otype, i, b.n[t], aligned, v[k]);
     }
   }
 }
@@ -184,15 +184,14 @@ using namespace ono;
 extern "C" long long ono_clip_scratch(void) { return CLIP_MAX_BLOCKS * 8; }
 
 extern "C" int ono_clip(const OnoClip* c, ono_stream_t stream) {
-  if (!c || c->n_tensors < 0 || (c->n_tensors && !c->t) || !c->scratch || c->scratch_bytes < ono_clip_scratch() || ((uintptr_t)c->scratch & 7)) {
+  if (!c || c->n_tensors < 0 || (c->n_tensors && (!c->g || !c->n || !c->types)) || !c->scratch || c->scratch_bytes < ono_clip_scratch() || ((uintptr_t)c->scratch & 7)) {
     set_error("bad clip args%s", "", 0, 0);
     return -1;
   }
   if (!(c->max_norm > 0.0f) || !isfinite(c->scale)) { set_error("clip: max_norm must be positive and scale finite%s", "", 0, 0); return -1; }
   for (int k = 0; k < c->n_tensors; ++k) {
-    const OnoClipTensor& t = c->t[k];
-    if (t.n < 0 || (unsigned)t.g_dtype > 2u || (c->write && (unsigned)t.out_dtype > 2u) || (t.n && (!t.g || (c->write && !t.out))) ||
-        ((uintptr_t)t.g & (t.g_dtype ? 1 : 3)) || (c->write && ((uintptr_t)t.out & (t.out_dtype ? 1 : 3)))) {
+    const int type = c->types[k] & 3, otype = c->types[k] >> 2;
+    if (c->n[k] < 0 || type > 2 || otype > 2 || (c->n[k] && (!c->g[k] || ((uintptr_t)c->g[k] & (type ? 1 : 3)) || (c->out && (!c->out[k] || ((uintptr_t)c->out[k] & (otype ? 1 : 3))))))) {
       set_error("bad clip tensor %s%lld", "", k, 0);
       return -1;
     }
@@ -206,15 +205,14 @@ extern "C" int ono_clip(const OnoClip* c, ono_stream_t stream) {
     b.count = 0;
     unsigned int end = 0;
     for (; next < c->n_tensors && b.count < CLIP_TENSORS; ++next) {
-      const OnoClipTensor& t = c->t[next];
-      if (t.n == 0) continue;
-      const int k = b.count, esz = t.g_dtype ? 2 : 4;
-      const int phase = (int)(((uintptr_t)t.g / esz) & 7);
-      const long long chunks = (t.n + phase + CLIP_CHUNK - 1) / CLIP_CHUNK;
+      const long long n = c->n[next];
+      if (n == 0) continue;
+      const int k = b.count, phase = (int)(((uintptr_t)c->g[next] / (c->types[next] & 3 ? 2 : 4)) & 7);
+      const long long chunks = (n + phase + CLIP_CHUNK - 1) / CLIP_CHUNK;
       if (end + chunks >= (1ll << 31)) break;
-      b.g[k] = t.g; b.out[k] = t.out; b.n[k] = t.n;
+      b.g[k] = c->g[next]; b.out[k] = c->out ? c->out[next] : nullptr; b.n[k] = n;
       b.phase[k] = (unsigned char)phase;
-      b.type[k] = (unsigned char)(t.g_dtype | (c->write ? t.out_dtype : 0) << 2);
+      b.type[k] = c->types[next];
       b.end[k] = end += (unsigned)chunks;
       ++b.count;
     }
@@ -231,7 +229,7 @@ extern "C" int ono_clip(const OnoClip* c, ono_stream_t stream) {
     clip_norm_kernel<<<grid, CLIP_THREADS, 0, st>>>(b, part, parts == 0);
     parts = std::max(parts, grid);
   }
-  if (!c->write || parts == 0) {
+  if (!c->out || parts == 0) {
     clip_finish_kernel<<<1, CLIP_THREADS, 0, st>>>(part, parts, c->scale, c->max_norm, c->norm, c->coef);
   } else {
     next = 0;

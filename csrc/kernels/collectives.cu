@@ -858,8 +858,7 @@ extern "C" int ono_sizeof(int which) {
     case 15: return (int)sizeof(OnoEmbeddingGrad);
     case 16: return (int)sizeof(OnoTokens);
     case 17: return (int)sizeof(OnoTokensGrad);
-    case 18: return (int)sizeof(OnoClipTensor);
-    case 19: return (int)sizeof(OnoClip);
+    case 18: return (int)sizeof(OnoClip);
     default: return -1;
   }
 }

@@ -544,18 +544,19 @@ typedef struct OnoTokensGrad {
 int ono_tokens_grad(const OnoTokensGrad* t, ono_stream_t stream);
 
 // ---------------------------------------------------------------------------------------------
-// Norm of all gradients and clipping (clip.cu). `t` lists the tensors (contiguous, any alignment of their type; dtypes 0 f32, 1 bf16, 2 f16).
+// Norm of all gradients and clipping (clip.cu). Tensors: contiguous, any number, any size, any alignment of their type (0 f32, 1 bf16, 2 f16).
 //   norm = |scale| sqrt(sum over all tensors of g^2);  coef = norm <= max_norm ? 1 : max_norm / norm (NaN for a NaN)
 //   out = coef * scale * g where out is given (it may be g itself, of the same type).
 // scratch: ono_clip_scratch bytes, 8-byte aligned; calls that overlap on the device need one each.
 // ---------------------------------------------------------------------------------------------
-typedef struct OnoClipTensor { const void* g; void* out; long long n; int g_dtype, out_dtype; } OnoClipTensor;
 typedef struct OnoClip {
-  const OnoClipTensor* t;    // host memory
-  int n_tensors;
+  int n_tensors;                   // the four arrays, in host memory, have as many entries
+  const void* const* g;
+  void* const* out;                // null: nothing is written
+  const long long* n;              // values of each
+  const unsigned char* types;      // type of g, and of out times four
   float scale, max_norm;
-  float* norm; float* coef;  // device, each optional
-  int write;                 // 1: out is written
+  float* norm; float* coef;        // device, each optional
   void* scratch; long long scratch_bytes;
 } OnoClip;
 long long ono_clip_scratch(void);

@@ -111,7 +111,7 @@ def _declare(lib) -> None:
     for i, st in enumerate((OnoGemm, OnoLoss, OnoOptim, OnoRows, OnoSync, OnoPsAsync, OnoRing, OnoStagePull, OnoRingEmu, OnoFeed, OnoColsum, OnoDenseStep)):
         if lib.ono_sizeof(i) != C.sizeof(st):
             raise RuntimeError(f"ABI mismatch for {st.__name__}: C {lib.ono_sizeof(i)} vs ctypes {C.sizeof(st)}")
-    for i, st in enumerate((OnoEmbedding, OnoEmbeddingGrad, OnoTokens, OnoTokensGrad, OnoClipTensor, OnoClip), 14):
+    for i, st in enumerate((OnoEmbedding, OnoEmbeddingGrad, OnoTokens, OnoTokensGrad, OnoClip), 14):
         if lib.ono_sizeof(i) != C.sizeof(st):
             raise RuntimeError(f"ABI mismatch for {st.__name__}: C {lib.ono_sizeof(i)} vs ctypes {C.sizeof(st)}")
 
@@ -127,52 +127,6 @@ def stream_ptr(stream=None) -> int:
 
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
-
-
-def one_device(first, *others) -> None:
-    """All on one GPU (None among them does not count)."""
-    if not first.is_cuda:
-        raise RuntimeError("this op runs on CUDA only (no CPU fallback on this path)")
-    at = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != at:
-            raise ValueError(f"tensors on different devices: cuda:{at} and {t.device}")
-
-
-def pitch(t) -> int:
-    """Elements from one row of a matrix to the next."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def status_ptr(t) -> int | None:
-    import torch
-
-    if t is not None and (t.dtype != torch.int32 or t.numel() < 1):
-        raise TypeError("status must be int32")
-    return None if t is None else t.data_ptr()
-
-
-def scratch(t, nbytes: int, stream):
-    """Memory for one call that launches on ``stream`` (None: the current one) of the GPU of ``t``: the allocator gives it to nobody else
-    before what that stream holds now has run."""
-    import torch
-
-    if stream is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=t.device)
-    with torch.cuda.stream(stream):
-        return torch.empty(nbytes, dtype=torch.uint8, device=t.device)
-
-
-def launch(t, stream, name: str, args) -> None:
-    """``name(args, stream)`` with the GPU of ``t`` as the current device, on ``stream`` (None: the one that is current there)."""
-    import torch
-
-    fn = getattr(load(), name)
-    if t.get_device() == torch.cuda.current_device():
-        check(fn(args, stream_ptr(stream)), name)
-    else:
-        with torch.cuda.device(t.device):
-            check(fn(args, stream_ptr(stream)), name)
 
 
 # --------------------------------------------------------------------------------------------
@@ -269,14 +223,11 @@ class OnoTokensGrad(C.Structure):
     ]
 
 
-class OnoClipTensor(C.Structure):
-    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("n", C.c_longlong), ("g_dtype", C.c_int), ("out_dtype", C.c_int)]
-
-
 class OnoClip(C.Structure):
     _fields_ = [
-        ("t", C.POINTER(OnoClipTensor)), ("n_tensors", C.c_int), ("scale", C.c_float), ("max_norm", C.c_float),
-        ("norm", C.c_void_p), ("coef", C.c_void_p), ("write", C.c_int), ("scratch", C.c_void_p), ("scratch_bytes", C.c_longlong),
+        ("n_tensors", C.c_int), ("g", C.c_void_p), ("out", C.c_void_p), ("n", C.c_void_p), ("types", C.c_char_p),
+        ("scale", C.c_float), ("max_norm", C.c_float), ("norm", C.c_void_p), ("coef", C.c_void_p),
+        ("scratch", C.c_void_p), ("scratch_bytes", C.c_longlong),
     ]
 
 

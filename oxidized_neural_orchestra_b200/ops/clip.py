@@ -7,12 +7,29 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 
 import torch
 
 from . import _lib
+from ._launch import launch, one_device, scratch as scratch_for
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _types(ts: list[torch.Tensor]) -> bytes:
+    if not all([t.is_contiguous() for t in ts]):
+        raise ValueError("gradients must be contiguous")
+    kinds = {t.dtype for t in ts}
+    if not kinds <= _DTYPE.keys():
+        raise TypeError("gradients must be float32, bfloat16 or float16")
+    return bytes([_DTYPE[t.dtype] for t in ts]) if len(kinds) > 1 else bytes([_DTYPE[k] for k in kinds]) * len(ts)
+
+
+def _mixed(types: bytes, out_types: bytes) -> bytes:
+    if len(types) and types == types[:1] * len(types) and out_types == out_types[:1] * len(types):
+        return bytes([types[0] | out_types[0] << 2]) * len(types)
+    return bytes([i | j << 2 for i, j in zip(types, out_types)])
 
 
 def _one(t: torch.Tensor | None, what: str) -> int | None:
@@ -23,43 +40,45 @@ def _one(t: torch.Tensor | None, what: str) -> int | None:
     return t.data_ptr()
 
 
-def _clip(grads, outs, norm, coef, max_norm: float, scale: float, scratch, stream) -> None:
+def _clip(grads, outs, write: bool, norm, coef, max_norm: float, scale: float, scratch, stream) -> None:
     if isinstance(grads, torch.Tensor) or isinstance(outs, torch.Tensor):
         raise TypeError("gradients come as a list of tensors")
     grads = list(grads)
     if not (max_norm > 0.0) or not math.isfinite(scale):
         raise ValueError("max_norm must be positive and scale finite")
-    if outs is not None:
-        outs = list(outs)
-        if len(outs) != len(grads):
-            raise ValueError("one output for each gradient")
-        for g, o in zip(grads, outs):
-            if o.shape != g.shape or o.dtype != g.dtype and o.data_ptr() == g.data_ptr() != 0:
-                raise ValueError("an output has its gradient's shape, and over the gradient its type")
-        at = [o.data_ptr() for o in outs if o.numel()]
-        if len(set(at)) != len(at):
+    # (hundreds of tensors are common: lists of what is asked of all of them, rather than a look at each)
+    types, at, sizes, n = _types(grads), [t.data_ptr() for t in grads], [t.numel() for t in grads], len(grads)
+    to, out_types = [], types
+    if write:
+        if outs is None:
+            to = at
+        else:
+            outs = list(outs)
+            if len(outs) != n:
+                raise ValueError("one output for each gradient")
+            out_types, to = _types(outs), [t.data_ptr() for t in outs]
+            if [t.numel() for t in outs] != sizes:
+                raise ValueError("an output has as many values as its gradient")
+            if types != out_types and any([p == q != 0 and i != j for p, q, i, j in zip(at, to, types, out_types)]):
+                raise ValueError("an output over its gradient has the gradient's type")
+        there = to if all(to) else [p for p in to if p]
+        if len(set(there)) != len(there):
             raise ValueError("two outputs at one place")
-    for t in grads if outs is None else grads + outs:
-        if t.dtype not in _DTYPE:
-            raise TypeError("gradients must be float32, bfloat16 or float16")
-        if not t.is_contiguous():
-            raise ValueError("gradients must be contiguous")
     home = norm if norm is not None else coef if coef is not None else grads[0] if grads else None
     if home is None:
         return
-    _lib.one_device(home, *grads, *(outs or ()), norm, coef, scratch)
-    lib = _lib.load()
-    n = len(grads)
-    arr = (_lib.OnoClipTensor * n)(*[
-        (g.data_ptr(), None if outs is None else outs[k].data_ptr(), g.numel(), _DTYPE[g.dtype], 0 if outs is None else _DTYPE[outs[k].dtype])
-        for k, g in enumerate(grads)])
+    one_device(home, norm, coef, scratch)
+    home_at = home.get_device()
+    if any([t.get_device() != home_at for t in grads]) or outs and any([t.get_device() != home_at for t in outs]):
+        raise ValueError("tensors on different devices")
     if scratch is None:
-        scratch = _lib.scratch(home, lib.ono_clip_scratch(), stream)
+        scratch = scratch_for(home, clip_scratch(), stream)
     elif not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous")
-    c = _lib.OnoClip(arr, n, scale, max_norm, _one(norm, "norm"), _one(coef, "coef"), outs is not None, scratch.data_ptr(),
-                     scratch.numel() * scratch.element_size())
-    _lib.launch(home, stream, "ono_clip", C.byref(c))
+    words = [array("q", v) for v in (at, to, sizes)]
+    c = _lib.OnoClip(n, words[0].buffer_info()[0], words[1].buffer_info()[0] if write else None, words[2].buffer_info()[0], _mixed(types, out_types),
+                     scale, max_norm, _one(norm, "norm"), _one(coef, "coef"), scratch.data_ptr(), scratch.numel() * scratch.element_size())
+    launch(home, stream, "ono_clip", C.byref(c))
 
 
 def clip_scratch() -> int:
@@ -72,12 +91,11 @@ def grad_norm(grads: list[torch.Tensor], norm: torch.Tensor, *, max_norm: float 
     """``norm[0] = |scale| * sqrt(sum over all gradients of g^2)`` and, if wanted, ``coef[0]``, what clipping to ``max_norm`` multiplies the
     scaled gradients by: 1 up to ``max_norm``, ``max_norm / norm`` above (0 for an infinite norm, NaN for a NaN). ``elementwise.optim_step``
     takes it as ``grad_coef``: the step then clips as it goes, without a pass over the gradients."""
-    _clip(grads, None, norm, coef, max_norm, scale, scratch, stream)
+    _clip(grads, None, False, norm, coef, max_norm, scale, scratch, stream)
 
 
 def clip_grads(grads: list[torch.Tensor], max_norm: float, *, scale: float = 1.0, norm: torch.Tensor | None = None,
                coef: torch.Tensor | None = None, out: list[torch.Tensor] | None = None, scratch: torch.Tensor | None = None, stream=None) -> None:
-    """``out[k] = coef * scale * grads[k]`` (None: in place), coef as in ``grad_norm``, rounded once to the output's type: the gradients
+    """``out[k] = coef * scale * grads[k]`` (None: in place; else as many values, in their order), coef as in ``grad_norm``, rounded once to the output's type: the gradients
     clipped together, into another type on the way if wanted (a 16-bit wire)."""
-    grads = list(grads)
-    _clip(grads, grads if out is None else out, norm, coef, max_norm, scale, scratch, stream)
+    _clip(grads, out, True, norm, coef, max_norm, scale, scratch, stream)

@@ -9,22 +9,24 @@ import ctypes as C
 import torch
 
 from . import _lib
+from ._launch import launch, one_device, rows_of, scratch as scratch_for, status_ptr
 
 NO_PADDING = -(2**63)
+_IDS = {torch.int32: 0, torch.int64: 1}
 
 
-def _rows(t: torch.Tensor, what: str, dtypes=(torch.float32, torch.bfloat16)) -> None:
-    if t.dtype not in dtypes:
-        raise TypeError(f"{what} must be {' or '.join(str(d)[6:] for d in dtypes)}")
-    if t.dim() != 2 or t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < t.shape[1] and t.shape[0] > 1:
-        raise ValueError(f"{what} must be 2-D rows with unit inner stride")
-
-
-def _ids(ids: torch.Tensor, n: int) -> None:
-    if ids.dtype not in (torch.int32, torch.int64):
+def _ids(ids: torch.Tensor, n: int) -> int:
+    wide = _IDS.get(ids.dtype)
+    if wide is None:
         raise TypeError("ids must be int32 or int64")
-    if not ids.is_contiguous() or ids.numel() != n:
+    if ids.numel() != n or not ids.is_contiguous():
         raise ValueError(f"ids must be contiguous, one for each of the {n} rows")
+    return wide
+
+
+def _sizes(vocab: int, width: int) -> None:
+    if vocab >= 2**31 - 1 or width >= 2**31 - 16:
+        raise ValueError("a table has less than 2^31 rows and columns")
 
 
 def embedding(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, *, scale: float = 1.0, padding_id: int | None = -1,
@@ -33,19 +35,21 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, *, scal
 
     An id equal to ``padding_id`` (None: there is none) stands for no token: its row is zeros. So is that of any other id
     outside the table, and then ``status`` (int32[1]) becomes non-zero."""
-    _rows(table, "table")
-    _rows(out, "out")
+    ld_table, ld_out = rows_of(table, "table"), rows_of(out, "out")
     n, width = out.shape
-    _ids(ids, n)
+    vocab = table.shape[0]
+    wide = _ids(ids, n)
     if table.shape[1] != width:
         raise ValueError(f"table rows have {table.shape[1]} values, out rows {width}")
-    _lib.one_device(table, ids, out, status)
+    _sizes(vocab, width)
+    one_device(table, ids, out, status)
     if n == 0 or width == 0:
         return
-    e = _lib.OnoEmbedding(table.data_ptr(), ids.data_ptr(), out.data_ptr(), n, _lib.pitch(table), _lib.pitch(out),
-                          NO_PADDING if padding_id is None else padding_id, table.shape[0], width, table.dtype == torch.bfloat16,
-                          out.dtype == torch.bfloat16, ids.dtype == torch.int64, scale, _lib.status_ptr(status))
-    _lib.launch(table, stream, "ono_embedding", C.byref(e))
+    if vocab == 0:
+        raise ValueError("a table without rows")
+    e = _lib.OnoEmbedding(table.data_ptr(), ids.data_ptr(), out.data_ptr(), n, ld_table, ld_out, NO_PADDING if padding_id is None else padding_id,
+                          vocab, width, table.dtype == torch.bfloat16, out.dtype == torch.bfloat16, wide, scale, status_ptr(status))
+    launch(table, stream, "ono_embedding", C.byref(e))
 
 
 def embedding_grad_scratch(n: int, vocab: int, width: int) -> int:
@@ -62,24 +66,23 @@ def embedding_grad(d: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, *, sc
 
     Sums are f32 and go over the tokens in one order that depends on the ids alone: the same bits every time. ``scratch``: a
     contiguous tensor of at least ``embedding_grad_scratch`` bytes that no overlapping call uses (None: allocated for this call)."""
-    _rows(d, "d")
-    _rows(grad, "grad", (torch.float32,))
+    ld_d, ld_grad = rows_of(d, "d"), rows_of(grad, "grad", (torch.float32,))
     n, width = d.shape
     vocab = grad.shape[0]
-    _ids(ids, n)
+    wide = _ids(ids, n)
     if grad.shape[1] != width:
         raise ValueError(f"d rows have {width} values, grad rows {grad.shape[1]}")
     if scratch is not None and not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous")
-    _lib.one_device(d, ids, grad, status, scratch)
+    _sizes(vocab, width)
+    one_device(d, ids, grad, status, scratch)
     if vocab == 0 or width == 0:
         return
     if scratch is None:
         need = embedding_grad_scratch(n, vocab, width)
         if need:
-            scratch = _lib.scratch(grad, need, stream)
-    e = _lib.OnoEmbeddingGrad(d.data_ptr(), ids.data_ptr(), grad.data_ptr(), n, _lib.pitch(d), _lib.pitch(grad),
-                              NO_PADDING if padding_id is None else padding_id, vocab, width, d.dtype == torch.bfloat16,
-                              ids.dtype == torch.int64, accumulate, scale, _lib.status_ptr(status), None if scratch is None else scratch.data_ptr(),
-                              0 if scratch is None else scratch.numel() * scratch.element_size())
-    _lib.launch(grad, stream, "ono_embedding_grad", C.byref(e))
+            scratch = scratch_for(grad, need, stream)
+    e = _lib.OnoEmbeddingGrad(d.data_ptr(), ids.data_ptr(), grad.data_ptr(), n, ld_d, ld_grad, NO_PADDING if padding_id is None else padding_id,
+                              vocab, width, d.dtype == torch.bfloat16, wide, accumulate, scale, status_ptr(status),
+                              None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel() * scratch.element_size())
+    launch(grad, stream, "ono_embedding_grad", C.byref(e))

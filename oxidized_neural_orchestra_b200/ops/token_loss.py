@@ -14,7 +14,10 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .embedding import NO_PADDING, _rows
+from ._launch import launch, one_device, rows_of, status_ptr
+
+NO_TARGET = -(2**63)
+_TARGETS = {torch.int32: 0, torch.int64: 1}
 
 TOP_MAX = 32
 
@@ -27,28 +30,38 @@ def _column(t: torch.Tensor | None, rows: int, what: str) -> int | None:
     return t.data_ptr()
 
 
-def _targets(t: torch.Tensor | None, rows: int) -> None:
+def _targets(t: torch.Tensor | None, rows: int) -> int:
     if t is None:
-        return
-    if t.dtype not in (torch.int32, torch.int64):
+        return 0
+    wide = _TARGETS.get(t.dtype)
+    if wide is None:
         raise TypeError("targets must be int32 or int64")
     if t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
         raise ValueError(f"targets must be a contiguous vector of {rows} values")
+    return wide
 
 
-def _out(out: torch.Tensor, logits: torch.Tensor) -> None:
-    _rows(out, "out")
+def _logits(t: torch.Tensor) -> int:
+    pitch = rows_of(t, "logits")
+    if t.shape[1] >= 2**31 - 16:
+        raise ValueError("a vocabulary has less than 2^31 tokens")
+    return pitch
+
+
+def _out(out: torch.Tensor, logits: torch.Tensor) -> int:
+    pitch = rows_of(out, "out")
     if out.shape != logits.shape:
         raise ValueError("out must have the logits' shape")
     if out.data_ptr() == logits.data_ptr() and (out.dtype != logits.dtype or out.stride(0) != logits.stride(0)):
         raise ValueError("out over the logits needs the same type and rows")
+    return pitch
 
 
-def _tokens(logits, targets, ignore_id, status, stream, *, logp=None, lse=None, entropy=None, top_logp=None, top_id=None, out=None, weight=None,
-            scale=1.0) -> None:
-    _rows(logits, "logits")
+def _tokens(logits, targets, ignore_id, status, stream, *, logp=None, lse=None, entropy=None, top_logp=None, top_id=None, out=None, ld_out=0,
+            weight=None, scale=1.0) -> None:
+    ld = _logits(logits)
     rows, vocab = logits.shape
-    _targets(targets, rows)
+    wide = _targets(targets, rows)
     top = 0
     if top_logp is not None or top_id is not None:
         if top_logp is None or top_id is None or top_logp.dtype != torch.float32 or top_id.dtype != torch.int32:
@@ -58,18 +71,17 @@ def _tokens(logits, targets, ignore_id, status, stream, *, logp=None, lse=None, 
         top = top_logp.shape[1]
         if top > min(TOP_MAX, vocab):
             raise ValueError(f"at most {min(TOP_MAX, vocab)} alternatives")
-    _lib.one_device(logits, targets, status, logp, lse, entropy, top_logp, top_id, out, weight)
-    a = _lib.OnoTokens(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, _lib.pitch(logits),
-                       0 if out is None else _lib.pitch(out), NO_PADDING if ignore_id is None else ignore_id, vocab,
-                       logits.dtype == torch.bfloat16, targets is not None and targets.dtype == torch.int64, top,
-                       _column(logp, rows, "logp"), _column(lse, rows, "lse"), _column(entropy, rows, "entropy"),
-                       top_logp.data_ptr() if top else None, top_id.data_ptr() if top else None, None if out is None else out.data_ptr(),
-                       out is not None and out.dtype == torch.bfloat16, _column(weight, rows, "weight"), scale, _lib.status_ptr(status))
+    one_device(logits, targets, status, logp, lse, entropy, top_logp, top_id, out, weight)
+    a = _lib.OnoTokens(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, ld, ld_out, NO_TARGET if ignore_id is None else ignore_id,
+                       vocab, logits.dtype == torch.bfloat16, wide, top, _column(logp, rows, "logp"), _column(lse, rows, "lse"),
+                       _column(entropy, rows, "entropy"), top_logp.data_ptr() if top else None, top_id.data_ptr() if top else None,
+                       None if out is None else out.data_ptr(), out is not None and out.dtype == torch.bfloat16, _column(weight, rows, "weight"),
+                       scale, status_ptr(status))
     if rows == 0:
         return
     if vocab == 0:
         raise ValueError("logits of no tokens")
-    _lib.launch(logits, stream, "ono_tokens", C.byref(a))
+    launch(logits, stream, "ono_tokens", C.byref(a))
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None, *, logp: torch.Tensor | None = None, lse: torch.Tensor | None = None,
@@ -91,8 +103,7 @@ def token_loss(logits: torch.Tensor, targets: torch.Tensor, *, out: torch.Tensor
     ``out`` may be ``logits``) and the rows' ``logp``, in one call: elementwise.loss_backward's counterpart for integer targets."""
     if targets is None:
         raise ValueError("a token loss needs targets")
-    _out(out, logits)
-    _tokens(logits, targets, ignore_id, status, stream, logp=logp, lse=lse, out=out, weight=weight, scale=scale)
+    _tokens(logits, targets, ignore_id, status, stream, logp=logp, lse=lse, out=out, ld_out=_out(out, logits), weight=weight, scale=scale)
 
 
 def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, *, lse: torch.Tensor, out: torch.Tensor,
@@ -100,22 +111,21 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, *, l
                         ignore_id: int | None = -1, status: torch.Tensor | None = None, stream=None) -> None:
     """The logits' gradient from those of ``token_logprobs``' results, ``lse`` and ``entropy`` being what it returned:
     ``out = d_logp (1[v = target] - p) - d_entropy p (ln p + entropy)``. ``out`` may be ``logits``."""
-    _rows(logits, "logits")
+    ld = _logits(logits)
     rows, vocab = logits.shape
-    _targets(targets, rows)
-    _out(out, logits)
+    wide = _targets(targets, rows)
+    ld_out = _out(out, logits)
     if d_logp is None and d_entropy is None:
         raise ValueError("d_logp, d_entropy or both")
     if d_logp is not None and targets is None:
         raise ValueError("d_logp needs targets")
     if (entropy is None) != (d_entropy is None):
         raise ValueError("d_entropy needs the entropy, which has no other use")
-    _lib.one_device(logits, targets, status, lse, entropy, d_logp, d_entropy, out)
-    a = _lib.OnoTokensGrad(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, _lib.pitch(logits), _lib.pitch(out),
-                           NO_PADDING if ignore_id is None else ignore_id, vocab, logits.dtype == torch.bfloat16,
-                           targets is not None and targets.dtype == torch.int64, _column(lse, rows, "lse"), _column(entropy, rows, "entropy"),
+    one_device(logits, targets, status, lse, entropy, d_logp, d_entropy, out)
+    a = _lib.OnoTokensGrad(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, ld, ld_out, NO_TARGET if ignore_id is None else ignore_id,
+                           vocab, logits.dtype == torch.bfloat16, wide, _column(lse, rows, "lse"), _column(entropy, rows, "entropy"),
                            _column(d_logp, rows, "d_logp"), _column(d_entropy, rows, "d_entropy"), out.data_ptr(), out.dtype == torch.bfloat16,
-                           _lib.status_ptr(status))
+                           status_ptr(status))
     if rows == 0 or vocab == 0:
         return
-    _lib.launch(logits, stream, "ono_tokens_grad", C.byref(a))
+    launch(logits, stream, "ono_tokens_grad", C.byref(a))

@@ -86,8 +86,8 @@ def test_tokens():
     with pytest.raises(ValueError):
         token_logprobs_grad(x, t, lse=v, d_logp=v, entropy=v, out=x)
     with pytest.raises(TypeError, match="status"):
-        from oxidized_neural_orchestra_b200.ops import _lib
-        _lib.status_ptr(v)
+        from oxidized_neural_orchestra_b200.ops._launch import status_ptr
+        status_ptr(v)
 
 
 def test_clip():
@@ -109,7 +109,7 @@ def test_clip():
             grad_norm(bad, n)
     with pytest.raises(TypeError):
         grad_norm(torch.zeros(4), n)
-    for out in ([torch.zeros(4)], [torch.zeros(4), torch.zeros(3, 2)], [g[0].view(torch.bfloat16)[:4], torch.zeros(2, 3)]):
+    for out in ([torch.zeros(4)], [torch.zeros(4), torch.zeros(3, 3)], [g[0].view(torch.bfloat16)[:4], torch.zeros(2, 3)]):
         with pytest.raises(ValueError):
             clip_grads(g, 1.0, out=out)
     with pytest.raises(ValueError, match="one place"):
