@@ -150,32 +150,38 @@ __device__ __forceinline__ unsigned int token_key(const OnoEmbeddingGrad& e, uns
   return r < 0 ? (unsigned int)e.vocab : (unsigned int)r;
 }
 
-// Few places: each finds its rank by comparing with all of them, four threads a place. One launch, no pass waits for another.
-constexpr int RANK_MAX = 4096, RANK_PLACES = 64;
+// Few places: each finds its rank by comparing with all of them, RANK_THREADS threads a place. One launch, no pass waits for another.
+constexpr int RANK_MAX = 4096, RANK_THREADS = 16, RANK_PLACES = 256 / RANK_THREADS;
 template <typename I>
-__global__ void __launch_bounds__(4 * RANK_PLACES) embedding_rank_kernel(const __grid_constant__ GradDev p, int ctas) {
+__global__ void __launch_bounds__(256) embedding_rank_kernel(const __grid_constant__ GradDev p, int ctas) {
   __shared__ __align__(16) unsigned int s_key[RANK_MAX];
   const OnoEmbeddingGrad& e = p.e;
   if ((int)blockIdx.x >= ctas) { fill_zeros(e, blockIdx.x - ctas); return; }
   const int n = (int)e.n, nv = (n + 3) / 4;
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
-  for (int j = threadIdx.x; j < 4 * nv; j += 4 * RANK_PLACES) s_key[j] = j < n ? token_key<I>(e, j) : 0xffffffffu;
+#pragma unroll
+  for (int q = 0; q < RANK_MAX / 256; ++q) {      // (all loads at once)
+    const int j = threadIdx.x + q * 256;
+    if (j < 4 * nv) s_key[j] = j < n ? token_key<I>(e, j) : 0xffffffffu;
+  }
   __syncthreads();
-  const int i = blockIdx.x * RANK_PLACES + (threadIdx.x >> 2), part = threadIdx.x & 3;
+  const int i = blockIdx.x * RANK_PLACES + threadIdx.x / RANK_THREADS, part = threadIdx.x % RANK_THREADS;
   const uint4* keys = reinterpret_cast<const uint4*>(s_key);
   unsigned int rank = 0, key = 0;
   if (i < n) {
     key = s_key[i];
     const int vi = i >> 2;
 #pragma unroll 4
-    for (int v = part; v < vi; v += 4) { const uint4 k = keys[v]; rank += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key); }
+    for (int v = part; v < vi; v += RANK_THREADS) { const uint4 k = keys[v]; rank += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key); }
 #pragma unroll 4
-    for (int v = vi + 1 + part; v < nv; v += 4) { const uint4 k = keys[v]; rank += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key); }
-    const unsigned int k = s_key[4 * vi + part];
-    rank += k < key || (k == key && 4 * vi + part < i);
+    for (int v = vi + 1 + part; v < nv; v += RANK_THREADS) { const uint4 k = keys[v]; rank += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key); }
+    if (part < 4) {
+      const unsigned int k = s_key[4 * vi + part];
+      rank += k < key || (k == key && 4 * vi + part < i);
+    }
   }
-  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-  rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+#pragma unroll
+  for (int o = RANK_THREADS / 2; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
   if (i < n && part == 0) p.item[p.sorted][rank] = make_uint2(key, (unsigned int)i);
 }
 
@@ -238,7 +244,7 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_scatter_kernel(const _
   }
   // a digit a thread: its places in the tiles before, and in all
   unsigned int before = 0, all = 0;
-#pragma unroll 8
+#pragma unroll 16
   for (int t = 0; t < p.tiles; ++t) {
     const unsigned int h = __ldg(hist + t * SORT_RADIX + tid);
     if (t < (int)blockIdx.x) before += h;
@@ -281,35 +287,62 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_scatter_kernel(const _
 // Second launch: a warp adds up the rows of a chunk of `chunk` sorted places, 32 * VEC columns of them. A run of equal tokens belongs to
 // the chunk it starts in, whose warp follows it into the next chunk if it ends there. A longer run is summed chunk by chunk: part[c][1]
 // has the sum of what starts in c, part[c][0] of what comes from before; the third launch adds them in order.
-// Whether the run of token k that starts in the chunk before place b and reaches it is one of the long ones.
-__device__ __forceinline__ bool long_run(const uint2* item, unsigned int n, unsigned int b, unsigned int chunk, unsigned int k) {
-  return b + chunk <= n && item[b + chunk - 1].x == k;
-}
-
-template <int VEC>
-struct GradVec {      // what a lane has of an f32 row: 16-byte accesses where the row is aligned and the lane's columns are all there
-  static __device__ __forceinline__ void load(float (&v)[VEC], const float* p, int left, bool aligned) {
-    if (VEC > 1 && aligned && left >= VEC) {
+// A lane's values of a row: VEC of them, one behind the other (STEP 1, where rows are aligned) or every 32nd (STEP 32). `left`: columns from the first
+// of them on.
+template <typename T, int VEC, int STEP>
+struct RowPart {
+  static constexpr int WORDS = STEP == 1 ? 4 : VEC;
+  uint32_t w[WORDS];
+  static __device__ __forceinline__ int column(int tile, int lane) { return tile * 32 * VEC + (STEP == 1 ? lane * VEC : lane); }
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if constexpr (STEP == 1) {
+      static_assert(VEC * sizeof(T) == 16, "16 bytes");
+      if (left >= VEC) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      } else {
+        T* t = reinterpret_cast<T*>(w);
 #pragma unroll
-      for (int k = 0; k < VEC; k += 4) { const float4 w = *reinterpret_cast<const float4*>(p + k); v[k] = w.x; v[(k + 1) % VEC] = w.y; v[(k + 2) % VEC] = w.z; v[(k + 3) % VEC] = w.w; }
+        for (int k = 0; k < VEC; ++k) t[k] = k < left ? p[k] : from_f32<T>(0.0f);
+      }
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = k < left ? p[k] : 0.0f;
+      for (int k = 0; k < VEC; ++k) w[k] = k * STEP < left ? __float_as_uint(to_f32(p[k * STEP])) : 0u;
+    }
+  }
+  __device__ __forceinline__ void add_to(float (&acc)[VEC]) const {
+    if constexpr (STEP == 1) {
+      add_piece<T, VEC>(acc, make_uint4(w[0], w[1], w[2], w[3]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += __uint_as_float(w[k]);
+    }
+  }
+};
+template <int VEC, int STEP>
+struct GradVec {      // the same of an f32 row; 16-byte accesses where it is aligned and the lane's columns are all there
+  static __device__ __forceinline__ void load(float (&v)[VEC], const float* p, int left, bool aligned) {
+    if (STEP == 1 && aligned && left >= VEC) {
+#pragma unroll
+      for (int k = 0; k < VEC; k += 4) { const float4 w = *reinterpret_cast<const float4*>(p + k); v[k] = w.x; v[k + 1] = w.y; v[k + 2] = w.z; v[k + 3] = w.w; }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = k * STEP < left ? p[k * STEP] : 0.0f;
     }
   }
   static __device__ __forceinline__ void store(float* p, const float (&v)[VEC], int left, bool aligned) {
-    if (VEC > 1 && aligned && left >= VEC) {
+    if (STEP == 1 && aligned && left >= VEC) {
 #pragma unroll
-      for (int k = 0; k < VEC; k += 4) *reinterpret_cast<float4*>(p + k) = make_float4(v[k], v[(k + 1) % VEC], v[(k + 2) % VEC], v[(k + 3) % VEC]);
+      for (int k = 0; k < VEC; k += 4) *reinterpret_cast<float4*>(p + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) if (k < left) p[k] = v[k];
+      for (int k = 0; k < VEC; ++k) if (k * STEP < left) p[k * STEP] = v[k];
     }
   }
 };
 
 // U rows are in flight; with ACC those of the table that they are added to as well.
-template <typename T, int VEC, bool ACC, int U>
+template <typename T, int VEC, int STEP, bool ACC, int U>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constant__ GradDev p, int tiles) {
   const OnoEmbeddingGrad& e = p.e;
   const unsigned int n = (unsigned int)e.n, L = (unsigned int)p.chunk, none = (unsigned int)e.vocab;
@@ -317,7 +350,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
   const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const unsigned int c = (unsigned int)(job / tiles);
-  const int tile = (int)(job - (long long)c * tiles), col = (tile * 32 + lane) * VEC, left = e.width - col;
+  const int tile = (int)(job - (long long)c * tiles), col = RowPart<T, VEC, STEP>::column(tile, lane), left = e.width - col;
   const bool aligned = (((uintptr_t)e.grad | (uintptr_t)(e.ld_grad * 4)) & 15) == 0;
   if ((unsigned long long)c * L >= n) return;
   const unsigned int s = c * L, own = min(n, s + L);
@@ -328,7 +361,8 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
   unsigned int at = s;
   if (from_before) {
     const bool just_before = s == L || item[s - L].x != k0 || item[s - L - 1].x != k0;      // it starts in the chunk before
-    if (just_before && !long_run(item, n, s, L, k0)) {                                 // whose warp finishes it
+    const bool is_long = s + L <= n && kl == k0;                                           // and fills this one, so that all of it goes by chunks
+    if (just_before && !is_long) {                                                         // that chunk's warp finishes it
       if (kl == k0) return;
       for (bool found = false; !found; ) {
         const unsigned int j = at + lane;
@@ -341,7 +375,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
   const bool head = from_before && at == s;      // a piece of a run that started earlier
   bool tail_long = false;
   if (goes_on && !(head && kl == k0) && kl != none) {
-    tail_long = long_run(item, n, own, L, kl);
+    tail_long = own + L <= n && item[own + L - 1].x == kl;      // the run fills the next chunk
     if (!tail_long) {
       end = min(n, own + L);      // this warp finishes it; it stops at the next token
     } else if (tile == 0) {       // where it ends: the last place of token kl, 32 probes at a time
@@ -368,11 +402,11 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
   auto flush = [&](bool tail) {
     if (cur == none || left <= 0) return;
     if (piece || (tail && tail_long)) {
-      GradVec<VEC>::store(p.part + ((long long)c * 2 + (piece ? 0 : 1)) * p.pitch + col, acc, left, true);
+      GradVec<VEC, STEP>::store(p.part + ((long long)c * 2 + (piece ? 0 : 1)) * p.pitch + col, acc, left, true);
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] = ACC ? old[k] + e.scale * acc[k] : e.scale * acc[k];
-      GradVec<VEC>::store(e.grad + (long long)cur * e.ld_grad + col, acc, left, aligned);
+      GradVec<VEC, STEP>::store(e.grad + (long long)cur * e.ld_grad + col, acc, left, aligned);
     }
   };
   for (unsigned int j0 = at; j0 < end; j0 += 32) {
@@ -381,8 +415,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
     const unsigned int kj = ij.x, pj = ij.y;
     const int m = (int)min(32u, end - j0);
     for (int q0 = 0; q0 < m; q0 += U) {
-      uint4 w[U];
-      float f[U][1];
+      RowPart<T, VEC, STEP> w[U];
       float was[ACC ? U : 1][VEC];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -390,17 +423,8 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
         const unsigned int k = __shfl_sync(0xffffffffu, kj, q & 31), from = __shfl_sync(0xffffffffu, pj, q & 31);
         const unsigned int kp = __shfl_sync(0xffffffffu, kj, (q - 1) & 31);
         if (q < m && k != none && left > 0) {
-          const T* row = reinterpret_cast<const T*>(e.d) + (long long)from * e.ld_d + col;
-          if constexpr (VEC == 1) {
-            f[u][0] = to_f32(*row);
-          } else if (left >= VEC) {
-            w[u] = __ldg(reinterpret_cast<const uint4*>(row));
-          } else {
-            T* t = reinterpret_cast<T*>(&w[u]);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) t[i] = i < left ? row[i] : from_f32<T>(0.0f);
-          }
-          if (ACC && (q == 0 || kp != k)) GradVec<VEC>::load(was[ACC ? u : 0], e.grad + (long long)k * e.ld_grad + col, left, aligned);
+          w[u].load(reinterpret_cast<const T*>(e.d) + (long long)from * e.ld_d + col, left);
+          if (ACC && (q == 0 || kp != k)) GradVec<VEC, STEP>::load(was[ACC ? u : 0], e.grad + (long long)k * e.ld_grad + col, left, aligned);
         }
       }
 #pragma unroll
@@ -416,10 +440,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
 #pragma unroll
           for (int i = 0; i < VEC; ++i) { acc[i] = 0.0f; if (ACC) old[i] = was[ACC ? u : 0][i]; }
         }
-        if (left > 0) {
-          if constexpr (VEC == 1) acc[0] += f[u][0];
-          else add_piece<T, VEC>(acc, w[u]);
-        }
+        if (left > 0) w[u].add_to(acc);
       }
     }
   }
@@ -429,9 +450,9 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
 // Very few places: no sorting. A warp takes a place and 32 * VEC columns, looks for the place's token among all, and where the place is the
 // token's first adds up its rows, U in flight. The other CTAs fill the rows of the table that no token means with zeros. One launch.
 constexpr int FEW_MAX = 512, FEW_VALUES = 1 << 14;      // FEW_VALUES: zeros of a CTA
-template <typename T, int VEC, typename I>
+template <typename T, int VEC, int STEP, typename I>
 __global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGrad e, int tiles, int ctas) {
-  constexpr int U = 16, WORDS = FEW_MAX / 32;
+  constexpr int U = STEP == 1 ? 16 : 8, WORDS = FEW_MAX / 32;
   __shared__ unsigned int s_word[8 * FEW_MAX / 2];      // rows with a token, or the warps' lists of 16 bits a place
   static_assert(FEW_VALUES / 32 + 1 <= 8 * FEW_MAX / 2, "a bit for each of a CTA's rows");
   const I* ids = reinterpret_cast<const I*>(e.ids);
@@ -469,7 +490,7 @@ __global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGr
     return;
   }
   const long long job = (long long)blockIdx.x * 8 + warp;
-  const int i = (int)(job / tiles), col = ((int)(job - (long long)i * tiles) * 32 + lane) * VEC, left = e.width - col;
+  const int i = (int)(job / tiles), col = RowPart<T, VEC, STEP>::column((int)(job - (long long)i * tiles), lane), left = e.width - col;
   if (i >= n) return;
   const I id = ids[i];
   unsigned int same[WORDS];
@@ -497,38 +518,23 @@ __global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGr
   float acc[VEC], old[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-  if (e.accumulate) GradVec<VEC>::load(old, g, left, aligned);
+  if (e.accumulate) GradVec<VEC, STEP>::load(old, g, left, aligned);
   for (int q0 = 0; q0 < count; q0 += U) {
-    uint4 w[U];
-    float f[U];
+    RowPart<T, VEC, STEP> w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (q0 + u >= count) continue;
-      const T* src = reinterpret_cast<const T*>(e.d) + (long long)list[q0 + u] * e.ld_d + col;
-      if (VEC == 1) {
-        f[u] = to_f32(*src);
-      } else if (left >= VEC) {
-        w[u] = __ldg(reinterpret_cast<const uint4*>(src));
-      } else {
-        T* t = reinterpret_cast<T*>(&w[u]);
+    for (int u = 0; u < U; ++u)
+      if (q0 + u < count) w[u].load(reinterpret_cast<const T*>(e.d) + (long long)list[q0 + u] * e.ld_d + col, left);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) t[k] = k < left ? src[k] : from_f32<T>(0.0f);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (q0 + u >= count) break;
-      if constexpr (VEC == 1) acc[0] += f[u];
-      else add_piece<T, VEC>(acc, w[u]);
-    }
+    for (int u = 0; u < U; ++u)
+      if (q0 + u < count) w[u].add_to(acc);
   }
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = e.accumulate ? old[k] + e.scale * acc[k] : e.scale * acc[k];
-  GradVec<VEC>::store(g, acc, left, aligned);
+  GradVec<VEC, STEP>::store(g, acc, left, aligned);
 }
 
 // Third launch: a block takes a long run's sums, 32 * VEC columns of them; its warps every JOIN_WARPS-th, then one adds up theirs.
-constexpr int JOIN_WARPS = 16;
+constexpr int JOIN_WARPS = 16, JOIN_LOADS = 2;
 template <int VEC>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const __grid_constant__ GradDev p, int tiles) {
   __shared__ float s_sum[JOIN_WARPS][32 * VEC];
@@ -543,12 +549,19 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const _
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
     if (left > 0) {
-#pragma unroll 8
-      for (unsigned int q = c + warp; q <= c1; q += JOIN_WARPS) {
-        float v[VEC];
-        GradVec<VEC>::load(v, p.part + ((long long)q * 2 + (q == c ? 1 : 0)) * p.pitch + col, left, true);
+      for (unsigned int q0 = c + warp; q0 <= c1; q0 += JOIN_LOADS * JOIN_WARPS) {
+        float v[JOIN_LOADS][VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+        for (int u = 0; u < JOIN_LOADS; ++u) {
+          const unsigned int q = q0 + u * JOIN_WARPS;
+          if (q <= c1) GradVec<VEC, 1>::load(v[u], p.part + ((long long)q * 2 + (q == c ? 1 : 0)) * p.pitch + col, VEC, true);      // (a row of sums is whole groups)
+        }
+#pragma unroll
+        for (int u = 0; u < JOIN_LOADS; ++u) {
+          if (q0 + u * JOIN_WARPS > c1) break;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
+        }
       }
     }
 #pragma unroll
@@ -557,7 +570,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const _
     if (warp == 0 && left > 0) {
       float* g = e.grad + (long long)p.item[p.sorted][c * L + L - 1].x * e.ld_grad + col;
       float old[VEC];
-      if (e.accumulate) GradVec<VEC>::load(old, g, left, aligned);
+      if (e.accumulate) GradVec<VEC, 1>::load(old, g, left, aligned);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         float t = 0.0f;
@@ -565,7 +578,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const _
         for (int w = 0; w < JOIN_WARPS; ++w) t += s_sum[w][lane * VEC + k];
         acc[k] = e.accumulate ? old[k] + e.scale * t : e.scale * t;
       }
-      GradVec<VEC>::store(g, acc, left, aligned);
+      GradVec<VEC, 1>::store(g, acc, left, aligned);
     }
     __syncthreads();
   }
@@ -656,7 +669,7 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
   p.pitch = g.pitch;
   const int esz = e->d_bf16 ? 2 : 4;
   const bool vec = ((uintptr_t)e->d & 15) == 0 && e->ld_d * esz % 16 == 0;
-  const int cols = 32 * (vec ? 16 / esz : 1), tiles = (e->width + cols - 1) / cols;
+  const int cols = 32 * (vec ? 16 / esz : 4), tiles = (e->width + cols - 1) / cols;
   const long long chunks = (e->n + g.chunk - 1) / g.chunk, blocks = (chunks * tiles + 7) / 8;
   if (blocks >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
   using B = __nv_bfloat16;
@@ -666,11 +679,11 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
     auto few = [&](auto kern) { kern<<<(unsigned)(ctas + zero), 256, 0, st>>>(*e, tiles, (int)ctas); };
     if (ctas + zero >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
     if (e->ids64) {
-      if (e->d_bf16) { if (vec) few(embedding_few_kernel<B, 8, long long>); else few(embedding_few_kernel<B, 1, long long>); }
-      else { if (vec) few(embedding_few_kernel<float, 4, long long>); else few(embedding_few_kernel<float, 1, long long>); }
+      if (e->d_bf16) { if (vec) few(embedding_few_kernel<B, 8, 1, long long>); else few(embedding_few_kernel<B, 4, 32, long long>); }
+      else { if (vec) few(embedding_few_kernel<float, 4, 1, long long>); else few(embedding_few_kernel<float, 4, 32, long long>); }
     } else {
-      if (e->d_bf16) { if (vec) few(embedding_few_kernel<B, 8, int>); else few(embedding_few_kernel<B, 1, int>); }
-      else { if (vec) few(embedding_few_kernel<float, 4, int>); else few(embedding_few_kernel<float, 1, int>); }
+      if (e->d_bf16) { if (vec) few(embedding_few_kernel<B, 8, 1, int>); else few(embedding_few_kernel<B, 4, 32, int>); }
+      else { if (vec) few(embedding_few_kernel<float, 4, 1, int>); else few(embedding_few_kernel<float, 4, 32, int>); }
     }
     if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad: %s", cudaGetErrorString(r), 0, 0); return -7; }
     return 0;
@@ -680,8 +693,8 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
   if (e->n <= RANK_MAX) {
     const int ctas = (int)((e->n + RANK_PLACES - 1) / RANK_PLACES);
     p.sorted = 0;
-    if (e->ids64) embedding_rank_kernel<long long><<<(unsigned)(ctas + zeros), 4 * RANK_PLACES, 0, st>>>(p, ctas);
-    else embedding_rank_kernel<int><<<(unsigned)(ctas + zeros), 4 * RANK_PLACES, 0, st>>>(p, ctas);
+    if (e->ids64) embedding_rank_kernel<long long><<<(unsigned)(ctas + zeros), 256, 0, st>>>(p, ctas);
+    else embedding_rank_kernel<int><<<(unsigned)(ctas + zeros), 256, 0, st>>>(p, ctas);
     r = cudaGetLastError();
   } else {
     const int need = 32 - __builtin_clz((unsigned)e->vocab);      // tokens, and `vocab` for none
@@ -709,11 +722,11 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
   if (e->n == 0) return 0;
   auto sum = [&](auto kern) { kern<<<(unsigned)blocks, 256, 0, st>>>(p, tiles); };
   if (e->accumulate) {
-    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, true, 4>); else sum(embedding_sum_kernel<B, 1, true, 8>); }
-    else { if (vec) sum(embedding_sum_kernel<float, 4, true, 4>); else sum(embedding_sum_kernel<float, 1, true, 8>); }
+    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, 1, true, 4>); else sum(embedding_sum_kernel<B, 4, 32, true, 4>); }
+    else { if (vec) sum(embedding_sum_kernel<float, 4, 1, true, 4>); else sum(embedding_sum_kernel<float, 4, 32, true, 4>); }
   } else {
-    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, false, 8>); else sum(embedding_sum_kernel<B, 1, false, 8>); }
-    else { if (vec) sum(embedding_sum_kernel<float, 4, false, 8>); else sum(embedding_sum_kernel<float, 1, false, 8>); }
+    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, 1, false, 8>); else sum(embedding_sum_kernel<B, 4, 32, false, 8>); }
+    else { if (vec) sum(embedding_sum_kernel<float, 4, 1, false, 8>); else sum(embedding_sum_kernel<float, 4, 32, false, 8>); }
   }
   if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad sum: %s", cudaGetErrorString(r), 0, 0); return -7; }
   if (e->n > g.chunk) {      // (a long run fills a whole chunk and begins ahead of it)
