@@ -17,124 +17,12 @@
 #include <algorithm>
 #include <atomic>
 
-#include "ono_kernels.h"
-#include "piece.cuh"
-#include "ptx.cuh"
+#include "token.cuh"
 
 namespace ono {
-void set_error(const char* fmt, const char* a, long long b, long long c);
-
-// What a launch computes: log probabilities, with entropy, with entropy and alternatives, the token loss's gradient, the gradient from
-// those of log probability and entropy.
-enum TokMode : int { TOK_LOGP, TOK_ENTROPY, TOK_TOP, TOK_LOSS, TOK_GRAD };
-
-struct TokDev {
-  const void* x; const void* targets;
-  long long R, ld, ld_out, ignore_id;
-  int V, targets64, top, per, staged;      // per: 16-byte groups of a row that a CTA takes; staged: they are kept in shared memory
-  float *logp, *lse, *entropy, *top_logp;
-  int* top_id;
-  void* out;
-  const float* weight;
-  float scale;
-  const float *lse_in, *entropy_in, *d_logp, *d_entropy;
-  int* status;
-};
-
-// lse comes rounded to f32: half a step of it is an error relative in p. Beyond this (2^-17 there) the gradient takes the row's maximum and sum
-// again; a row that is masked by the type's lowest value would have no sum at all beside it.
-constexpr float LSE_EXACT = 128.0f;
-constexpr int TOK_CTAS = 8;      // of a cluster, at most
-
-// 2^t
-__device__ __forceinline__ float exp2_of(float t) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
-  return r;
-}
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-__device__ __forceinline__ float exp_of(float d) { return exp2_of(d * LOG2E); }
-// Two values an instruction.
-__device__ __forceinline__ float2 fma_2(float2 a, float2 b, float2 c) {
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 z, x, y, z;\n\t"
-      "mov.b64 {%0, %1}, z;\n\t}"
-      : "=f"(a.x), "=f"(a.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return a;
-}
-__device__ __forceinline__ float2 mul_2(float2 a, float2 b) {
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(a.x), "=f"(a.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return a;
-}
-__device__ __forceinline__ float2 add_2(float2 a, float2 b) {
-  add_f32x2(a.x, a.y, b.x, b.y);
-  return a;
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-
-// A maximum beyond this in size, times log2 e, is rounded by more than a few hundredths (and may leave f32): such a row is gone through again.
-constexpr float TOK_FAR = 1e6f;
-// What exponents are taken relative to, in units of log2: the maximum's, of any size, rounded; a logit is then one multiply-add, and its error
-// that of the difference. Zero where there is nothing but far negative ones (all exponentials are zero then).
-__device__ __forceinline__ float shift_of(float m) { return m < -TOK_FAR ? 0.0f : m * LOG2E; }
-
-__device__ __forceinline__ uint4 load16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
 __device__ __forceinline__ void cp_async16(void* smem, const void* g) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(g) : "memory");
 }
-
-// Larger for a larger float. (-0 counts as 0.)
-__device__ __forceinline__ unsigned int order_of(float v) {
-  const unsigned int u = __float_as_uint(v + 0.0f);
-  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
-}
-__device__ __forceinline__ float of_order(unsigned int o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
-// ... and among equal logits for the lower index.
-__device__ __forceinline__ unsigned long long top_key(float v, int j) { return ((unsigned long long)order_of(v) << 32) | (0xffffffffu - (unsigned int)j); }
-
-template <typename T> struct TokVec;
-template <> struct TokVec<float> {
-  static constexpr int E = 4;
-  static __device__ __forceinline__ void get(const uint4& w, float (&v)[4]) {
-    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
-  }
-  static constexpr uint32_t NINF = 0xff800000u;      // a word of logits that are -inf
-  static __device__ __forceinline__ float most(const uint4& w) {
-    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
-  }
-  static __device__ __forceinline__ float most(const uint4 (&w)[4]) {
-    float m = __int_as_float(0xff800000);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) m = fmaxf(m, most(w[k]));
-    return m;
-  }
-};
-template <> struct TokVec<__nv_bfloat16> {
-  static constexpr int E = 8;
-  static __device__ __forceinline__ void get(const uint4& w, float (&v)[8]) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) { v[2 * k] = __uint_as_float(u[k] << 16); v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
-  }
-  static constexpr uint32_t NINF = 0xff80ff80u;
-  static __device__ __forceinline__ __nv_bfloat162 most2(const uint4& w) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  }
-  static __device__ __forceinline__ float most(const uint4& w) {
-    const __nv_bfloat162 m = most2(w);
-    return fmaxf(__low2float(m), __high2float(m));
-  }
-  static __device__ __forceinline__ float most(const uint4 (&w)[4]) {
-    const __nv_bfloat162 m = __hmax2(__hmax2(most2(w[0]), most2(w[1])), __hmax2(most2(w[2]), most2(w[3])));
-    return fmaxf(__low2float(m), __high2float(m));
-  }
-};
 
 template <int W>
 __device__ __forceinline__ void group_sync() {
@@ -402,20 +290,7 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
 #pragma unroll
             for (int k = 0; k < E; ++k) if (v * E + k - ph == t) w[k] += hit;
           }
-          O* o = d + (v * E - ph);
-          if constexpr (sizeof(O) == 4) {
-#pragma unroll
-            for (int k = 0; k < E; k += 4) *reinterpret_cast<float4*>(o + k) = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
-          } else {
-            uint32_t u[E / 2];
-#pragma unroll
-            for (int k = 0; k < E / 2; ++k) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(w[2 * k], w[2 * k + 1]);
-              u[k] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            if constexpr (E == 4) *reinterpret_cast<uint2*>(o) = make_uint2(u[0], u[1]);
-            else *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[E / 2 - 2], u[E / 2 - 1]);
-          }
+          store_group<O, E>(d + (v * E - ph), w);
         };
         int v = va + gt;
         for (; v + 3 * GT < vb; v += 4 * GT) {
@@ -699,14 +574,16 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
 // How a launch is laid out.
 struct TokShape { int warps, ctas, per, staged; size_t smem; };
 
-constexpr int TOK_WARP_ROW = 8192, TOK_SLICE = 32768;
+constexpr int TOK_SLICE = 32768;      // bytes of a row that is kept, to a CTA
 
 static TokShape tok_shape(long long rows, int V, int esz, int mode) {
-  const int E = 16 / esz;
-  const long long groups = ((long long)V + 2 * E - 2) / E, bytes = groups * 16;      // of a row that begins anywhere
+  const long long groups = tok_groups(V, esz), bytes = groups * 16;
   TokShape s = {};
   s.ctas = 1;
-  s.warps = bytes <= TOK_WARP_ROW ? 1 : 4;
+  // A warp to a row where there are rows for all of them: what a row costs beside its logits is then paid once (us, four warps against one:
+  // entropy of 47005 x 2322 f32 123.8, 69.9, of 8000 x 15000 bf16 51.2, 45.3; loss of 16000 x 5000 bf16 79.4, 67.7, but of 8000 x 8000 57.1, 60.7;
+  // entropy of 300 x 5000 4.8, 7.7).
+  s.warps = rows >= 16ll * ono_num_sms() && bytes <= (mode == TOK_LOSS ? 12288 : 32768) ? 1 : 4;
   if (s.warps > 1) {
     while (s.ctas < TOK_CTAS && ((mode == TOK_LOSS && bytes > (long long)TOK_SLICE * s.ctas) || (rows * s.ctas <= 4 * ono_num_sms() && bytes > 8192ll * s.ctas))) s.ctas *= 2;
   }
@@ -751,6 +628,7 @@ static cudaError_t tok_go(const TokDev& d, const TokShape& s, cudaStream_t st) {
 
 template <typename T, typename O, int MODE>
 static int tok_run(TokDev& d, cudaStream_t st) {
+  if (16 * tok_groups(d.V, sizeof(T)) <= (MODE == TOK_TOP ? TOK_SHORT_TOP : TOK_SHORT_ROW)) return tok_short(d, MODE, sizeof(T) == 2, sizeof(O) == 2, st);
   const TokShape s = tok_shape(d.R, d.V, sizeof(T), MODE);
   d.per = s.per;
   d.staged = s.staged;

@@ -1,0 +1,252 @@
+// The operators of token_loss.cu on short rows: a row lies in the registers of one warp, or of a few lanes of it, which load all of it at once.
+// Nothing is looped over and nothing goes through shared memory; a row costs its loads, a handful of shuffles and its stores, so that
+// what bounds it is memory or, of rows of a few logits, the launch and the latency of its one chain of loads.
+#include <type_traits>
+
+#include "token.cuh"
+
+namespace ono {
+
+// NV groups of 16 bytes to a lane. NV == 1: 2^lg lanes to a row, 32 >> lg rows to a warp.
+template <typename T, typename O, int MODE, int NV>
+__global__ void __launch_bounds__(256, NV == 1 ? 6 : 4) tok_short_kernel(const __grid_constant__ TokDev a, int lg) {
+  constexpr int E = TokVec<T>::E;
+  constexpr bool TOP = MODE == TOK_TOP, ENT = MODE == TOK_ENTROPY || MODE == TOK_TOP, FWD = MODE <= TOK_TOP;
+  const float ninf = __int_as_float(0xff800000);
+  const unsigned int full = 0xffffffffu;
+  const int lane = threadIdx.x & 31, G = NV == 1 ? 1 << lg : 32, gl = lane & (G - 1);
+  const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), r = NV == 1 ? (job << (5 - lg)) + (lane >> lg) : job;
+  const bool in = r < a.R;
+  const long long rr = in ? r : 0;
+  const T* const x = reinterpret_cast<const T*>(a.x) + rr * a.ld;
+  const int ph = (int)(((uintptr_t)x / sizeof(T)) & (E - 1));
+  long long raw = 0;
+  if (in && a.targets) raw = a.targets64 ? __ldg(reinterpret_cast<const long long*>(a.targets) + r) : (long long)__ldg(reinterpret_cast<const int*>(a.targets) + r);
+  // The ends of a row that begins anywhere: groups that are not whole. Where the row has that many lanes each takes a logit of either, else the
+  // lane of the group takes them one by one.
+  const bool split = G >= E;
+  const int tail = (ph + a.V) / E * E - ph, jh = gl - ph, jt = tail + gl;
+  const bool has_h = split && in && ph && gl < E && jh >= 0 && jh < a.V, has_t = split && in && gl < E && jt < a.V && (tail >= 0 || !ph);
+  const bool ends = __any_sync(full, has_h || has_t);
+  const float xh = has_h ? to_f32(x[jh]) : ninf, xt = has_t ? to_f32(x[jt]) : ninf;
+  uint4 w[NV];
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    const int j = (gl + q * G) * E - ph;
+    w[q] = make_uint4(TokVec<T>::NINF, TokVec<T>::NINF, TokVec<T>::NINF, TokVec<T>::NINF);
+    if (!in || j >= a.V) continue;
+    if (j >= 0 && j + E <= a.V) {
+      w[q] = load16(x + j);
+    } else if (!split) {
+      T* o = reinterpret_cast<T*>(&w[q]);
+#pragma unroll
+      for (int k = 0; k < E; ++k) if (j + k >= 0 && j + k < a.V) o[k] = x[j + k];
+    }
+  }
+  float i0 = 1.0f, i1 = 0.0f, i2 = 0.0f, i3 = 0.0f;
+  if (MODE == TOK_LOSS && a.weight) i0 = __ldg(a.weight + rr);
+  if (MODE == TOK_GRAD) {
+    i0 = __ldg(a.lse_in + rr);
+    if (a.d_logp) i1 = __ldg(a.d_logp + rr);
+    if (a.d_entropy) { i2 = __ldg(a.d_entropy + rr); i3 = __ldg(a.entropy_in + rr); }
+  }
+  int t = -1;      // the row counts for nothing
+  if (in && !(a.targets && raw == a.ignore_id)) {
+    if (raw >= 0 && raw < a.V) t = (int)raw;
+    else if (a.status && gl == 0) atomicExch(a.status, ONO_ERR_BAD_ARG);
+  }
+  const bool live = t >= 0;
+  float x_t = 0.0f;
+  if (MODE != TOK_GRAD && live && gl == 0) x_t = to_f32(x[t]);
+  auto group = [&](float v, auto join) {      // over the row's lanes
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) if (o < G) v = join(v, __shfl_xor_sync(full, v, o));
+    return v;
+  };
+  auto values = [&](auto f) {      // f(two logits, their places)
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      float o[E];
+      TokVec<T>::get(w[q], o);
+#pragma unroll
+      for (int k = 0; k < E; k += 2) f(make_float2(o[k], o[k + 1]), (gl + q * G) * E - ph + k, (gl + q * G) * E - ph + k + 1);
+    }
+    if (ends) f(make_float2(xh, xt), jh, jt);
+  };
+  float m = 0.0f, z = 1.0f, u = 0.0f, log_z = 0.0f;
+  bool far = false;
+  if (MODE != TOK_GRAD || __any_sync(full, live && fabsf(i0) > LSE_EXACT)) {
+    m = fmaxf(xh, xt);
+#pragma unroll
+    for (int q = 0; q < NV; ++q) m = fmaxf(m, TokVec<T>::most(w[q]));
+    m = group(m, [](float p, float q) { return fmaxf(p, q); });
+    far = fabsf(m) > TOK_FAR && m > ninf;      // (differences first then, see token_loss.cu)
+    const float at = shift_of(m);
+    if (!__any_sync(full, far)) {
+      float2 z2 = both(0.0f), u2 = both(0.0f);
+      values([&](float2 v, int, int) {
+        const float2 q = fma_2(v, both(LOG2E), both(-at)), e = make_float2(exp2_of(q.x), exp2_of(q.y));
+        z2 = add_2(z2, e);
+        if (ENT) u2 = fma_2(e, make_float2(fmaxf(q.x, -1e4f), fmaxf(q.y, -1e4f)), u2);
+      });
+      z = z2.x + z2.y;
+      u = u2.x + u2.y;
+    } else {
+      z = u = 0.0f;
+      values([&](float2 v, int, int) {
+        const float p = far ? (v.x - m) * LOG2E : fmaf(v.x, LOG2E, -at), q = far ? (v.y - m) * LOG2E : fmaf(v.y, LOG2E, -at), e = exp2_of(p), f = exp2_of(q);
+        z += e + f;
+        if (ENT) u += e * fmaxf(p, -1e4f) + f * fmaxf(q, -1e4f);
+      });
+    }
+    auto add = [](float p, float q) { return p + q; };
+    z = group(z, add);
+    if (ENT) u = group(u, add);
+    const bool empty = z == 0.0f;
+    const float log2_z = empty ? 0.0f : log2f(z);
+    log_z = (fabsf(m) <= TOK_FAR ? log2_z - fmaf(m, LOG2E, -at) : log2_z) * LN2;
+    auto lp = [&](float v) { return far || fabsf(v) > TOK_FAR ? (v - m) - log_z : (fmaf(v, LOG2E, -at) - log2_z) * LN2; };
+    if (MODE != TOK_GRAD && in && gl == 0) {
+      if (a.lse) a.lse[r] = !live ? 0.0f : empty ? ninf : far ? m + log_z : (at + log2_z) * LN2;
+      if (a.logp) a.logp[r] = !live ? 0.0f : empty ? ninf : lp(x_t);
+      if (ENT && a.entropy) a.entropy[r] = !live || empty ? 0.0f : (log2_z - u / z) * LN2;
+    }
+    if (TOP) {
+      // the row's lanes find the best of their best logits, `top` times; the lane that had it goes on to its next
+      unsigned long long keys[NV * E + 2], best = 0;
+      {
+        int k = 0;
+        keys[NV * E] = keys[NV * E + 1] = 0;
+        values([&](float2 v, int j, int i) {
+          keys[k++] = v.x > ninf ? top_key(v.x, j) : 0;
+          keys[k++] = v.y > ninf ? top_key(v.y, i) : 0;
+        });
+      }
+      auto next = [&](unsigned long long taken) {
+        best = 0;
+#pragma unroll
+        for (int k = 0; k < NV * E + 2; ++k) {
+          if (keys[k] == taken) keys[k] = 0;
+          best = keys[k] > best ? keys[k] : best;
+        }
+      };
+      next(~0ull);
+      for (int k = 0; k < a.top; ++k) {
+        unsigned long long key = best;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          if (o < G) { const unsigned long long other = __shfl_xor_sync(full, key, o); key = other > key ? other : key; }
+        if (in && gl == 0) {
+          a.top_logp[r * a.top + k] = live && key ? lp(of_order((unsigned int)(key >> 32))) : ninf;
+          a.top_id[r * a.top + k] = live && key ? (int)(0xffffffffu - (unsigned int)key) : -1;
+        }
+        if (key && best == key) next(key);
+      }
+    }
+  }
+  if (FWD) return;
+  O* const d = reinterpret_cast<O*>(a.out) + rr * a.ld_out;
+  // scale * 2^(x log2 e - c) * (1 or A + B * exponent), or differences first
+  float c = 0.0f, A = 0.0f, B = 0.0f, hit = 0.0f;
+  bool zeros = !live, slow = far;
+  if (MODE == TOK_LOSS) {
+    const float f = a.scale * i0;
+    zeros = zeros || z == 0.0f;
+    c = shift_of(m);
+    A = far ? f : f / z;
+    hit = -f;
+  } else {
+    zeros = zeros || i0 == ninf;
+    hit = i1;
+    slow = !(fabsf(i0) <= LSE_EXACT);
+    if (isnan(i0)) m = i0;      // as for a NaN
+    if (slow) {
+      A = -(i1 + i2 * i3);
+      B = -i2 * LN2;
+    } else {      // see token_loss.cu
+      c = i0 * LOG2E;
+      const float off = fmaf(i0, LOG2E, -c), f = -exp2_of(-off);
+      A = f * (i1 + i2 * (i3 - LN2 * off));
+      B = f * LN2 * i2;
+    }
+  }
+  const bool aligned = (((uintptr_t)d / sizeof(O) - ph) & (E - 1)) == 0;
+  const bool any_slow = __any_sync(full, live && slow);      // (and out may be x: the row is in registers, its target has been read)
+  if (!in) return;
+  auto write = [&](auto with_slow) {
+    auto result = [&](float2 v) {
+      float2 p = fma_2(v, both(LOG2E), both(-c));
+      if (with_slow.value && slow) p = make_float2(((v.x - m) - log_z) * LOG2E, ((v.y - m) - log_z) * LOG2E);
+      const float2 e = make_float2(exp2_of(p.x), exp2_of(p.y));
+      if (MODE == TOK_LOSS) return mul_2(e, both(A));
+      return mul_2(e, fma_2(make_float2(fmaxf(p.x, -1e4f), fmaxf(p.y, -1e4f)), both(B), both(A)));      // (zero times a number; a NaN is in e)
+    };
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      const int j = (gl + q * G) * E - ph;
+      if (j >= a.V) continue;
+      float o[E];
+      TokVec<T>::get(w[q], o);
+#pragma unroll
+      for (int k = 0; k < E; k += 2) { const float2 v = result(make_float2(o[k], o[k + 1])); o[k] = v.x; o[k + 1] = v.y; }
+      if (t >= j && t < j + E) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) if (j + k == t) o[k] += hit;
+      }
+      if (zeros) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) o[k] = 0.0f;
+      }
+      const bool whole = j >= 0 && j + E <= a.V;
+      if (whole && aligned) {
+        store_group<O, E>(d + j, o);
+      } else if (whole || !split) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) if (j + k >= 0 && j + k < a.V) d[j + k] = from_f32<O>(o[k]);
+      }
+    }
+    if (has_h || has_t) {
+      const float2 v = result(make_float2(xh, xt));
+      if (has_h) d[jh] = from_f32<O>(zeros ? 0.0f : v.x + (jh == t ? hit : 0.0f));
+      if (has_t) d[jt] = from_f32<O>(zeros ? 0.0f : v.y + (jt == t ? hit : 0.0f));
+    }
+  };
+  if (any_slow) write(std::true_type{});
+  else write(std::false_type{});
+}
+
+template <typename T, typename O, int MODE>
+static int tok_short_go(const TokDev& d, cudaStream_t st) {
+  const long long groups = tok_groups(d.V, sizeof(T));
+  int lg = 0;
+  while (lg < 5 && groups > 1 << lg) ++lg;
+  const long long rows = groups <= 32 ? 32 >> lg : 1, blocks = (d.R + 8 * rows - 1) / (8 * rows);      // rows of a warp
+  if (blocks >= (1ll << 31)) { set_error("tokens: too many rows%s", "", 0, 0); return -1; }
+  auto go = [&](auto kern) { kern<<<(unsigned)blocks, 256, 0, st>>>(d, lg); };
+  if constexpr (MODE == TOK_TOP) {
+    go(tok_short_kernel<T, O, MODE, 1>);
+  } else {
+    if (groups <= 32) go(tok_short_kernel<T, O, MODE, 1>);
+    else if (groups <= 128) go(tok_short_kernel<T, O, MODE, 4>);
+    else go(tok_short_kernel<T, O, MODE, 8>);
+  }
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) { set_error("tokens launch: %s", cudaGetErrorString(e), 0, 0); return -7; }
+  return 0;
+}
+
+int tok_short(const TokDev& d, int mode, int x_bf16, int out_bf16, cudaStream_t st) {
+  using B = __nv_bfloat16;
+  switch (mode) {
+    case TOK_LOGP: return x_bf16 ? tok_short_go<B, float, TOK_LOGP>(d, st) : tok_short_go<float, float, TOK_LOGP>(d, st);
+    case TOK_ENTROPY: return x_bf16 ? tok_short_go<B, float, TOK_ENTROPY>(d, st) : tok_short_go<float, float, TOK_ENTROPY>(d, st);
+    case TOK_TOP: return x_bf16 ? tok_short_go<B, float, TOK_TOP>(d, st) : tok_short_go<float, float, TOK_TOP>(d, st);
+    case TOK_LOSS:
+      if (x_bf16) return out_bf16 ? tok_short_go<B, B, TOK_LOSS>(d, st) : tok_short_go<B, float, TOK_LOSS>(d, st);
+      return out_bf16 ? tok_short_go<float, B, TOK_LOSS>(d, st) : tok_short_go<float, float, TOK_LOSS>(d, st);
+    default:
+      if (x_bf16) return out_bf16 ? tok_short_go<B, B, TOK_GRAD>(d, st) : tok_short_go<B, float, TOK_GRAD>(d, st);
+      return out_bf16 ? tok_short_go<float, B, TOK_GRAD>(d, st) : tok_short_go<float, float, TOK_GRAD>(d, st);
+  }
+}
+}  // namespace ono
