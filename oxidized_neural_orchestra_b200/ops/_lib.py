@@ -181,7 +181,7 @@ class OnoOptim(C.Structure):
         ("n", C.c_longlong), ("kind", C.c_int),
         ("lr", C.c_float), ("mu", C.c_float), ("b1", C.c_float), ("b2", C.c_float), ("eps", C.c_float),
         ("grad_scale", C.c_float), ("adam_pows", C.c_void_p), ("p_bf16", C.c_void_p),
-        ("zero_grad", C.c_int), ("grad_coef", C.c_void_p),
+        ("zero_grad", C.c_int), ("grad_coef", C.c_void_p), ("ob1", C.c_float), ("ob2", C.c_float),
     ]
 
 

@@ -150,7 +150,8 @@ def optim_step(p: torch.Tensor, g: torch.Tensor, *, kind: str, lr: float, mu: fl
                grad_scale: float = 1.0, p_bf16: torch.Tensor | None = None, zero_grad: bool = False,
                grad_coef: torch.Tensor | None = None, stream=None) -> None:
     """SGD / momentum / Adam on a flat f32 buffer (one kernel). ``grad_coef``: one f32 on the device that the gradient is multiplied by beside
-    ``grad_scale`` (``clip.grad_norm``'s coefficient for gradients scaled by ``grad_scale``)."""
+    ``grad_scale`` (``clip.grad_norm``'s coefficient for gradients scaled by ``grad_scale``). With it Adam's 1 - b1 and 1 - b2 are rounded once;
+    without it they are those of b1 and b2 as f32 has them, as the reference's (1.3e-5 off for 0.999)."""
     _need_cuda(p)
     if grad_coef is not None and (grad_coef.dtype != torch.float32 or grad_coef.numel() != 1 or grad_coef.device != p.device):
         raise ValueError("grad_coef must be one float32 on the parameters' device")
@@ -164,7 +165,8 @@ def optim_step(p: torch.Tensor, g: torch.Tensor, *, kind: str, lr: float, mu: fl
     o.adam_pows = _p(adam_pows)
     o.p_bf16 = _p(p_bf16)
     o.zero_grad = int(zero_grad)
-    o.grad_coef = _p(grad_coef)
+    if grad_coef is not None:
+        o.grad_coef, o.ob1, o.ob2 = grad_coef.data_ptr(), 1.0 - b1, 1.0 - b2
     _lib.check(lib.ono_optim(C.byref(o), _lib.stream_ptr(stream)), "ono_optim")
 
 

@@ -188,11 +188,19 @@ def test_optimizer_takes_the_coefficient(kind):
         if clipped:
             out = [torch.empty_like(g)]
             clip_grads([g], 1.5, scale=0.5, out=out)
-            ew.optim_step(p, out[0], m=m, v=v, **hp)
+            ew.optim_step(p, out[0], m=m, v=v, grad_coef=torch.ones(1, device="cuda"), **hp)
         else:
             grad_norm([g], norm, max_norm=1.5, coef=coef, scale=0.5)
             ew.optim_step(p, g, m=m, v=v, grad_scale=0.5, grad_coef=coef, **hp)
         got.append((p, m, v))
+    if kind == "adam":      # v itself, of numbers where 1 - b2 counts: b2 v + (1 - b2) g^2 with the rounding of each part
+        c = 1.5 / (0.5 * math.sqrt(float(g.double().square().sum())))
+        parts = 0.999 * v0.double(), 0.001 * (0.5 * c * g.double()).square()
+        assert ((got[0][2].double() - parts[0] - parts[1]).abs() <= 2.0 ** -24 * (3 * parts[0] + 24 * parts[1])).all()
+        zero, m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+        ew.optim_step(zero, g, m=m, v=v, grad_coef=torch.ones(1, device="cuda"), **hp)
+        assert ((v.double() - 0.001 * g.double().square()).abs() <= 4 * 2.0 ** -24 * 0.001 * g.double().square() + 1e-44).all()
+        assert ((m.double() - 0.1 * g.double()).abs() <= 3 * 2.0 ** -24 * 0.1 * g.double().abs() + 1e-44).all()
     want = 0.5 * math.sqrt(float(g.double().square().sum()))
     assert abs(norm.item() - want) <= NORM_TOL * want and abs(coef.item() - 1.5 / want) <= 2 * NORM_TOL * 1.5 / want
     for a, b, start in zip(got[0], got[1], (p0, m0, v0)):

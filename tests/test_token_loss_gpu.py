@@ -226,6 +226,24 @@ def test_rows_of_every_kind(kind, vocab, dtype):
     _check_loss(x, whole, targets, dtype, in_place=True)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(2400, 1030), (2400, 2500), (2500, 7001), (2368, 4099), (700, 9000), (200, 30011), (3000, 64), (5000, 3), (601, 250)])
+def test_many_rows_of_mixed_kinds(rows, vocab, dtype):
+    """As many rows as take other forms than a few do (a warp to a row, several rows to a warp, one CTA to a row), extraordinary ones among them."""
+    torch.manual_seed(rows)
+    x, whole = _logits(rows, vocab, dtype, vocab + 1 if rows % 3 else None)
+    kinds = ["equal", "ascending", "few values", "one allowed", "nothing allowed", "masked by the lowest value", "huge", "far from zero", "infinity", "nan"]
+    for k, kind in enumerate(kinds):
+        _special(kind, x[7 + 11 * k:13 + 11 * k])
+    targets = torch.randint(-1, vocab, (rows,), device="cuda")
+    for k in sorted({0, 1, min(5, vocab), min(20, vocab)}):
+        _check_forward(x, targets, k)
+    _check_grad(x, targets, dtype)
+    _check_grad(x, None, BF16, logp=False)
+    _check_loss(x, whole, targets, BF16)
+    _check_loss(x, whole, targets, dtype, in_place=True)
+
+
 def test_ignored_and_unknown_targets():
     from oxidized_neural_orchestra_b200.ops.token_loss import token_logprobs, token_logprobs_grad, token_loss
 

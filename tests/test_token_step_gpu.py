@@ -72,9 +72,8 @@ def test_step_against_64_bits():
         assert rel(g, r.grad) <= tol, k
     norm = float(ref.norm())
     assert norm > MAX_NORM and abs(s.norm.item() - norm) <= tol * norm and abs(s.coef.item() - MAX_NORM / norm) <= tol * MAX_NORM / norm
-    # Adam's first step: m = (1 - b1) g of the clipped gradient, three roundings; b1 is 0.9 as f32 has it, 2^-25 off, and with it 1 - b1 by up to
-    # 5 units of its own
-    own = s.g.double() * s.coef.double() * (1.0 - float(torch.tensor(0.9)))
+    # Adam's first step: m = (1 - b1) g of the clipped gradient, 1 - b1 rounded once and three more roundings
+    own = s.g.double() * s.coef.double() * 0.1
     assert ((s.m.double() - own).abs() <= 4 * 2.0 ** -24 * own.abs() + 1e-40).all()
 
 
