@@ -7,15 +7,16 @@
 
 namespace ono {
 
-// NV groups of 16 bytes to a lane. NV == 1: 2^lg lanes to a row, 32 >> lg rows to a warp.
+// NV groups of 16 bytes to a lane. NV == 1: 2^lg lanes to a row, 32 >> lg rows to a warp. CTAs of 128 threads: of 256 they took one to three percent
+// longer (16384 rows of 1000 f32 logits, loss 23.1 us against 22.4).
 template <typename T, typename O, int MODE, int NV>
-__global__ void __launch_bounds__(256, NV == 1 ? 6 : 4) tok_short_kernel(const __grid_constant__ TokDev a, int lg) {
+__global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const __grid_constant__ TokDev a, int lg) {
   constexpr int E = TokVec<T>::E;
   constexpr bool TOP = MODE == TOK_TOP, ENT = MODE == TOK_ENTROPY || MODE == TOK_TOP, FWD = MODE <= TOK_TOP;
   const float ninf = __int_as_float(0xff800000);
   const unsigned int full = 0xffffffffu;
   const int lane = threadIdx.x & 31, G = NV == 1 ? 1 << lg : 32, gl = lane & (G - 1);
-  const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), r = NV == 1 ? (job << (5 - lg)) + (lane >> lg) : job;
+  const long long job = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), r = NV == 1 ? (job << (5 - lg)) + (lane >> lg) : job;
   const bool in = r < a.R;
   const long long rr = in ? r : 0;
   const T* const x = reinterpret_cast<const T*>(a.x) + rr * a.ld;
@@ -111,36 +112,65 @@ __global__ void __launch_bounds__(256, NV == 1 ? 6 : 4) tok_short_kernel(const _
       if (a.logp) a.logp[r] = !live ? 0.0f : empty ? ninf : lp(x_t);
       if (ENT && a.entropy) a.entropy[r] = !live || empty ? 0.0f : (log2_z - u / z) * LN2;
     }
-    if (TOP) {
-      // the row's lanes find the best of their best logits, `top` times; the lane that had it goes on to its next
-      unsigned long long keys[NV * E + 2], best = 0;
+    if constexpr (TOP) {
+      // The row's lanes find the largest of their largest logits, `top` times, of equal ones the lane with the lowest place; it goes on to its next.
+      // A lane's logits are in the order of their places: of the row's beginning, its group, of the row's end. 0: none left. (65536 rows of 100 f32: five take
+      // 60 us, twenty 154; with the place as the lower half of 64-bit keys, and shuffles for all of it, 84 and 244.)
+      static_assert(NV == 1, "one group to a lane");
+      unsigned int key[E + 2], best, slot;
+      auto key_of = [&](float v) { return v > ninf ? order_of(v) : 0u; };
       {
-        int k = 0;
-        keys[NV * E] = keys[NV * E + 1] = 0;
-        values([&](float2 v, int j, int i) {
-          keys[k++] = v.x > ninf ? top_key(v.x, j) : 0;
-          keys[k++] = v.y > ninf ? top_key(v.y, i) : 0;
-        });
+        float o[E];
+        TokVec<T>::get(w[0], o);
+        key[0] = key_of(xh);
+#pragma unroll
+        for (int k = 0; k < E; ++k) key[1 + k] = key_of(o[k]);
+        key[E + 1] = key_of(xt);
       }
-      auto next = [&](unsigned long long taken) {
-        best = 0;
+      auto find = [&] {
+        best = slot = 0;
 #pragma unroll
-        for (int k = 0; k < NV * E + 2; ++k) {
-          if (keys[k] == taken) keys[k] = 0;
-          best = keys[k] > best ? keys[k] : best;
-        }
+        for (int k = 0; k < E + 2; ++k) if (key[k] > best) { best = key[k]; slot = k; }
       };
-      next(~0ull);
-      for (int k = 0; k < a.top; ++k) {
-        unsigned long long key = best;
+      find();
+      const int lane0 = lane - gl;
+      auto most = [&](unsigned int v) {
+        if (G == 32) return __reduce_max_sync(full, v);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-          if (o < G) { const unsigned long long other = __shfl_xor_sync(full, key, o); key = other > key ? other : key; }
-        if (in && gl == 0) {
-          a.top_logp[r * a.top + k] = live && key ? lp(of_order((unsigned int)(key >> 32))) : ninf;
-          a.top_id[r * a.top + k] = live && key ? (int)(0xffffffffu - (unsigned int)key) : -1;
+        for (int o = 8; o > 0; o >>= 1) { const unsigned int other = __shfl_xor_sync(full, v, o & (G - 1)); v = max(v, other); }
+        return v;
+      };
+      unsigned int out_key = 0, out_id = 0;      // the k-th at the k-th lane, G of them at a time
+      auto put = [&](int k, unsigned int o, unsigned int id) {
+        if (!in) return;
+        a.top_logp[r * a.top + k] = live && o ? lp(of_order(o)) : ninf;
+        a.top_id[r * a.top + k] = live && o ? (int)id : -1;
+      };
+      for (int k = 0; k < a.top; ++k) {
+        const unsigned int largest = most(best);
+        if (__all_sync(full, largest == 0)) {      // none left: the pending ones, and nothing behind them
+          for (int i = k - (k & (G - 1)) + gl; i < a.top; i += G) put(i, i < k ? out_key : 0, out_id);
+          break;
         }
-        if (key && best == key) next(key);
+        const unsigned int at = (unsigned int)(slot == 0 ? jh : slot == E + 1 ? jt : gl * E - ph + (int)slot - 1);
+        const bool mine = largest != 0 && best == largest;
+        unsigned int who = __ballot_sync(full, mine) >> lane0 & (full >> (32 - G));
+        if (__any_sync(full, (who & (who - 1)) != 0)) {
+          const unsigned int low = ~most(mine ? ~at : 0u);
+          who = __ballot_sync(full, mine && at == low) >> lane0 & (full >> (32 - G));
+        }
+        const int taken = who ? __ffs(who) - 1 : 0;
+        const unsigned int id = __shfl_sync(full, at, lane0 + taken);
+        if ((k & (G - 1)) == gl) { out_key = largest; out_id = id; }
+        if ((k & (G - 1)) == G - 1 || k == a.top - 1) {
+          const int i = k - (k & (G - 1)) + gl;
+          if (i <= k) put(i, out_key, out_id);
+        }
+        if (who && taken == gl) {
+#pragma unroll
+          for (int i = 0; i < E + 2; ++i) if (i == (int)slot) key[i] = 0;
+          find();
+        }
       }
     }
   }
@@ -220,9 +250,9 @@ static int tok_short_go(const TokDev& d, cudaStream_t st) {
   const long long groups = tok_groups(d.V, sizeof(T));
   int lg = 0;
   while (lg < 5 && groups > 1 << lg) ++lg;
-  const long long rows = groups <= 32 ? 32 >> lg : 1, blocks = (d.R + 8 * rows - 1) / (8 * rows);      // rows of a warp
+  const long long rows = groups <= 32 ? 32 >> lg : 1, blocks = (d.R + 4 * rows - 1) / (4 * rows);      // rows of a warp
   if (blocks >= (1ll << 31)) { set_error("tokens: too many rows%s", "", 0, 0); return -1; }
-  auto go = [&](auto kern) { kern<<<(unsigned)blocks, 256, 0, st>>>(d, lg); };
+  auto go = [&](auto kern) { kern<<<(unsigned)blocks, 128, 0, st>>>(d, lg); };
   if constexpr (MODE == TOK_TOP) {
     go(tok_short_kernel<T, O, MODE, 1>);
   } else {
