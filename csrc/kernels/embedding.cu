@@ -4,7 +4,7 @@
 //
 // Either is bound by memory: the rows read and written, and for the gradient the whole table where it is not added to. Sums go over the tokens
 // in the order of their places, so that a gradient is the same to the bit from run to run: the places are sorted by token (stable), and
-// one warp adds up a run of equal tokens, or an L-th of a long one.
+// one warp adds up a run of equal tokens, or a long one's part in a chunk of the sorted places.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -631,7 +631,7 @@ static int embedding_go(const OnoEmbedding& e, bool vec, cudaStream_t st) {
 using namespace ono;
 
 extern "C" int ono_embedding(const OnoEmbedding* e, ono_stream_t stream) {
-  if (!e || e->n < 0 || e->vocab <= 0 || e->width <= 0 || e->ld_table < e->width || e->ld_out < e->width || (e->n && (!e->table || !e->ids || !e->out))) {
+  if (!e || e->n < 0 || e->vocab <= 0 || e->vocab > ONO_DIM_MAX || e->width <= 0 || e->width > ONO_DIM_MAX || e->ld_table < e->width || e->ld_out < e->width || (e->n && (!e->table || !e->ids || !e->out))) {
     set_error("bad embedding args%s", "", 0, 0);
     return -1;
   }
@@ -645,11 +645,11 @@ extern "C" int ono_embedding(const OnoEmbedding* e, ono_stream_t stream) {
 }
 
 extern "C" long long ono_embedding_grad_scratch(long long n, int vocab, int width) {
-  return n < 0 || vocab <= 0 || width <= 0 ? -1 : n <= FEW_MAX ? 0 : grad_scratch(n, width).bytes;
+  return n < 0 || vocab <= 0 || vocab > ONO_DIM_MAX || width <= 0 || width > ONO_DIM_MAX ? -1 : n <= FEW_MAX ? 0 : grad_scratch(n, width).bytes;
 }
 
 extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream) {
-  if (!e || e->n < 0 || e->n > (1ll << 31) - 65536 || e->vocab <= 0 || e->width <= 0 || e->ld_d < e->width || e->ld_grad < e->width || !e->grad ||
+  if (!e || e->n < 0 || e->n > (1ll << 31) - 65536 || e->vocab <= 0 || e->vocab > ONO_DIM_MAX || e->width <= 0 || e->width > ONO_DIM_MAX || e->ld_d < e->width || e->ld_grad < e->width || !e->grad ||
       (e->n && (!e->d || !e->ids))) {
     set_error("bad embedding_grad args%s", "", 0, 0);
     return -1;

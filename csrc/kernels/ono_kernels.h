@@ -482,7 +482,9 @@ int ono_sparse_lift_range(float* acc, long long begin, long long end, const unsi
 // ---------------------------------------------------------------------------------------------
 // Rows of a table by token (embedding.cu). ids: int32, or int64 with ids64; an id equal to padding_id stands for no token, any other outside
 // [0, vocab) likewise, and *status (optional) is set to ONO_ERR_BAD_ARG for those. dtypes: 0 f32, 1 bf16. Leading dimensions in elements.
+// vocab and width are at most ONO_DIM_MAX, as is V below: they are counted in 32 bits, here and there up to a block's stride beyond.
 // ---------------------------------------------------------------------------------------------
+#define ONO_DIM_MAX (0x7fffffff - 0xffff)
 typedef struct OnoEmbedding {
   const void* table;         // [vocab, ld_table]
   const void* ids;           // [n]
@@ -515,12 +517,12 @@ int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream);
 //   lse = m + ln z,  logp = (x[target] - m) - ln z,  entropy = ln z - sum exp(x - m) (x - m) / z,  top: the largest logits, ties to the
 //   lowest index. A logit of -inf has probability zero; a row of nothing else has logp = lse = -inf, entropy 0 and a gradient of zeros. A row
 //   with a NaN or +inf has NaN for all of them. A row whose target is ignore_id (or outside [0, V), which sets *status to ONO_ERR_BAD_ARG)
-//   is not read: zeros, and no alternatives. Places that have no alternative: id -1, log probability -inf.
+//   counts for nothing, whatever is in it: zeros, and no alternatives. Places that have no alternative: id -1, log probability -inf.
 // ---------------------------------------------------------------------------------------------
 #define ONO_TOP_MAX 32
 typedef struct OnoTokens {
   const void* x;             // [R, ld] logits
-  const void* targets;       // [R], optional (every row is read then, and logp, out are not to be had)
+  const void* targets;       // [R], optional (every row counts then, and logp, out are not to be had)
   long long R, ld, ld_out, ignore_id;
   int V, x_bf16, targets64, top;
   float *logp, *lse, *entropy;       // [R], each optional

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
     if (r >= a.R) return a.ignore_id;
     return a.targets64 ? __ldg(reinterpret_cast<const long long*>(a.targets) + r) : (long long)__ldg(reinterpret_cast<const int*>(a.targets) + r);
   };
-  auto target = [&](long long t) -> int {      // -1: the row is not read
+  auto target = [&](long long t) -> int {      // -1: the row counts for nothing
     if (a.targets && t == a.ignore_id) return -1;
     if (t >= 0 && t < a.V) return (int)t;
     if (a.status && gt == 0) atomicExch(a.status, ONO_ERR_BAD_ARG);
@@ -643,7 +643,7 @@ static int tok_run(TokDev& d, cudaStream_t st) {
 using namespace ono;
 
 extern "C" int ono_tokens(const OnoTokens* t, ono_stream_t stream) {
-  if (!t || t->R < 0 || t->V <= 0 || t->ld < t->V || (t->R && !t->x) || t->top < 0 || t->top > ONO_TOP_MAX || t->top > t->V ||
+  if (!t || t->R < 0 || t->V <= 0 || t->V > ONO_DIM_MAX || t->ld < t->V || (t->R && !t->x) || t->top < 0 || t->top > ONO_TOP_MAX || t->top > t->V ||
       (t->top > 0 && t->R && (!t->top_logp || !t->top_id)) || (t->out && (t->ld_out < t->V || t->entropy || t->top)) || (!t->targets && (t->logp || t->out))) {
     set_error("bad tokens args%s", "", 0, 0);
     return -1;
@@ -665,7 +665,7 @@ extern "C" int ono_tokens(const OnoTokens* t, ono_stream_t stream) {
 }
 
 extern "C" int ono_tokens_grad(const OnoTokensGrad* t, ono_stream_t stream) {
-  if (!t || t->R < 0 || t->V <= 0 || t->ld < t->V || t->ld_out < t->V || (t->R && (!t->x || !t->out || !t->lse)) || (!t->d_logp && !t->d_entropy) ||
+  if (!t || t->R < 0 || t->V <= 0 || t->V > ONO_DIM_MAX || t->ld < t->V || t->ld_out < t->V || (t->R && (!t->x || !t->out || !t->lse)) || (!t->d_logp && !t->d_entropy) ||
       (t->d_logp && !t->targets) || (t->entropy == nullptr) != (t->d_entropy == nullptr)) {
     set_error("bad tokens_grad args%s", "", 0, 0);
     return -1;

@@ -6,6 +6,18 @@ import torch
 
 from . import _lib
 
+DIM_MAX = 2**31 - 2**16      # rows' lengths and tables' rows: the kernels count them in 32 bits, some a block's stride beyond the last
+NO_ID = -(2**63)
+
+
+def id_or_none(value: int | None) -> int:
+    """An id that stands for no token, or one that no ids have."""
+    if value is None:
+        return NO_ID
+    if not NO_ID < value < -NO_ID:
+        raise ValueError(f"no id is {value}")
+    return value
+
 
 def one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
     """All on one GPU (None among them does not count)."""

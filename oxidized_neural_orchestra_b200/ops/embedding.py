@@ -9,9 +9,8 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._launch import launch, one_device, rows_of, scratch as scratch_for, status_ptr
+from ._launch import DIM_MAX, id_or_none, launch, one_device, rows_of, scratch as scratch_for, status_ptr
 
-NO_PADDING = -(2**63)
 _IDS = {torch.int32: 0, torch.int64: 1}
 
 
@@ -25,8 +24,8 @@ def _ids(ids: torch.Tensor, n: int) -> int:
 
 
 def _sizes(vocab: int, width: int) -> None:
-    if vocab >= 2**31 - 1 or width >= 2**31 - 16:
-        raise ValueError("a table has less than 2^31 rows and columns")
+    if vocab > DIM_MAX or width > DIM_MAX:
+        raise ValueError(f"a table has at most {DIM_MAX} rows and columns")
 
 
 def embedding(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, *, scale: float = 1.0, padding_id: int | None = -1,
@@ -42,18 +41,20 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, *, scal
     if table.shape[1] != width:
         raise ValueError(f"table rows have {table.shape[1]} values, out rows {width}")
     _sizes(vocab, width)
+    padding_id = id_or_none(padding_id)
     one_device(table, ids, out, status)
     if n == 0 or width == 0:
         return
     if vocab == 0:
         raise ValueError("a table without rows")
-    e = _lib.OnoEmbedding(table.data_ptr(), ids.data_ptr(), out.data_ptr(), n, ld_table, ld_out, NO_PADDING if padding_id is None else padding_id,
+    e = _lib.OnoEmbedding(table.data_ptr(), ids.data_ptr(), out.data_ptr(), n, ld_table, ld_out, padding_id,
                           vocab, width, table.dtype == torch.bfloat16, out.dtype == torch.bfloat16, wide, scale, status_ptr(status))
     launch(table, stream, "ono_embedding", C.byref(e))
 
 
 def embedding_grad_scratch(n: int, vocab: int, width: int) -> int:
     """Bytes of scratch that ``embedding_grad`` wants for ``n`` tokens (0 for few)."""
+    _sizes(vocab, width)
     return _lib.load().ono_embedding_grad_scratch(n, vocab, width)
 
 
@@ -75,14 +76,15 @@ def embedding_grad(d: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, *, sc
     if scratch is not None and not scratch.is_contiguous():
         raise ValueError("scratch must be contiguous")
     _sizes(vocab, width)
+    padding_id = id_or_none(padding_id)
     one_device(d, ids, grad, status, scratch)
     if vocab == 0 or width == 0:
         return
     if scratch is None:
-        need = embedding_grad_scratch(n, vocab, width)
+        need = _lib.load().ono_embedding_grad_scratch(n, vocab, width)
         if need:
             scratch = scratch_for(grad, need, stream)
-    e = _lib.OnoEmbeddingGrad(d.data_ptr(), ids.data_ptr(), grad.data_ptr(), n, ld_d, ld_grad, NO_PADDING if padding_id is None else padding_id,
+    e = _lib.OnoEmbeddingGrad(d.data_ptr(), ids.data_ptr(), grad.data_ptr(), n, ld_d, ld_grad, padding_id,
                               vocab, width, d.dtype == torch.bfloat16, wide, accumulate, scale, status_ptr(status),
                               None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel() * scratch.element_size())
     launch(grad, stream, "ono_embedding_grad", C.byref(e))

@@ -5,8 +5,8 @@ Logits are 2-D rows with unit inner stride, f32 or bf16; targets int32 or int64,
 stream, can be captured into a graph and returns nothing.
 
 A logit of -inf has probability zero. A row of nothing else has log probability and ``lse`` of -inf, entropy 0 and a gradient of zeros; a
-row with a NaN or +inf has NaN for them. A row whose target is ``ignore_id`` (None: there is none) is not read: zeros, and no
-alternatives. So is one whose target is outside the vocabulary, and then ``status`` (int32[1]) becomes non-zero."""
+row with a NaN or +inf has NaN for them. A row whose target is ``ignore_id`` (None: there is none) counts for nothing, whatever is in it:
+zeros, and no alternatives. So does one whose target is outside the vocabulary, and then ``status`` (int32[1]) becomes non-zero."""
 from __future__ import annotations
 
 import ctypes as C
@@ -14,9 +14,8 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._launch import launch, one_device, rows_of, status_ptr
+from ._launch import DIM_MAX, id_or_none, launch, one_device, rows_of, status_ptr
 
-NO_TARGET = -(2**63)
 _TARGETS = {torch.int32: 0, torch.int64: 1}
 
 TOP_MAX = 32
@@ -43,8 +42,8 @@ def _targets(t: torch.Tensor | None, rows: int) -> int:
 
 def _logits(t: torch.Tensor) -> int:
     pitch = rows_of(t, "logits")
-    if t.shape[1] >= 2**31 - 16:
-        raise ValueError("a vocabulary has less than 2^31 tokens")
+    if t.shape[1] > DIM_MAX:
+        raise ValueError(f"a vocabulary has at most {DIM_MAX} tokens")
     return pitch
 
 
@@ -71,8 +70,9 @@ def _tokens(logits, targets, ignore_id, status, stream, *, logp=None, lse=None, 
         top = top_logp.shape[1]
         if top > min(TOP_MAX, vocab):
             raise ValueError(f"at most {min(TOP_MAX, vocab)} alternatives")
+    ignore_id = id_or_none(ignore_id)
     one_device(logits, targets, status, logp, lse, entropy, top_logp, top_id, out, weight)
-    a = _lib.OnoTokens(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, ld, ld_out, NO_TARGET if ignore_id is None else ignore_id,
+    a = _lib.OnoTokens(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, ld, ld_out, ignore_id,
                        vocab, logits.dtype == torch.bfloat16, wide, top, _column(logp, rows, "logp"), _column(lse, rows, "lse"),
                        _column(entropy, rows, "entropy"), top_logp.data_ptr() if top else None, top_id.data_ptr() if top else None,
                        None if out is None else out.data_ptr(), out is not None and out.dtype == torch.bfloat16, _column(weight, rows, "weight"),
@@ -90,7 +90,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None, *, logp: 
     """With ``lse = ln sum_v exp(x_v)``: ``logp[r] = x[r, targets[r]] - lse[r]``, ``entropy[r] = -sum_v p_v ln p_v`` (natural logarithms, f32), and
     the ``top_id.shape[1]`` (at most ``TOP_MAX``) largest logits' tokens and log probabilities, the largest first and among equal ones
     the lowest token first. Where a row has fewer logits above -inf, id -1 and -inf follow. The logits are read once. Without ``targets`` every row
-    is read and there is no ``logp``."""
+    counts and there is no ``logp``."""
     if targets is None and logp is not None:
         raise ValueError("logp needs targets")
     _tokens(logits, targets, ignore_id, status, stream, logp=logp, lse=lse, entropy=entropy, top_logp=top_logp, top_id=top_id)
@@ -121,8 +121,9 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, *, l
         raise ValueError("d_logp needs targets")
     if (entropy is None) != (d_entropy is None):
         raise ValueError("d_entropy needs the entropy, which has no other use")
+    ignore_id = id_or_none(ignore_id)
     one_device(logits, targets, status, lse, entropy, d_logp, d_entropy, out)
-    a = _lib.OnoTokensGrad(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, ld, ld_out, NO_TARGET if ignore_id is None else ignore_id,
+    a = _lib.OnoTokensGrad(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, ld, ld_out, ignore_id,
                            vocab, logits.dtype == torch.bfloat16, wide, _column(lse, rows, "lse"), _column(entropy, rows, "entropy"),
                            _column(d_logp, rows, "d_logp"), _column(d_entropy, rows, "d_entropy"), out.data_ptr(), out.dtype == torch.bfloat16,
                            status_ptr(status))

@@ -114,3 +114,37 @@ def test_clip():
             clip_grads(g, 1.0, out=out)
     with pytest.raises(ValueError, match="one place"):
         clip_grads([g[0], g[0]], 1.0)
+
+
+def test_sizes_and_ids_that_32_and_64_bits_do_not_hold():
+    """Rows whose indexes would pass 32 bits within a block's stride of their end, and ids that a 64-bit integer would take for another."""
+    from oxidized_neural_orchestra_b200.ops import _lib
+    from oxidized_neural_orchestra_b200.ops.embedding import embedding, embedding_grad, embedding_grad_scratch
+    from oxidized_neural_orchestra_b200.ops.token_loss import token_logprobs, token_logprobs_grad, token_loss
+
+    def of(rows, width, dtype=torch.bfloat16):
+        return torch.empty(rows, width, dtype=dtype, device="meta")
+
+    top, ids, v = 2**31 - 2**16, torch.empty(1, dtype=torch.int64, device="meta"), torch.empty(1, device="meta")
+    for size in (top + 1, 2**31 - 100, 2**31):
+        for call in (lambda: embedding(of(1, size), ids, of(1, size)), lambda: embedding(of(size, 4), ids, of(1, 4)),
+                     lambda: embedding_grad(of(1, size), ids, of(1, size, torch.float32)), lambda: embedding_grad(of(1, 4), ids, of(size, 4, torch.float32)),
+                     lambda: token_logprobs(of(1, size), ids, logp=v), lambda: token_loss(of(1, size), ids, out=of(1, size)),
+                     lambda: token_logprobs_grad(of(1, size), ids, lse=v, d_logp=v, out=of(1, size))):
+            with pytest.raises(ValueError, match=str(top)):
+                call()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        token_logprobs(of(1, top), ids, logp=v)
+    assert embedding_grad_scratch(1000, top, 4) > 0
+    for vocab, width in ((top + 1, 4), (4, top + 1), (2**32 + 4, 4)):
+        with pytest.raises(ValueError, match=str(top)):
+            embedding_grad_scratch(1000, vocab, width)
+    lib = _lib.load()
+    assert lib.ono_embedding_grad_scratch(1000, top + 1, 4) == -1 and lib.ono_embedding_grad_scratch(1000, 4, top + 1) == -1
+    assert lib.ono_tokens(_lib.C.byref(_lib.OnoTokens(16, 16, 1, 2**31 - 100, 0, -1, 2**31 - 100)), None) != 0
+    x, t, w = torch.zeros(3, 9), torch.zeros(3, dtype=torch.int64), torch.zeros(3)
+    for wide in (2**63, 2**64 - 1, -(2**63), -(2**64)):
+        for call in (lambda: embedding(x, t, x, padding_id=wide), lambda: embedding_grad(x, t, x, padding_id=wide), lambda: token_logprobs(x, t, lse=w, ignore_id=wide),
+                     lambda: token_loss(x, t, out=x, ignore_id=wide), lambda: token_logprobs_grad(x, t, lse=w, d_logp=w, out=x, ignore_id=wide)):
+            with pytest.raises(ValueError, match="no id"):
+                call()
