@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ono_kernels.h"
 #include "piece.cuh"
@@ -43,65 +44,68 @@ __device__ __forceinline__ long long token_row(I id, int vocab, long long paddin
 // ------------------------------------------------------------------------------------------------
 // Lookup: a warp takes 32 * EMB_LOADS groups of VEC values of a row, or several rows where one has fewer groups than lanes.
 // ------------------------------------------------------------------------------------------------
-// Two loads to a lane; more leave fewer warps, each of which waits for its row's number first (131072 x 2048 bf16, us: one 174, two 134, four 161,
-// eight 387). Values that come one by one are four bytes or two, and then eight are in flight (100000 x 517 f32: two 123, four 85).
-template <int VEC> constexpr int EMB_LOADS = VEC == 1 ? 8 : 2;
+// Loads to a lane: more of them leave fewer warps, each of which waits for its row's number first. Us: eight values a load, two against four: 141, 137
+// (131072 x 2048 bf16), but 2.4, 2.9 (8 x 4096); four values, two, four, eight: 251, 204, 201 (131072 x 2048 bf16 to f32), but 21.0 and 21.5 of the last
+// two (30000 x 700 f32); values one by one, four, eight, sixteen: 78, 60, 50 (100000 x 517 f32 to bf16), 80, 60, 64 (bf16), 33, 22, 30 (91538 x 179). A row's loads
+// are shared out evenly over its warps (517: six, six and five a lane, and not eight, eight and one; f32 to bf16 55.6).
+template <typename TO> constexpr int EMB_VEC = 16 / sizeof(TO);      // values of a 16-byte store
+template <int VEC> constexpr int EMB_LOADS = VEC == 1 ? 8 : VEC == 4 ? 4 : 2;
+// BYTES of a row in as few accesses as there can be.
+template <int BYTES> struct Words {
+  using Word = std::conditional_t<BYTES == 2, unsigned short, std::conditional_t<BYTES == 4, unsigned int, std::conditional_t<BYTES == 8, uint2, uint4>>>;
+  static constexpr int N = BYTES / (int)sizeof(Word);
+  Word w[N];
+};
 
 template <typename TI, typename TO, int VEC, typename I>
-__global__ void __launch_bounds__(256) embedding_kernel(const OnoEmbedding e, int groups, int segs, int lanes) {
+__global__ void __launch_bounds__(256) embedding_kernel(const OnoEmbedding e, int groups, int segs, int per, int lanes) {
   constexpr int U = EMB_LOADS<VEC>;
   const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   // lanes: log2 of those that a row takes
   const long long i = lanes < 5 ? job * (32 >> lanes) + (lane >> lanes) : job / segs;
   if (i >= e.n) return;
-  const int g0 = lanes < 5 ? lane & ((1 << lanes) - 1) : (int)(job - i * segs) * 32 * U + lane;
+  const int first = lanes < 5 ? 0 : (int)(job - i * segs) * 32 * per, end = min(groups, first + 32 * per);
+  const int g0 = first + (lanes < 5 ? lane & ((1 << lanes) - 1) : lane);
   const long long row = token_row(reinterpret_cast<const I*>(e.ids)[i], e.vocab, e.padding_id, e.status);
   const TI* src = reinterpret_cast<const TI*>(e.table) + (row < 0 ? 0 : row) * e.ld_table;
   TO* dst = reinterpret_cast<TO*>(e.out) + i * e.ld_out;
-  float v[U][VEC];
+  // Values are kept as they came until all loads are under way: converted where they are loaded, each would be waited for by itself
+  // (100000 x 517 f32 to bf16 74 us, so 57; bf16 96 against 62).
+  using In = Words<VEC * (int)sizeof(TI)>;
+  In w[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int g = g0 + 32 * u;
-    if (g >= groups) continue;
-    if (VEC > 1 && (g + 1) * VEC <= e.width) {
-      constexpr int N = VEC * (int)sizeof(TI) / 16 > 0 ? VEC * (int)sizeof(TI) / 16 : 1;
-      constexpr int EL = 16 / (int)sizeof(TI);
+    const TI* const at = src + (long long)g * VEC;
+    if (row < 0 || g >= end) continue;
+    if (VEC > 1 && (g + 1) * VEC > e.width) {
+      TI* const t = reinterpret_cast<TI*>(&w[u]);
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const uint4 w = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(src + (long long)g * VEC) + k);
-        const TI* t = reinterpret_cast<const TI*>(&w);
-#pragma unroll
-        for (int q = 0; q < EL && k * EL + q < VEC; ++q) v[u][k * EL + q] = to_f32(t[q]);
-      }
+      for (int k = 0; k < VEC; ++k) t[k] = g * VEC + k < e.width ? at[k] : from_f32<TI>(0.0f);
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[u][k] = row >= 0 && g * VEC + k < e.width ? to_f32(src[(long long)g * VEC + k]) : 0.0f;
+      for (int k = 0; k < In::N; ++k) w[u].w[k] = __ldg(reinterpret_cast<const typename In::Word*>(at) + k);
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int g = g0 + 32 * u;
-    if (g >= groups) continue;
-    if (row >= 0) {
+    if (g >= end) continue;
+    using Out = Words<VEC * (int)sizeof(TO)>;
+    Out o;
+    const TI* const t = reinterpret_cast<const TI*>(&w[u]);
+    TO* const q = reinterpret_cast<TO*>(&o);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[u][k] *= e.scale;
-    }
-    if (VEC > 1 && (g + 1) * VEC <= e.width) {
-      constexpr int N = VEC * (int)sizeof(TO) / 16 > 0 ? VEC * (int)sizeof(TO) / 16 : 1;
-      constexpr int EL = 16 / (int)sizeof(TO);
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        uint4 w;
-        TO* t = reinterpret_cast<TO*>(&w);
-#pragma unroll
-        for (int q = 0; q < EL; ++q) t[q] = from_f32<TO>(k * EL + q < VEC ? v[u][k * EL + q] : 0.0f);
-        *(reinterpret_cast<uint4*>(dst + (long long)g * VEC) + k) = w;
-      }
-    } else {
+    for (int k = 0; k < VEC; ++k) q[k] = from_f32<TO>(row < 0 ? 0.0f : to_f32(t[k]) * e.scale);
+    TO* const to = dst + (long long)g * VEC;
+    if (VEC > 1 && (g + 1) * VEC > e.width) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
-        if (g * VEC + k < e.width) dst[(long long)g * VEC + k] = from_f32<TO>(v[u][k]);
+        if (g * VEC + k < e.width) to[k] = q[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < Out::N; ++k) reinterpret_cast<typename Out::Word*>(to)[k] = o.w[k];
     }
   }
 }
@@ -118,28 +122,36 @@ struct GradDev {
   int sorted;                          // which of `item` holds the result
   int chunk, pitch;
   int bits, tile, tiles;               // radix sort: bits a pass, places of a CTA, CTAs
+  int zero;                            // values of a CTA that fills the table with zeros (a multiple of 4)
 };
 
-// Zeros for the CTAs behind the first `from` of a launch: values [cta * ZERO_VALUES, ...) of the table, `cta` from `first` on.
-constexpr int ZERO_VALUES = 1 << 16;      // of a CTA (a multiple of 4)
-__device__ __forceinline__ void fill_zeros(const OnoEmbeddingGrad& e, long long cta) {
+// Zeros for the CTAs behind the first ones of a launch: of the table's values, `zero` to a CTA, or of whole rows that many values long.
+constexpr int ZERO_VALUES = 1 << 16, ZERO_LEAST = 2048;
+__device__ __forceinline__ void fill_zeros(const GradDev& p, long long cta) {
+  const OnoEmbeddingGrad& e = p.e;
   const int threads = (int)blockDim.x;
   if (e.ld_grad == e.width && ((uintptr_t)e.grad & 15) == 0) {
-    const long long all = (long long)e.vocab * e.width, end = min(all, (cta + 1) * ZERO_VALUES);
-    for (long long i = cta * ZERO_VALUES + 4 * threadIdx.x; i < end; i += 4 * threads) {
+    const long long all = (long long)e.vocab * e.width, end = min(all, (cta + 1) * p.zero);
+    for (long long i = cta * p.zero + 4 * threadIdx.x; i < end; i += 4 * threads) {
       if (i + 4 <= all) *reinterpret_cast<float4*>(e.grad + i) = make_float4(0.f, 0.f, 0.f, 0.f);
       else for (long long k = i; k < all; ++k) e.grad[k] = 0.0f;
     }
   } else {
-    const long long rows = (ZERO_VALUES + e.width - 1) / e.width, end = min((long long)e.vocab, (cta + 1) * rows);
+    const long long rows = (p.zero + e.width - 1) / e.width, end = min((long long)e.vocab, (cta + 1) * rows);
     for (long long v = cta * rows + (threadIdx.x >> 5); v < end; v += threads >> 5)
       for (int k = threadIdx.x & 31; k < e.width; k += 32) e.grad[v * e.ld_grad + k] = 0.0f;
   }
 }
-static long long zero_ctas(const OnoEmbeddingGrad& e) {
+// A small table is shared out over four CTAs an SM, of a large one a CTA takes `most` values (gradient of 30 x 64 of 1000 rows, with 16384 a CTA 10.0 us,
+// so 3.6; of 9625 x 389 of 2135 with 65536 29.8, 26.7).
+static int zero_share(const OnoEmbeddingGrad& e, int most) {
+  const long long even = ((long long)e.vocab * e.width / (4 * ono_num_sms()) + 3) / 4 * 4;
+  return (int)std::min<long long>(most, std::max<long long>(ZERO_LEAST, even));
+}
+static long long zero_ctas(const OnoEmbeddingGrad& e, int share) {
   if (e.accumulate) return 0;
-  if (e.ld_grad == e.width && ((uintptr_t)e.grad & 15) == 0) return ((long long)e.vocab * e.width + ZERO_VALUES - 1) / ZERO_VALUES;
-  const long long rows = (ZERO_VALUES + e.width - 1) / e.width;
+  if (e.ld_grad == e.width && ((uintptr_t)e.grad & 15) == 0) return ((long long)e.vocab * e.width + share - 1) / share;
+  const long long rows = (share + e.width - 1) / e.width;
   return (e.vocab + rows - 1) / rows;
 }
 
@@ -156,7 +168,7 @@ template <typename I>
 __global__ void __launch_bounds__(256) embedding_rank_kernel(const __grid_constant__ GradDev p, int ctas) {
   __shared__ __align__(16) unsigned int s_key[RANK_MAX];
   const OnoEmbeddingGrad& e = p.e;
-  if ((int)blockIdx.x >= ctas) { fill_zeros(e, blockIdx.x - ctas); return; }
+  if ((int)blockIdx.x >= ctas) { fill_zeros(p, blockIdx.x - ctas); return; }
   const int n = (int)e.n, nv = (n + 3) / 4;
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
 #pragma unroll
@@ -197,7 +209,7 @@ template <typename I>
 __global__ void __launch_bounds__(SORT_THREADS) embedding_count_kernel(const __grid_constant__ GradDev p, long long zero) {
   __shared__ unsigned int s_count[SORT_RADIX];
   const OnoEmbeddingGrad& e = p.e;
-  if ((int)blockIdx.x >= p.tiles) { fill_zeros(e, zero + blockIdx.x - p.tiles); return; }
+  if ((int)blockIdx.x >= p.tiles) { fill_zeros(p, zero + blockIdx.x - p.tiles); return; }
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
   s_count[threadIdx.x] = 0;
   unsigned int* const mine = p.hist + blockIdx.x * SORT_RADIX + threadIdx.x;
@@ -214,7 +226,7 @@ template <typename I>
 __global__ void __launch_bounds__(SORT_THREADS) embedding_scatter_kernel(const __grid_constant__ GradDev p, int pass, int last, long long zero) {
   __shared__ unsigned int s_count[SORT_WARPS][SORT_RADIX], s_base[SORT_RADIX], s_sum[SORT_WARPS];
   const OnoEmbeddingGrad& e = p.e;
-  if ((int)blockIdx.x >= p.tiles) { fill_zeros(e, zero + blockIdx.x - p.tiles); return; }
+  if ((int)blockIdx.x >= p.tiles) { fill_zeros(p, zero + blockIdx.x - p.tiles); return; }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int shift = pass * p.bits;
   const unsigned int mask = (1u << p.bits) - 1, below = (1u << lane) - 1u;
@@ -455,7 +467,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
 // token's first adds up its rows, U in flight. The other CTAs fill the rows of the table that no token means with zeros. One launch.
 constexpr int FEW_MAX = 512, FEW_VALUES = 1 << 14;      // FEW_VALUES: zeros of a CTA
 template <typename T, int VEC, int STEP, typename I>
-__global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGrad e, int tiles, int ctas) {
+__global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGrad e, int tiles, int ctas, int rows) {
   constexpr int U = STEP == 1 ? 16 : 8, WORDS = FEW_MAX / 32;
   __shared__ unsigned int s_word[8 * FEW_MAX / 2];      // rows with a token, or the warps' lists of 16 bits a place
   static_assert(FEW_VALUES / 32 + 1 <= 8 * FEW_MAX / 2, "a bit for each of a CTA's rows");
@@ -464,7 +476,6 @@ __global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGr
   const bool aligned = (((uintptr_t)e.grad | (uintptr_t)(e.ld_grad * 4)) & 15) == 0;
   if ((int)blockIdx.x >= ctas) {
     const long long cta = blockIdx.x - ctas;
-    const int rows = (FEW_VALUES + e.width - 1) / e.width;
     const long long first = cta * rows;
     const int mine = (int)min((long long)rows, e.vocab - first);
     for (int k = threadIdx.x; k <= mine / 32; k += 256) s_word[k] = 0;
@@ -615,18 +626,20 @@ static GradScratch grad_scratch(long long n, int width) {
 template <typename TI, typename TO, int VEC, typename I>
 static int embedding_go(const OnoEmbedding& e, cudaStream_t st) {
   const int groups = (e.width + VEC - 1) / VEC, segs = (groups + 32 * EMB_LOADS<VEC> - 1) / (32 * EMB_LOADS<VEC>);
+  const int per = ((groups + 31) / 32 + segs - 1) / segs;      // loads of a lane, the same of every warp
   int lanes = 5;
   while (lanes > 0 && groups <= 1 << (lanes - 1)) --lanes;
   const long long jobs = lanes < 5 ? (e.n + (32 >> lanes) - 1) / (32 >> lanes) : e.n * segs, blocks = (jobs + 7) / 8;
   if (blocks >= (1ll << 31)) { set_error("embedding: too many values%s", "", 0, 0); return -1; }
-  embedding_kernel<TI, TO, VEC, I><<<(unsigned)blocks, 256, 0, st>>>(e, groups, segs, lanes);
+  embedding_kernel<TI, TO, VEC, I><<<(unsigned)blocks, 256, 0, st>>>(e, groups, segs, per, lanes);
   const cudaError_t r = cudaGetLastError();
   if (r != cudaSuccess) { set_error("embedding launch: %s", cudaGetErrorString(r), 0, 0); return -7; }
   return 0;
 }
 template <typename TI, typename TO>
-static int embedding_go(const OnoEmbedding& e, bool vec, cudaStream_t st) {
-  constexpr int VEC = sizeof(TI) == 4 && sizeof(TO) == 4 ? 4 : 8;
+static int embedding_go(const OnoEmbedding& e, cudaStream_t st) {
+  constexpr int VEC = EMB_VEC<TO>, I = VEC * (int)sizeof(TI) < 16 ? VEC * (int)sizeof(TI) : 16;
+  const bool vec = (uintptr_t)e.table % I == 0 && e.ld_table * (long long)sizeof(TI) % I == 0 && (uintptr_t)e.out % 16 == 0 && e.ld_out * (long long)sizeof(TO) % 16 == 0;
   if (e.ids64) return vec ? embedding_go<TI, TO, VEC, long long>(e, st) : embedding_go<TI, TO, 1, long long>(e, st);
   return vec ? embedding_go<TI, TO, VEC, int>(e, st) : embedding_go<TI, TO, 1, int>(e, st);
 }
@@ -641,11 +654,9 @@ extern "C" int ono_embedding(const OnoEmbedding* e, ono_stream_t stream) {
   }
   if (e->n == 0) return 0;
   cudaStream_t st = (cudaStream_t)stream;
-  const int ti = e->table_bf16 ? 2 : 4, to = e->out_bf16 ? 2 : 4;
-  const bool vec = (((uintptr_t)e->table | (uintptr_t)e->out) & 15) == 0 && e->ld_table * ti % 16 == 0 && e->ld_out * to % 16 == 0;
   using B = __nv_bfloat16;
-  if (e->table_bf16) return e->out_bf16 ? embedding_go<B, B>(*e, vec, st) : embedding_go<B, float>(*e, vec, st);
-  return e->out_bf16 ? embedding_go<float, B>(*e, vec, st) : embedding_go<float, float>(*e, vec, st);
+  if (e->table_bf16) return e->out_bf16 ? embedding_go<B, B>(*e, st) : embedding_go<B, float>(*e, st);
+  return e->out_bf16 ? embedding_go<float, B>(*e, st) : embedding_go<float, float>(*e, st);
 }
 
 extern "C" long long ono_embedding_grad_scratch(long long n, int vocab, int width) {
@@ -679,8 +690,8 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
   using B = __nv_bfloat16;
   cudaError_t r;
   if (e->n <= FEW_MAX && e->n > 0) {
-    const long long ctas = (e->n * tiles + 7) / 8, rows = (FEW_VALUES + e->width - 1) / e->width, zero = e->accumulate ? 0 : (e->vocab + rows - 1) / rows;
-    auto few = [&](auto kern) { kern<<<(unsigned)(ctas + zero), 256, 0, st>>>(*e, tiles, (int)ctas); };
+    const long long ctas = (e->n * tiles + 7) / 8, rows = (zero_share(*e, FEW_VALUES) + e->width - 1) / e->width, zero = e->accumulate ? 0 : (e->vocab + rows - 1) / rows;
+    auto few = [&](auto kern) { kern<<<(unsigned)(ctas + zero), 256, 0, st>>>(*e, tiles, (int)ctas, (int)rows); };
     if (ctas + zero >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
     if (e->ids64) {
       if (e->d_bf16) { if (vec) few(embedding_few_kernel<B, 8, 1, long long>); else few(embedding_few_kernel<B, 4, 32, long long>); }
@@ -692,7 +703,8 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
     if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad: %s", cudaGetErrorString(r), 0, 0); return -7; }
     return 0;
   }
-  const long long zeros = zero_ctas(*e);
+  p.zero = zero_share(*e, ZERO_VALUES);
+  const long long zeros = zero_ctas(*e, p.zero);
   if (zeros >= (1ll << 30)) { set_error("embedding_grad: too large a table%s", "", 0, 0); return -1; }
   if (e->n <= RANK_MAX) {
     const int ctas = (int)((e->n + RANK_PLACES - 1) / RANK_PLACES);
