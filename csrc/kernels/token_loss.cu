@@ -576,7 +576,7 @@ struct TokShape { int warps, ctas, per, staged; size_t smem; };
 
 constexpr int TOK_SLICE = 32768;      // bytes of a row that is kept, to a CTA
 
-static TokShape tok_shape(long long rows, int V, int esz, int mode) {
+static TokShape tok_shape(long long rows, int V, int esz, int mode, int top) {
   const long long groups = tok_groups(V, esz), bytes = groups * 16;
   TokShape s = {};
   s.ctas = 1;
@@ -589,6 +589,9 @@ static TokShape tok_shape(long long rows, int V, int esz, int mode) {
   }
   if (s.warps > 1 && mode != TOK_LOSS && rows * s.ctas <= 2 * ono_num_sms()) s.warps = 8;
   s.per = (int)((groups + s.ctas - 1) / s.ctas);
+  // A warp whose lanes have fewer logits than its share of the alternatives bounds nothing, and every logit would be a candidate (us, five of
+  // 35 x 519 bf16 17.8, so 4.6; twenty of 75 x 355 f32 10.5, 6.3).
+  while (mode == TOK_TOP && s.warps > 1 && s.ctas == 1 && s.per < 32 * (s.warps - 1) + (top + s.warps - 1) / s.warps) s.warps = s.warps == 8 ? 4 : 1;
   const int rows_of_cta = s.warps == 1 ? 4 : 1;
   s.staged = mode == TOK_LOSS && s.per * 16 <= 100 * 1024;
   if (s.staged) s.smem = (size_t)s.per * 16 * rows_of_cta;
@@ -629,7 +632,7 @@ static cudaError_t tok_go(const TokDev& d, const TokShape& s, cudaStream_t st) {
 template <typename T, typename O, int MODE>
 static int tok_run(TokDev& d, cudaStream_t st) {
   if (16 * tok_groups(d.V, sizeof(T)) <= (MODE == TOK_TOP ? TOK_SHORT_TOP : TOK_SHORT_ROW)) return tok_short(d, MODE, sizeof(T) == 2, sizeof(O) == 2, st);
-  const TokShape s = tok_shape(d.R, d.V, sizeof(T), MODE);
+  const TokShape s = tok_shape(d.R, d.V, sizeof(T), MODE, d.top);
   d.per = s.per;
   d.staged = s.staged;
   cudaError_t e;
