@@ -20,6 +20,7 @@
 namespace ono {
 void set_error(const char* fmt, const char* a, long long b, long long c);
 
+// Two groups of eight values in flight a thread: one or four take from 7 % less to 25 % more or less by the tensors, neither of them less over all.
 constexpr int CLIP_TENSORS = 256, CLIP_THREADS = 256, CLIP_GROUPS = 2, CLIP_CHUNK = 8 * CLIP_THREADS * CLIP_GROUPS, CLIP_MAX_BLOCKS = 8 * 148;
 
 // A tensor's values are counted from the 8 values' boundary in front of the first (`phase` before it), so that groups of eight

@@ -162,8 +162,9 @@ __device__ __forceinline__ unsigned int token_key(const OnoEmbeddingGrad& e, uns
   return r < 0 ? (unsigned int)e.vocab : (unsigned int)r;
 }
 
-// Few places: each finds its rank by comparing with all of them, RANK_THREADS threads a place. One launch, no pass waits for another.
-constexpr int RANK_MAX = 4096, RANK_THREADS = 16, RANK_PLACES = 256 / RANK_THREADS;
+// Few places: each finds its rank by comparing with all of them, RANK_THREADS threads a place. One launch, no pass waits for another. (Us, the gradient by
+// ranks against the radix sort: 2000 x 64 12.3, 13.8; 1500 x 256 18.0, 24.0; 3000 x 64 15.4, 14.2; 4096 x 1024 49.2, 46.3. Eight threads a place: 4096 52.2.)
+constexpr int RANK_MAX = 2048, RANK_THREADS = 16, RANK_PLACES = 256 / RANK_THREADS;
 template <typename I>
 __global__ void __launch_bounds__(256) embedding_rank_kernel(const __grid_constant__ GradDev p, int ctas) {
   __shared__ __align__(16) unsigned int s_key[RANK_MAX];
@@ -202,7 +203,8 @@ __global__ void __launch_bounds__(256) embedding_rank_kernel(const __grid_consta
 // 131072 places 74 us, so 62). Positions are sums of counts: over the warps, over the tiles before (each CTA adds them up itself) and
 // over the digits. The first launch counts; every pass then counts for the next one where its places go to.
 constexpr int SORT_THREADS = 512, SORT_WARPS = SORT_THREADS / 32, SORT_BITS = 9, SORT_RADIX = 1 << SORT_BITS, SORT_BATCH = 2;
-constexpr int SORT_TILE = SORT_THREADS * SORT_BATCH, SORT_TILES = 256;      // places of a CTA, or as many times that as leave SORT_TILES of them
+constexpr int SORT_TILE = SORT_THREADS * SORT_BATCH, SORT_TILES = 128;      // places of a CTA, or as many times that as leave SORT_TILES of them
+// (a CTA adds up the counts of all: 131072 x 256 in 256 tiles 61.9 us, in 128 59.9, in 64 59.3, but then 600000 x 64 150 against 136)
 static_assert(SORT_THREADS == SORT_RADIX, "a thread for each digit");
 
 template <typename I>
@@ -465,7 +467,12 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constan
 
 // Very few places: no sorting. A warp takes a place and 32 * VEC columns, looks for the place's token among all, and where the place is the
 // token's first adds up its rows, U in flight. The other CTAs fill the rows of the table that no token means with zeros. One launch.
-constexpr int FEW_MAX = 512, FEW_VALUES = 1 << 14;      // FEW_VALUES: zeros of a CTA
+constexpr int FEW_MAX = 512, FEW_VALUES = 1 << 14;      // FEW_VALUES: zeros of a CTA, at most
+// Where a token has FEW_RUN places and more on average, a warp would go through too many alone: ranks. (Us, this form against ranks: 500 places of 2 tokens, 64
+// columns, 38.9, 9.4; of 20 11.4, 9.9; of 100 8.7, 9.9; 100 of 5 5.9, 9.1; 300 of 50000, 256 columns, 11.9, 18.1. With FEW_MAX 1024: 1000 of 50000 15.5,
+// 18.8, but of 100 15.2, 10.8.)
+constexpr int FEW_RUN = 24;
+static bool grad_few(long long n, int vocab) { return n > 0 && n <= FEW_MAX && n <= (long long)FEW_RUN * vocab; }
 template <typename T, int VEC, int STEP, typename I>
 __global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGrad e, int tiles, int ctas, int rows) {
   constexpr int U = STEP == 1 ? 16 : 8, WORDS = FEW_MAX / 32;
@@ -549,7 +556,8 @@ __global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGr
 }
 
 // Third launch: a block takes a long run's sums, 32 * VEC columns of them; its warps every JOIN_WARPS-th, then one adds up theirs.
-constexpr int JOIN_WARPS = 16, JOIN_LOADS = 2;
+// (Eight of them: 60000 x 256 of 1000 tokens 45.8 us against 42.6; 32: 9916 x 3509 58.0 against 56.2, but 600000 x 64 132 against 136.)
+constexpr int JOIN_WARPS = 16;
 template <int VEC>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const __grid_constant__ GradDev p, int tiles) {
   __shared__ float s_sum[JOIN_WARPS][32 * VEC];
@@ -564,19 +572,11 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const _
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
     if (left > 0) {
-      for (unsigned int q0 = c + warp; q0 <= c1; q0 += JOIN_LOADS * JOIN_WARPS) {
-        float v[JOIN_LOADS][VEC];
+      for (unsigned int q = c + warp; q <= c1; q += JOIN_WARPS) {
+        float v[VEC];
+        GradVec<VEC, 1>::load(v, p.part + ((long long)q * 2 + (q == c ? 1 : 0)) * p.pitch + col, VEC, true);      // (a row of sums is whole groups)
 #pragma unroll
-        for (int u = 0; u < JOIN_LOADS; ++u) {
-          const unsigned int q = q0 + u * JOIN_WARPS;
-          if (q <= c1) GradVec<VEC, 1>::load(v[u], p.part + ((long long)q * 2 + (q == c ? 1 : 0)) * p.pitch + col, VEC, true);      // (a row of sums is whole groups)
-        }
-#pragma unroll
-        for (int u = 0; u < JOIN_LOADS; ++u) {
-          if (q0 + u * JOIN_WARPS > c1) break;
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
-        }
+        for (int k = 0; k < VEC; ++k) acc[k] += v[k];
       }
     }
 #pragma unroll
@@ -660,7 +660,7 @@ extern "C" int ono_embedding(const OnoEmbedding* e, ono_stream_t stream) {
 }
 
 extern "C" long long ono_embedding_grad_scratch(long long n, int vocab, int width) {
-  return n < 0 || vocab <= 0 || vocab > ONO_DIM_MAX || width <= 0 || width > ONO_DIM_MAX ? -1 : n <= FEW_MAX ? 0 : grad_scratch(n, width).bytes;
+  return n < 0 || vocab <= 0 || vocab > ONO_DIM_MAX || width <= 0 || width > ONO_DIM_MAX ? -1 : n == 0 || grad_few(n, vocab) ? 0 : grad_scratch(n, width).bytes;
 }
 
 extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream) {
@@ -670,7 +670,8 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
     return -1;
   }
   const GradScratch g = grad_scratch(e->n, e->width);
-  if (e->n > FEW_MAX && (!e->scratch || e->scratch_bytes < g.bytes || ((uintptr_t)e->scratch & 15))) { set_error("embedding_grad: scratch of %s%lld bytes, 16-byte aligned", "", g.bytes, 0); return -1; }
+  const bool few_places = grad_few(e->n, e->vocab);
+  if (e->n > 0 && !few_places && (!e->scratch || e->scratch_bytes < g.bytes || ((uintptr_t)e->scratch & 15))) { set_error("embedding_grad: scratch of %s%lld bytes, 16-byte aligned", "", g.bytes, 0); return -1; }
   if (e->n == 0 && e->accumulate) return 0;
   cudaStream_t st = (cudaStream_t)stream;
   GradDev p = {};
@@ -689,7 +690,7 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
   if (blocks >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
   using B = __nv_bfloat16;
   cudaError_t r;
-  if (e->n <= FEW_MAX && e->n > 0) {
+  if (few_places) {
     const long long ctas = (e->n * tiles + 7) / 8, rows = (zero_share(*e, FEW_VALUES) + e->width - 1) / e->width, zero = e->accumulate ? 0 : (e->vocab + rows - 1) / rows;
     auto few = [&](auto kern) { kern<<<(unsigned)(ctas + zero), 256, 0, st>>>(*e, tiles, (int)ctas, (int)rows); };
     if (ctas + zero >= (1ll << 31)) { set_error("embedding_grad: too many values%s", "", 0, 0); return -1; }
