@@ -599,7 +599,8 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const _
   }
 }
 
-// Places to a chunk: as many as leave enough warps to fill the GPU (a lane has U rows in flight whatever the chunk).
+// Places to a chunk: as many as leave enough warps to fill the GPU (a lane has U rows in flight whatever the chunk), fewer warps for short chunks.
+// Us, 64 a multiprocessor for every length: 131072 x 2048 268 against 255, 16384 x 1024 of 500 tokens 31 against 28; 128: 131072 x 256 79 against 62.
 static int grad_chunk(long long n, int width) {
   const long long tiles = (width + 127) / 128;
   int L = 512;

@@ -574,7 +574,8 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
 // How a launch is laid out.
 struct TokShape { int warps, ctas, per, staged; size_t smem; };
 
-constexpr int TOK_SLICE = 32768;      // bytes of a row that is kept, to a CTA
+// Bytes of a row that is kept, to a CTA. (Us, loss of 4096 x 50257 bf16: 16384 207, 32768 168, 65536 164; of 1000 x 128256 113, 113, 122.)
+constexpr int TOK_SLICE = 32768;
 
 static TokShape tok_shape(long long rows, int V, int esz, int mode, int top) {
   const long long groups = tok_groups(V, esz), bytes = groups * 16;
