@@ -359,9 +359,11 @@ struct GradVec {      // the same of an f32 row; 16-byte accesses where it is al
   }
 };
 
-// U rows are in flight; with ACC those of the table that they are added to as well.
+// U rows are in flight; with ACC those of the table that they are added to as well. (Eight values a lane are many registers: fewer rows, more warps. Us,
+// eight rows, four: 131072 x 512 of 200 tokens 58.0, 53.3, 16384 x 1024 58.9, 57.1, 131072 x 2048 318, 321; with ACC four, two in four blocks:
+// 131072 x 2048 257.6, 251.4, 131072 x 512 73.6, 62.9. Four values: 60000 x 1024 f32 with ACC four, two 105.8, 112.3, without eight, four 122.0, 124.2.)
 template <typename T, int VEC, int STEP, bool ACC, int U>
-__global__ void __launch_bounds__(256) embedding_sum_kernel(const __grid_constant__ GradDev p, int tiles) {
+__global__ void __launch_bounds__(256, U == 2 ? 4 : 1) embedding_sum_kernel(const __grid_constant__ GradDev p, int tiles) {
   const OnoEmbeddingGrad& e = p.e;
   const unsigned int n = (unsigned int)e.n, L = (unsigned int)p.chunk, none = (unsigned int)e.vocab;
   const uint2* const item = p.item[p.sorted];
@@ -740,10 +742,10 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
   if (e->n == 0) return 0;
   auto sum = [&](auto kern) { kern<<<(unsigned)blocks, 256, 0, st>>>(p, tiles); };
   if (e->accumulate) {
-    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, 1, true, 4>); else sum(embedding_sum_kernel<B, 4, 32, true, 4>); }
+    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, 1, true, 2>); else sum(embedding_sum_kernel<B, 4, 32, true, 4>); }
     else { if (vec) sum(embedding_sum_kernel<float, 4, 1, true, 4>); else sum(embedding_sum_kernel<float, 4, 32, true, 4>); }
   } else {
-    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, 1, false, 8>); else sum(embedding_sum_kernel<B, 4, 32, false, 8>); }
+    if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, 1, false, 4>); else sum(embedding_sum_kernel<B, 4, 32, false, 8>); }
     else { if (vec) sum(embedding_sum_kernel<float, 4, 1, false, 8>); else sum(embedding_sum_kernel<float, 4, 32, false, 8>); }
   }
   if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad sum: %s", cudaGetErrorString(r), 0, 0); return -7; }
