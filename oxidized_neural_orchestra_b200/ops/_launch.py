@@ -1,4 +1,4 @@
-"""What the operators on tokens and gradients share on the host: their checks, their scratch memory and the launch itself. A call of theirs may
+"""What the operators on tokens, on gradients and of the optimizer share on the host: their checks, their scratch memory and the launch itself. A call of theirs may
 take the GPU a few microseconds, so nothing here costs more than it has to."""
 from __future__ import annotations
 
@@ -59,13 +59,13 @@ def scratch(t: torch.Tensor, nbytes: int, stream) -> torch.Tensor:
         return torch.empty(nbytes, dtype=torch.uint8, device=t.device)
 
 
-def launch(t: torch.Tensor, stream, name: str, args) -> None:
-    """``name(args, stream)`` with the GPU of ``t`` as the current device, on ``stream`` (None: the one that is current there)."""
+def launch(t: torch.Tensor, stream, name: str, *args) -> None:
+    """``name(*args, stream)`` with the GPU of ``t`` as the current device, on ``stream`` (None: the one that is current there)."""
     fn, at = getattr(_lib.load(), name), t.get_device()
     if at == torch._C._cuda_getDevice():
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(at) if stream is None else stream.cuda_stream)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(at) if stream is None else stream.cuda_stream)
     else:
         with torch.cuda.device(at):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(at) if stream is None else stream.cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(at) if stream is None else stream.cuda_stream)
     if rc:
         _lib.check(rc, name)

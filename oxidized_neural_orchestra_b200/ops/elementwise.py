@@ -10,6 +10,7 @@ import ctypes as C
 import torch
 
 from . import _lib
+from ._launch import launch
 from .gemm import ACT
 
 OPT_KIND = {"sgd": 0, "gradient_descent": 0, "momentum": 1, "gradient_descent_with_momentum": 1, "adam": 2}
@@ -153,26 +154,20 @@ def optim_step(p: torch.Tensor, g: torch.Tensor, *, kind: str, lr: float, mu: fl
     ``grad_scale`` (``clip.grad_norm``'s coefficient for gradients scaled by ``grad_scale``). With it Adam's 1 - b1 and 1 - b2 are rounded once;
     without it they are those of b1 and b2 as f32 has them, as the reference's (1.3e-5 off for 0.999)."""
     _need_cuda(p)
-    if grad_coef is not None and (grad_coef.dtype != torch.float32 or grad_coef.numel() != 1 or grad_coef.device != p.device):
-        raise ValueError("grad_coef must be one float32 on the parameters' device")
-    lib = _lib.load()
-    o = _lib.OnoOptim()
-    o.p, o.g, o.m, o.v = p.data_ptr(), g.data_ptr(), _p(m), _p(v)
-    o.n = p.numel()
-    o.kind = OPT_KIND[kind]
-    o.lr, o.mu, o.b1, o.b2, o.eps = lr, mu, b1, b2, eps
-    o.grad_scale = grad_scale
-    o.adam_pows = _p(adam_pows)
-    o.p_bf16 = _p(p_bf16)
-    o.zero_grad = int(zero_grad)
+    coef = None
     if grad_coef is not None:
-        o.grad_coef, o.ob1, o.ob2 = grad_coef.data_ptr(), 1.0 - b1, 1.0 - b2
-    _lib.check(lib.ono_optim(C.byref(o), _lib.stream_ptr(stream)), "ono_optim")
+        if grad_coef.dtype != torch.float32 or grad_coef.numel() != 1 or grad_coef.get_device() != p.get_device():
+            raise ValueError("grad_coef must be one float32 on the parameters' device")
+        coef = grad_coef.data_ptr()
+    o = _lib.OnoOptim(p.data_ptr(), g.data_ptr(), _p(m), _p(v), p.numel(), OPT_KIND[kind], lr, mu, b1, b2, eps, grad_scale, _p(adam_pows), _p(p_bf16),
+                      int(zero_grad), coef, 0.0 if coef is None else 1.0 - b1, 0.0 if coef is None else 1.0 - b2)
+    launch(p, stream, "ono_optim", C.byref(o))
 
 
 def adam_tick(pows: torch.Tensor, b1: float, b2: float, stream=None) -> None:
     """Advance the running products ``{b1^t, b2^t}`` kept in device memory (graph friendly)."""
-    _lib.check(_lib.load().ono_adam_tick(pows.data_ptr(), b1, b2, _lib.stream_ptr(stream)), "ono_adam_tick")
+    _need_cuda(pows)
+    launch(pows, stream, "ono_adam_tick", pows.data_ptr(), b1, b2)
 
 
 def local_sgd(p: torch.Tensor, g: torch.Tensor, r: torch.Tensor, lr: float,

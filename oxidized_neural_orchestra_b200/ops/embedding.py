@@ -53,7 +53,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, *, scal
 
 
 def embedding_grad_scratch(n: int, vocab: int, width: int) -> int:
-    """Bytes of scratch that ``embedding_grad`` wants for ``n`` tokens (0 for few)."""
+    """Bytes of scratch that ``embedding_grad`` wants for ``n`` tokens (0 for few; more tokens may want less)."""
     _sizes(vocab, width)
     return _lib.load().ono_embedding_grad_scratch(n, vocab, width)
 
@@ -65,7 +65,7 @@ def embedding_grad(d: torch.Tensor, ids: torch.Tensor, grad: torch.Tensor, *, sc
     zeros for tokens that do not occur; with ``accumulate`` the sums are added to what is there and the other rows stay as they are. ``padding_id``
     and ``status`` as for ``embedding``.
 
-    Sums are f32 and go over the tokens in one order that depends on the ids alone: the same bits every time. ``scratch``: a
+    Sums are f32 and go over the places in one order that the sizes and the ids give: the same bits every time. ``scratch``: a
     contiguous tensor of at least ``embedding_grad_scratch`` bytes that no overlapping call uses (None: allocated for this call)."""
     ld_d, ld_grad = rows_of(d, "d"), rows_of(grad, "grad", (torch.float32,))
     n, width = d.shape
