@@ -206,3 +206,26 @@ def test_optimizer_takes_the_coefficient(kind):
     for a, b, start in zip(got[0], got[1], (p0, m0, v0)):
         # four roundings of the gradient and the update's own few, relative to what is added up
         assert ((a - b).abs() <= 16 * 2.0 ** -24 * (start.abs() + b.abs() + 0.05)).all()
+
+
+@pytest.mark.parametrize("dtype,out_dtype,total", [(BF16, F32, 17_000_011), (F16, F16, 17_000_011), (F32, BF16, 34_000_011), (F32, F32, 34_000_011)])
+def test_many_values(dtype, out_dtype, total):
+    """So many values that a thread has twice as many in flight: tensors of every alignment, groups that are not whole, a tensor shorter than one."""
+    from oxidized_neural_orchestra_b200.ops.clip import clip_grads
+
+    torch.manual_seed(3)
+    sizes = [1, 5, 8191, 8193, 16384, 3, 1_000_003, total // 2]
+    sizes.append(total - sum(sizes))
+    ts, whole = _flat(sizes, dtype, 3)
+    want = _norm(ts)
+    out, ow = _flat(sizes, out_dtype, 3 if dtype == out_dtype else 6)
+    norm, coef = torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
+    clip_grads(ts, want / 3, norm=norm, coef=coef, out=out)
+    assert abs(norm.item() - want) <= NORM_TOL * want
+    _check_out(out, ts, 1 / 3, 1.0)
+    lead = 3 if dtype == out_dtype else 6
+    assert (ow[:lead] == SENTINEL).all() and (ow[lead + total:] == torch.tensor(SENTINEL, dtype=out_dtype)).all()
+    before = [t.clone() for t in ts]
+    clip_grads(ts, want / 3)
+    _check_out(ts, before, 1 / 3, 1.0)
+    assert (whole[:3] == SENTINEL).all() and (whole[3 + total:] == torch.tensor(SENTINEL, dtype=dtype)).all()

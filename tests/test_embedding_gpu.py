@@ -208,3 +208,13 @@ def test_on_two_streams_and_in_graphs():
     assert torch.equal(sets[0][4], wanted[0][1])
     with pytest.raises(RuntimeError, match="scratch"):
         embedding_grad(sets[0][2], sets[0][1], sets[0][4], scratch=own[:-1])
+
+
+@pytest.mark.parametrize("n,vocab", [(1, 100), (511, 22), (512, 21), (512, 22), (513, 600), (48, 2), (49, 2), (2048, 500), (2049, 500)])
+@pytest.mark.parametrize("width,d_dtype,lead", [(40, BF16, 0), (33, BF16, 1), (133, F32, 3)])
+def test_gradient_of_equal_tokens(n, vocab, width, d_dtype, lead):
+    """All places of one token, or of two, on both sides of the sizes where another form begins."""
+    torch.manual_seed(n)
+    for ids in (torch.full((n,), vocab - 1, device="cuda"), torch.arange(n, device="cuda") % 2 * (vocab - 1)):
+        for accumulate in (False, True):
+            _check_grad(ids, vocab, width, d_dtype, accumulate=accumulate, lead=lead)

@@ -369,3 +369,17 @@ def test_rows_far_into_a_large_matrix():
     want = torch.exp(ref)
     want[vocab - 1] -= 1
     assert ((x[rows - 1].double() - want).abs() <= want.abs() * 2.0 ** -8 * 1.02 + _tol(vocab) * torch.exp(ref)).all() and not x[1:rows - 1].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [129, 255, 400, 509, 519, 640, 900, 1019, 1027, 2043, 2061])
+def test_alternatives_of_rows_of_few_logits_a_warp(vocab, dtype):
+    """Rows that fill one warp or several, or leave the last one with a few logits or none: all different, equal, of few values, all but three masked."""
+    torch.manual_seed(vocab)
+    for kind in ("as drawn", "equal", "few values", "three allowed"):
+        for ld, lead in ((-(-vocab // 16) * 16, 0), (vocab + 5, 3)):
+            x, _ = _logits(5, vocab, dtype, ld, lead)
+            _special(kind, x)
+            targets = torch.randint(-1, vocab, (5,), device="cuda")
+            for k in (1, 5, 8, 9, 20, 32):
+                _check_forward(x, targets, k)
