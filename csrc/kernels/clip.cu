@@ -15,6 +15,7 @@
 
 #include <algorithm>
 
+#include "chain.cuh"
 #include "ono_kernels.h"
 
 namespace ono {
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(CLIP_THREADS) clip_norm_kernel(const __grid_co
 // Norm and coefficient from the blocks' sums; every block that calls it gets the same ones.
 __device__ __forceinline__ double clip_coef(const double* part, int parts, float scale, float max_norm, float* norm_out, float* coef_out, double* s) {
   double sum = 0.0;
-  for (int i = threadIdx.x; i < parts; i += CLIP_THREADS) sum += part[i];
+  for (int i = threadIdx.x; i < parts; i += CLIP_THREADS) sum += __ldcg(part + i);
   sum = block_sum(sum, s);
   const double norm = fabs((double)scale) * sqrt(sum), coef = norm <= (double)max_norm ? 1.0 : (double)max_norm / norm;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -197,6 +198,7 @@ __device__ __forceinline__ double clip_coef(const double* part, int parts, float
 
 __global__ void __launch_bounds__(CLIP_THREADS) clip_finish_kernel(const double* part, int parts, float scale, float max_norm, float* norm, float* coef) {
   __shared__ double s[CLIP_THREADS / 32];
+  chain_wait();
   clip_coef(part, parts, scale, max_norm, norm, coef, s);
 }
 
@@ -204,6 +206,7 @@ template <int G>
 __global__ void __launch_bounds__(CLIP_THREADS) clip_write_kernel(const __grid_constant__ ClipBatch b, const double* part, int parts, float scale, float max_norm,
                                                                   float* norm, float* coef) {
   __shared__ double s[CLIP_THREADS / 32];
+  chain_wait();
   const float f = (float)(clip_coef(part, parts, scale, max_norm, norm, coef, s) * (double)scale);
   for (unsigned int c = blockIdx.x; c < b.end[b.count - 1]; c += gridDim.x) {
     const int t = clip_find(b, c), type = b.type[t] & 3, otype = b.type[t] >> 2;
@@ -276,12 +279,14 @@ static cudaError_t clip_go(const OnoClip* c, cudaStream_t st) {
     parts = std::max(parts, grid);
   }
   if (!c->out || parts == 0) {
-    clip_finish_kernel<<<1, CLIP_THREADS, 0, st>>>(part, parts, c->scale, c->max_norm, c->norm, c->coef);
+    const cudaError_t e = launch_behind(clip_finish_kernel, 1u, CLIP_THREADS, st, (const double*)part, parts, c->scale, c->max_norm, c->norm, c->coef);
+    if (e != cudaSuccess) return e;
   } else {
     next = 0;
     while (fill()) {
       const int grid = (int)std::min<long long>(b.end[b.count - 1], 8 * ono_num_sms());
-      clip_write_kernel<G><<<grid, CLIP_THREADS, 0, st>>>(b, part, parts, c->scale, c->max_norm, c->norm, c->coef);
+      const cudaError_t e = launch_behind(clip_write_kernel<G>, (unsigned)grid, CLIP_THREADS, st, b, (const double*)part, parts, c->scale, c->max_norm, c->norm, c->coef);
+      if (e != cudaSuccess) return e;
     }
   }
   return cudaGetLastError();

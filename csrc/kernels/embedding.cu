@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "chain.cuh"
 #include "ono_kernels.h"
 #include "piece.cuh"
 #include "ptx.cuh"
@@ -228,7 +229,8 @@ template <typename I>
 __global__ void __launch_bounds__(SORT_THREADS) embedding_scatter_kernel(const __grid_constant__ GradDev p, int pass, int last, long long zero) {
   __shared__ unsigned int s_count[SORT_WARPS][SORT_RADIX], s_base[SORT_RADIX], s_sum[SORT_WARPS];
   const OnoEmbeddingGrad& e = p.e;
-  if ((int)blockIdx.x >= p.tiles) { fill_zeros(p, zero + blockIdx.x - p.tiles); return; }
+  if ((int)blockIdx.x >= p.tiles) { fill_zeros(p, zero + blockIdx.x - p.tiles); return; }      // (nothing ahead in the chain touches the table)
+  chain_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int shift = pass * p.bits;
   const unsigned int mask = (1u << p.bits) - 1, below = (1u << lane) - 1u;
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_scatter_kernel(const _
 #pragma unroll
     for (int b = 0; b < SORT_BATCH; ++b) {
       const long long j = j0 + 32 * b + lane;
-      if (j < end) it[b] = pass ? __ldg(in + j) : make_uint2(token_key<I>(e, (unsigned int)j), (unsigned int)j);
+      if (j < end) it[b] = pass ? __ldcg(in + j) : make_uint2(token_key<I>(e, (unsigned int)j), (unsigned int)j);
     }
   };
   items_from(begin);
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_scatter_kernel(const _
   unsigned int before = 0, all = 0;
 #pragma unroll 16
   for (int t = 0; t < p.tiles; ++t) {
-    const unsigned int h = __ldg(hist + t * SORT_RADIX + tid);
+    const unsigned int h = __ldcg(hist + t * SORT_RADIX + tid);
     if (t < (int)blockIdx.x) before += h;
     all += h;
   }
@@ -365,6 +367,7 @@ struct GradVec {      // the same of an f32 row; 16-byte accesses where it is al
 template <typename T, int VEC, int STEP, bool ACC, int U>
 __global__ void __launch_bounds__(256, U == 2 ? 4 : 1) embedding_sum_kernel(const __grid_constant__ GradDev p, int tiles) {
   const OnoEmbeddingGrad& e = p.e;
+  chain_wait();
   const unsigned int n = (unsigned int)e.n, L = (unsigned int)p.chunk, none = (unsigned int)e.vocab;
   const uint2* const item = p.item[p.sorted];
   const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -564,6 +567,7 @@ template <int VEC>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const __grid_constant__ GradDev p, int tiles) {
   __shared__ float s_sum[JOIN_WARPS][32 * VEC];
   const OnoEmbeddingGrad& e = p.e;
+  chain_wait();
   const unsigned int L = (unsigned int)p.chunk, runs = *p.runs;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool aligned = (((uintptr_t)e.grad | (uintptr_t)(e.ld_grad * 4)) & 15) == 0;
@@ -732,15 +736,14 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
     done += now;
     for (int pass = 0; pass < passes && r == cudaSuccess; ++pass) {
       now = zeros_for(pass + 1);
-      if (e->ids64) embedding_scatter_kernel<long long><<<(unsigned)(g.tiles + now), SORT_THREADS, 0, st>>>(p, pass, pass == passes - 1, done);
-      else embedding_scatter_kernel<int><<<(unsigned)(g.tiles + now), SORT_THREADS, 0, st>>>(p, pass, pass == passes - 1, done);
-      r = cudaGetLastError();
+      r = launch_behind(e->ids64 ? embedding_scatter_kernel<long long> : embedding_scatter_kernel<int>, (unsigned)(g.tiles + now), SORT_THREADS, st, p, pass,
+                        (int)(pass == passes - 1), done);
       done += now;
     }
   }
   if (r != cudaSuccess) { set_error("embedding_grad sort: %s", cudaGetErrorString(r), 0, 0); return -7; }
   if (e->n == 0) return 0;
-  auto sum = [&](auto kern) { kern<<<(unsigned)blocks, 256, 0, st>>>(p, tiles); };
+  auto sum = [&](auto kern) { r = launch_behind(kern, (unsigned)blocks, 256, st, p, tiles); };
   if (e->accumulate) {
     if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, 1, true, 2>); else sum(embedding_sum_kernel<B, 4, 32, true, 4>); }
     else { if (vec) sum(embedding_sum_kernel<float, 4, 1, true, 4>); else sum(embedding_sum_kernel<float, 4, 32, true, 4>); }
@@ -748,12 +751,12 @@ extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream
     if (e->d_bf16) { if (vec) sum(embedding_sum_kernel<B, 8, 1, false, 4>); else sum(embedding_sum_kernel<B, 4, 32, false, 8>); }
     else { if (vec) sum(embedding_sum_kernel<float, 4, 1, false, 8>); else sum(embedding_sum_kernel<float, 4, 32, false, 8>); }
   }
-  if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad sum: %s", cudaGetErrorString(r), 0, 0); return -7; }
+  if (r != cudaSuccess) { set_error("embedding_grad sum: %s", cudaGetErrorString(r), 0, 0); return -7; }
   if (e->n > g.chunk) {      // (a long run fills a whole chunk and begins ahead of it)
     const int jt = (e->width + 127) / 128;
     const unsigned grid = (unsigned)std::min<long long>(chunks * jt, 4ll * ono_num_sms());
-    embedding_join_kernel<4><<<grid, 32 * JOIN_WARPS, 0, st>>>(p, jt);
-    if ((r = cudaGetLastError()) != cudaSuccess) { set_error("embedding_grad join: %s", cudaGetErrorString(r), 0, 0); return -7; }
+    r = launch_behind(embedding_join_kernel<4>, grid, 32 * JOIN_WARPS, st, p, jt);
+    if (r != cudaSuccess) { set_error("embedding_grad join: %s", cudaGetErrorString(r), 0, 0); return -7; }
   }
   return 0;
 }
