@@ -148,3 +148,36 @@ def test_sizes_and_ids_that_32_and_64_bits_do_not_hold():
                      lambda: token_loss(x, t, out=x, ignore_id=wide), lambda: token_logprobs_grad(x, t, lse=w, d_logp=w, out=x, ignore_id=wide)):
             with pytest.raises(ValueError, match="no id"):
                 call()
+
+
+def test_launches_go_to_the_tensors_device(monkeypatch):
+    """The device of the tensors is the current one during a launch, whichever was, and the stream is that device's, or the one that was given."""
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+
+    from oxidized_neural_orchestra_b200.ops import _launch
+
+    now, calls = [0], []
+
+    @contextmanager
+    def device(d):
+        was, now[0] = now[0], d
+        yield
+        now[0] = was
+
+    lib = SimpleNamespace(op=lambda *args: calls.append((now[0], *args)) or 0, bad=lambda *args: 7, ono_last_error=lambda: b"why")
+    monkeypatch.setattr(_launch._lib, "load", lambda: lib)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 100 + d, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    for at in (0, 1):
+        t = SimpleNamespace(get_device=lambda at=at: at)
+        _launch.launch(t, None, "op", "x")
+        _launch.launch(t, SimpleNamespace(cuda_stream=5), "op", "x", "y")
+        assert calls[-2:] == [(at, "x", 100 + at), (at, "x", "y", 5)] and now == [0]
+        with pytest.raises(RuntimeError, match="bad.*why"):
+            _launch.launch(t, None, "bad", "x")
+    cuda = [SimpleNamespace(is_cuda=True, device=f"cuda:{d}", get_device=lambda d=d: d) for d in (0, 1)]
+    _launch.one_device(cuda[1], None, cuda[1])
+    with pytest.raises(ValueError, match="different devices"):
+        _launch.one_device(cuda[0], None, cuda[1])
