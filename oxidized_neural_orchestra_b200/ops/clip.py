@@ -2,8 +2,8 @@
 
 Gradients are any number of contiguous f32, bf16 or f16 tensors of any size and alignment (views of a flat gradient vector among them); what is
 written overlaps neither another output nor another gradient. The norm is that of all of them together, of ``scale`` times their values. Squares are
-summed in 64 bits above the first eight, in an order that the sizes give. Each call launches on the current (or given) stream, can be captured into a
-graph and returns nothing."""
+summed in 64 bits above the first eight, in an order that sizes and alignment give. Each call launches on the current (or given) stream, can be
+captured into a graph and returns nothing."""
 from __future__ import annotations
 
 import ctypes as C

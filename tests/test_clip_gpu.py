@@ -229,3 +229,34 @@ def test_many_values(dtype, out_dtype, total):
     clip_grads(ts, want / 3)
     _check_out(ts, before, 1 / 3, 1.0)
     assert (whole[:3] == SENTINEL).all() and (whole[3 + total:] == torch.tensor(SENTINEL, dtype=dtype)).all()
+
+
+@pytest.mark.parametrize("count", [31, 33, 300])
+def test_many_tensors_of_several_types(count):
+    """On both sides of the number of tensors that one cluster takes, and more than a launch takes."""
+    from oxidized_neural_orchestra_b200.ops.clip import clip_grads, grad_norm
+
+    torch.manual_seed(count)
+    kinds = (F32, BF16, F16)
+    ts = [torch.randn(1 + 37 * k % 1500, device="cuda").to(kinds[k % 3]) for k in range(count)]
+    out = [torch.empty(t.numel(), device="cuda", dtype=kinds[(k // 3) % 3]) for k, t in enumerate(ts)]
+    want = _norm(ts, 0.5)
+    norm, n2, coef = (torch.empty(1, device="cuda") for _ in range(3))
+    grad_norm(ts, norm, max_norm=want / 7, coef=coef, scale=0.5)
+    clip_grads(ts, want / 7, scale=0.5, norm=n2, out=out)
+    assert abs(norm.item() - want) <= NORM_TOL * want and torch.equal(norm, n2) and abs(coef.item() - 1 / 7) <= (NORM_TOL + 2.0 ** -24) / 7
+    _check_out(out, ts, 1 / 7, 0.5)
+
+
+@pytest.mark.parametrize("n", [1, 4096 * 16, 4096 * 32 - 3, 4096 * 32 - 2, 4096 * 32, 4096 * 32 + 1])
+def test_sizes_around_what_one_cluster_takes(n):
+    from oxidized_neural_orchestra_b200.ops.clip import clip_grads
+
+    torch.manual_seed(5)
+    for lead in (0, 3):
+        ts, whole = _flat([n], BF16, lead)
+        before, want, norm = [t.clone() for t in ts], _norm(ts), torch.empty(1, device="cuda")
+        clip_grads(ts, want / 2, norm=norm)
+        assert abs(norm.item() - want) <= NORM_TOL * want
+        _check_out(ts, before, 0.5, 1.0)
+        assert (whole[:lead] == SENTINEL).all() and (whole[lead + n:] == torch.tensor(SENTINEL, dtype=BF16)).all()
