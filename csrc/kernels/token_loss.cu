@@ -574,8 +574,9 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
 // How a launch is laid out.
 struct TokShape { int warps, ctas, per, staged; size_t smem; };
 
-// Bytes of a row that is kept, to a CTA. (Us, loss of 4096 x 50257 bf16: 16384 207, 32768 168, 65536 164; of 1000 x 128256 113, 113, 122.)
-constexpr int TOK_SLICE = 32768;
+// Bytes of a row that is kept, to a CTA. (Us, loss of 4096 x 50257 bf16: 16384 207, 32768 168, 65536 164; of 1000 x 128256 113, 113, 122.) Longer slices of
+// the longest rows are kept up to TOK_KEPT_MAX, beyond that nothing is.
+constexpr int TOK_SLICE = 32768, TOK_KEPT_MAX = 100 * 1024;
 
 static TokShape tok_shape(long long rows, int V, int esz, int mode, int top) {
   const long long groups = tok_groups(V, esz), bytes = groups * 16;
@@ -594,7 +595,7 @@ static TokShape tok_shape(long long rows, int V, int esz, int mode, int top) {
   // 35 x 519 bf16 17.8, so 4.6; twenty of 75 x 355 f32 10.5, 6.3).
   while (mode == TOK_TOP && s.warps > 1 && s.ctas == 1 && s.per < 32 * (s.warps - 1) + (top + s.warps - 1) / s.warps) s.warps = s.warps == 8 ? 4 : 1;
   const int rows_of_cta = s.warps == 1 ? 4 : 1;
-  s.staged = mode == TOK_LOSS && s.per * 16 <= 100 * 1024;
+  s.staged = mode == TOK_LOSS && (long long)s.per * 16 <= TOK_KEPT_MAX;
   if (s.staged) s.smem = (size_t)s.per * 16 * rows_of_cta;
   if (mode == TOK_TOP) s.smem = (size_t)(8 * ((s.warps == 1 ? 256 : 512) + ONO_TOP_MAX)) * rows_of_cta;
   return s;
@@ -603,7 +604,8 @@ static TokShape tok_shape(long long rows, int V, int esz, int mode, int top) {
 template <typename T, typename O, int MODE, int GW, int NT>
 static cudaError_t tok_go(const TokDev& d, const TokShape& s, cudaStream_t st) {
   auto kern = tok_kernel<T, O, MODE, GW, NT>;
-  cudaError_t e = s.smem > 32768 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)s.smem) : cudaSuccess;
+  // The allowance is the function's, for all threads of the host: always the most that any call takes, or one call would lower it under another's launch.
+  cudaError_t e = s.smem > 32768 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TOK_KEPT_MAX) : cudaSuccess;
   if (e != cudaSuccess) return e;
   const long long units = (d.R + NT / (GW * 32) - 1) / (NT / (GW * 32));      // of a CTA, or a cluster
   cudaLaunchConfig_t cfg = {};

@@ -383,3 +383,41 @@ def test_alternatives_of_rows_of_few_logits_a_warp(vocab, dtype):
             targets = torch.randint(-1, vocab, (5,), device="cuda")
             for k in (1, 5, 8, 9, 20, 32):
                 _check_forward(x, targets, k)
+
+
+def test_two_threads_with_rows_of_different_lengths():
+    """One kernel with two sizes of its shared memory, launched from two threads of the host at once (a call into the library lets other threads run):
+    neither takes the other's allowance away."""
+    import ctypes as C
+    import threading
+
+    from oxidized_neural_orchestra_b200.ops import _lib
+    from oxidized_neural_orchestra_b200.ops.token_loss import token_loss
+
+    torch.manual_seed(11)
+    lib, jobs, failed = _lib.load(), [], []
+    for vocab in (200003, 70001):
+        x, t = torch.randn(1, vocab, device="cuda"), torch.randint(0, vocab, (1,), device="cuda")
+        want, got = torch.empty_like(x), torch.zeros_like(x)
+        token_loss(x, t, out=want)
+        jobs.append((x, t, want, got, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def work(x, t, want, got, stream):
+        vocab = x.shape[1]
+        a = _lib.OnoTokens(x=x.data_ptr(), targets=t.data_ptr(), R=1, ld=vocab, ld_out=vocab, ignore_id=-1, V=vocab, targets64=1, out=got.data_ptr(), scale=1.0)
+        for k in range(2000):
+            rc = lib.ono_tokens(C.byref(a), stream.cuda_stream)
+            if rc:
+                failed.append((vocab, k, rc))
+            if k % 200 == 199:
+                stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not failed, failed[:5]
+    assert all(torch.equal(want, got) for _, _, want, got, _ in jobs)
