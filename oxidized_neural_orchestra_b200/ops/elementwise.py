@@ -165,7 +165,10 @@ def optim_step(p: torch.Tensor, g: torch.Tensor, *, kind: str, lr: float, mu: fl
 
 
 def adam_tick(pows: torch.Tensor, b1: float, b2: float, stream=None) -> None:
-    """Advance the running products ``{b1^t, b2^t}`` kept in device memory (graph friendly)."""
+    """Advance the running products ``{b1^t, b2^t}`` kept in device memory (graph friendly), or in pinned memory of the host."""
+    if not pows.is_cuda and pows.is_pinned():      # (then it is for the current device)
+        _lib.check(_lib.load().ono_adam_tick(pows.data_ptr(), b1, b2, _lib.stream_ptr(stream)), "ono_adam_tick")
+        return
     _need_cuda(pows)
     launch(pows, stream, "ono_adam_tick", pows.data_ptr(), b1, b2)
 

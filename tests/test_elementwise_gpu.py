@@ -137,3 +137,23 @@ def test_philox_init_is_shard_independent_and_distributed_right():
     other = torch.empty(n, device="cuda")
     ew.philox_init(other, seed=8, index_offset=0, kind="uniform", a=-0.25, b=0.75)
     assert not torch.equal(u, other)
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_powers_in_pinned_host_memory(own_stream):
+    """Adam's powers may lie in pinned memory of the host; a step reads them there as well."""
+    from oxidized_neural_orchestra_b200.ops import elementwise as ew
+
+    stream = torch.cuda.Stream() if own_stream else None
+    got = []
+    for where in (lambda t: t.cuda(), lambda t: t.pin_memory()):
+        pows, p, m, v = where(torch.tensor([1.0, 1.0])), *(torch.full((100,), x, device="cuda") for x in (0.5, 0.1, 0.2))
+        g = torch.linspace(-1, 1, 100, device="cuda")
+        torch.cuda.synchronize()
+        for _ in range(3):
+            ew.adam_tick(pows, 0.9, 0.999, stream=stream)
+            ew.optim_step(p, g, kind="adam", lr=0.01, m=m, v=v, adam_pows=pows, stream=stream)
+        torch.cuda.synchronize()
+        got.append((pows.cpu(), p, m, v))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert not torch.equal(got[0][0], torch.ones(2))

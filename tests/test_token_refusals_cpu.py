@@ -181,3 +181,10 @@ def test_launches_go_to_the_tensors_device(monkeypatch):
     _launch.one_device(cuda[1], None, cuda[1])
     with pytest.raises(ValueError, match="different devices"):
         _launch.one_device(cuda[0], None, cuda[1])
+
+
+def test_powers_that_the_gpu_cannot_read():
+    from oxidized_neural_orchestra_b200.ops import elementwise as ew
+
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ew.adam_tick(torch.ones(2), 0.9, 0.999)
