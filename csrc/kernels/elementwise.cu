@@ -437,7 +437,14 @@ static void colsum_any(const T* d, int M, int N, int ld, float* out, float beta,
 // ------------------------------------------------------------------------------------------------
 struct OptimScalars {
   float lr, mu, b1, b2, eps, gs, adam_step, ob1, ob2;
+  bool once;
 };
+
+// An average moved towards x by the share of ob, whose weights add up to one: with ob rounded once beside 1 - ob as f32 has it, those of v would be 1.3e-5 too
+// much for good. One that is infinite stays.
+__device__ __forceinline__ float toward(float old, float ob, float difference) {
+  return fabsf(old) <= 3.402823466e38f ? fmaf(ob, difference, old) : old;
+}
 
 __device__ __forceinline__ float optim_one(int kind, const OptimScalars& s, float p, float g, float* m, float* v) {
   g *= s.gs;
@@ -448,16 +455,16 @@ __device__ __forceinline__ float optim_one(int kind, const OptimScalars& s, floa
     return p - s.lr * vel;
   }
   // adam.rs:75-91: step = lr*sqrt(1-b2^t)/(1-b1^t); p -= step * m / (sqrt(v) + eps)
-  const float mm = s.b1 * (*m) + s.ob1 * g;
-  const float vv = s.b2 * (*v) + s.ob2 * g * g;
+  const float mm = s.once ? toward(*m, s.ob1, g - *m) : s.b1 * (*m) + (1.0f - s.b1) * g;
+  const float vv = s.once ? toward(*v, s.ob2, fmaf(g, g, -*v)) : s.b2 * (*v) + (1.0f - s.b2) * g * g;
   *m = mm;
   *v = vv;
   return p - s.adam_step * mm / (sqrtf(vv) + s.eps);
 }
 
 __global__ void optim_kernel(const OnoOptim o) {
-  OptimScalars s{o.lr, o.mu, o.b1, o.b2, o.eps, o.grad_coef ? o.grad_scale * *o.grad_coef : o.grad_scale, 0.0f,
-                 o.ob1 != 0.0f ? o.ob1 : 1.0f - o.b1, o.ob2 != 0.0f ? o.ob2 : 1.0f - o.b2};
+  OptimScalars s{o.lr, o.mu, o.b1, o.b2, o.eps, o.grad_coef ? o.grad_scale * *o.grad_coef : o.grad_scale, 0.0f, o.ob1, o.ob2,
+                 o.ob1 != 0.0f || o.ob2 != 0.0f};
   if (o.kind == 2) {
     const float b1t = o.adam_pows[0], b2t = o.adam_pows[1];
     s.adam_step = o.lr * sqrtf(1.0f - b2t) / (1.0f - b1t);

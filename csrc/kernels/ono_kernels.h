@@ -189,7 +189,8 @@ typedef struct OnoOptim {
   void* p_bf16;          // optional bf16 shadow of p
   int zero_grad;         // 1: g is zeroed after use (g must be writable)
   const float* grad_coef;// optional device scalar that g is multiplied by as well (a clipping coefficient, ono_clip)
-  float ob1, ob2;        // Adam's 1 - b1 and 1 - b2; 0: taken from b1 and b2 (whose rounding is 1.3e-5 of 1 - 0.999)
+  float ob1, ob2;        // Adam's 1 - b1 and 1 - b2, each rounded once, the moments m + ob1 (g - m) and so on; both 0: all of it from b1 and b2, whose
+                         // rounding is 1.3e-5 of 1 - 0.999
 } OnoOptim;
 int ono_optim(const OnoOptim* o, ono_stream_t stream);
 int ono_adam_tick(float* pows, float b1, float b2, ono_stream_t stream);  // pows *= {b1, b2}

@@ -149,18 +149,23 @@ def optim_step(p: torch.Tensor, g: torch.Tensor, *, kind: str, lr: float, mu: fl
                b2: float = 0.999, eps: float = 1e-8, m: torch.Tensor | None = None,
                v: torch.Tensor | None = None, adam_pows: torch.Tensor | None = None,
                grad_scale: float = 1.0, p_bf16: torch.Tensor | None = None, zero_grad: bool = False,
-               grad_coef: torch.Tensor | None = None, stream=None) -> None:
+               grad_coef: torch.Tensor | None = None, exact_betas: bool | None = None, stream=None) -> None:
     """SGD / momentum / Adam on a flat f32 buffer (one kernel). ``grad_coef``: one f32 on the device that the gradient is multiplied by beside
-    ``grad_scale`` (``clip.grad_norm``'s coefficient for gradients scaled by ``grad_scale``). With it Adam's 1 - b1 and 1 - b2 are rounded once;
-    without it they are those of b1 and b2 as f32 has them, as the reference's (1.3e-5 off for 0.999)."""
+    ``grad_scale`` (``clip.grad_norm``'s coefficient for gradients scaled by ``grad_scale``).
+
+    ``exact_betas``: Adam's moments for b1 and b2 as they are given, 1 - b1 and 1 - b2 rounded once (True), or for b1 and b2 as f32 has them, as the
+    reference's are (False; 1 - b2 is then 1.3e-5 off for 0.999). None: True with ``grad_coef``, False without it; a step that clips nothing has the
+    same bits as one without clipping where both are told the same. ``adam_pows`` are f32 powers of b1 and b2 as f32 has them either way."""
     _need_cuda(p)
     coef = None
     if grad_coef is not None:
         if grad_coef.dtype != torch.float32 or grad_coef.numel() != 1 or grad_coef.get_device() != p.get_device():
             raise ValueError("grad_coef must be one float32 on the parameters' device")
         coef = grad_coef.data_ptr()
+        if exact_betas is None:
+            exact_betas = True
     o = _lib.OnoOptim(p.data_ptr(), g.data_ptr(), _p(m), _p(v), p.numel(), OPT_KIND[kind], lr, mu, b1, b2, eps, grad_scale, _p(adam_pows), _p(p_bf16),
-                      int(zero_grad), coef, 0.0 if coef is None else 1.0 - b1, 0.0 if coef is None else 1.0 - b2)
+                      int(zero_grad), coef, 1.0 - b1 if exact_betas else 0.0, 1.0 - b2 if exact_betas else 0.0)
     launch(p, stream, "ono_optim", C.byref(o))
 
 

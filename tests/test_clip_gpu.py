@@ -260,3 +260,64 @@ def test_sizes_around_what_one_cluster_takes(n):
         assert abs(norm.item() - want) <= NORM_TOL * want
         _check_out(ts, before, 0.5, 1.0)
         assert (whole[:lead] == SENTINEL).all() and (whole[lead + n:] == torch.tensor(SENTINEL, dtype=BF16)).all()
+
+
+def _adam(p, g, m, v, pows, lr, b1, b2, eps, **kw):
+    from oxidized_neural_orchestra_b200.ops import elementwise as ew
+
+    ew.adam_tick(pows, b1, b2)
+    ew.optim_step(p, g, kind="adam", lr=lr, b1=b1, b2=b2, eps=eps, m=m, v=v, adam_pows=pows, **kw)
+
+
+@pytest.mark.parametrize("exact", [False, True])
+def test_a_coefficient_of_one_is_no_other_step(exact):
+    """Adam over several steps: the same bits with a coefficient of one as without, and both the 64-bit recurrence of the betas that were asked for."""
+    torch.manual_seed(2)
+    n, steps, lr, b1, b2, eps = 50003, 5, 1e-3, 0.9, 0.999, 1e-8
+    gs = [torch.randn(n, device="cuda") for _ in range(steps)]
+    p0, one, sets = torch.randn(n, device="cuda"), torch.ones(1, device="cuda"), []
+    for kw in (dict(grad_coef=one, exact_betas=exact), dict(exact_betas=exact), dict(grad_coef=one) if exact else {}):
+        p, m, v, pows, powers = p0.clone(), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), torch.ones(2, device="cuda"), []
+        for g in gs:
+            _adam(p, g, m, v, pows, lr, b1, b2, eps, **kw)
+            powers.append(pows.double())
+        sets.append((p, m, v))
+    assert all(torch.equal(a, b) for s in sets[1:] for a, b in zip(sets[0], s))
+    if not exact:
+        b1, b2 = (float(torch.tensor(b)) for b in (b1, b2))
+    p, m, v, size = p0.double(), 0.0, 0.0, 0.0
+    for g, t in zip(gs, powers):
+        g = g.double()
+        m, v, size = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g, b1 * size + (1 - b1) * g.abs()
+        step = lr * torch.sqrt(1 - t[1]) / (1 - t[0])
+        p = p - step * m / (v.sqrt() + eps)
+        moved = step * size / (v.sqrt() + eps)
+    # a step's moments: four roundings at most, relative to the parts that are added up; a step of p: theirs, ten of its own, one of p
+    u = 2.0 ** -24
+    assert ((sets[0][1].double() - m).abs() <= 4 * steps * u * size).all() and ((sets[0][2].double() - v).abs() <= 4 * steps * u * v).all()
+    assert ((sets[0][0].double() - p).abs() <= steps * u * (p.abs() + 0.01) + steps * (8 * steps + 10) * u * moved.clamp_min(20 * lr)).all()
+
+
+def test_the_weights_of_the_second_moment_add_up_to_one():
+    """After 4000 steps the mean of v over many values is that of 64 bits: its roundings are of either sign, some 11 units on a value (half a step in each of the
+    last thousand or so, at random) and a few thousandths of one on the mean. Weights of 1.0000129 would show as that."""
+    torch.manual_seed(3)
+    n, b1, b2 = 65536, 0.9, 0.999
+    gs, one = [torch.randn(n, device="cuda") for _ in range(16)], torch.ones(1, device="cuda")
+    p, m, v, pows = (torch.zeros(k, device="cuda") for k in (n, n, n, 2))
+    want = torch.zeros(n, device="cuda", dtype=torch.float64)
+    pows.fill_(0.5)
+    squares = [g.double().square() for g in gs]
+    for k in range(4000):
+        _adam(p, gs[k % 16], m, v, pows, 1e-6, b1, b2, 1e-8, grad_coef=one)
+        pows.fill_(0.5)
+        want.mul_(b2).add_(squares[k % 16], alpha=1 - b2)
+    assert abs(float((v.double() / want).mean()) - 1.0) <= 2.0 ** -20
+
+
+def test_moments_that_left_the_range_stay_there():
+    for exact in (False, True):
+        p, m, v = torch.zeros(4, device="cuda"), torch.tensor([math.inf, -math.inf, 1.0, 0.0], device="cuda"), torch.tensor([1.0, 1.0, math.inf, 1.0], device="cuda")
+        g, pows = torch.tensor([1.0, 1.0, 1.0, 1e25], device="cuda"), torch.tensor([0.5, 0.5], device="cuda")
+        _adam(p, g, m, v, pows, 0.1, 0.9, 0.999, 1e-8, exact_betas=exact)
+        assert m[:2].tolist() == [math.inf, -math.inf] and v[2:].tolist() == [math.inf, math.inf] and p[2:].tolist() == [0.0, 0.0]
