@@ -444,15 +444,15 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
         g.u = mine.u;
       }
       const bool empty = g.z == 0.0f;
-      const float log2_z = empty ? 0.0f : log2f(g.z), at = shift_of(g.m);
+      const float ln_z = empty ? 0.0f : logf(g.z);
       // (the sum is relative to the shift, which is the maximum times log2 e rounded)
-      log_z = (fabsf(g.m) <= TOK_FAR ? log2_z - fmaf(g.m, LOG2E, -at) : log2_z) * LN2;
-      // ln p of a logit
-      auto lp = [&](float v) { return far || fabsf(v) > TOK_FAR ? (v - g.m) - log_z : (fmaf(v, LOG2E, -at) - log2_z) * LN2; };
+      log_z = fabsf(g.m) <= TOK_FAR ? fmaf(-fmaf(g.m, LOG2E, -shift_of(g.m)), LN2, ln_z) : ln_z;
+      // ln p of a logit: the distance from the maximum first, which is rounded once if at all
+      auto lp = [&](float v) { return (v - g.m) - log_z; };
       if (MODE != TOK_GRAD && gt == 0 && rank == 0) {
-        if (a.lse) a.lse[r] = empty ? ninf : far ? g.m + log_z : (at + log2_z) * LN2;
+        if (a.lse) a.lse[r] = empty ? ninf : g.m + log_z;
         if (a.logp) a.logp[r] = empty ? ninf : lp(x_t);
-        if (ENT && a.entropy) a.entropy[r] = empty ? 0.0f : (log2_z - g.u / g.z) * LN2;
+        if (ENT && a.entropy) a.entropy[r] = empty ? 0.0f : fmaf(-(g.u / g.z), LN2, ln_z);
       }
       if (TOP) {
         auto offer = [&](float v, int j) {

@@ -104,13 +104,13 @@ __global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const 
     z = group(z, add);
     if (ENT) u = group(u, add);
     const bool empty = z == 0.0f;
-    const float log2_z = empty ? 0.0f : log2f(z);
-    log_z = (fabsf(m) <= TOK_FAR ? log2_z - fmaf(m, LOG2E, -at) : log2_z) * LN2;
-    auto lp = [&](float v) { return far || fabsf(v) > TOK_FAR ? (v - m) - log_z : (fmaf(v, LOG2E, -at) - log2_z) * LN2; };
+    const float ln_z = empty ? 0.0f : logf(z);
+    log_z = fabsf(m) <= TOK_FAR ? fmaf(-fmaf(m, LOG2E, -at), LN2, ln_z) : ln_z;
+    auto lp = [&](float v) { return (v - m) - log_z; };
     if (MODE != TOK_GRAD && in && gl == 0) {
-      if (a.lse) a.lse[r] = !live ? 0.0f : empty ? ninf : far ? m + log_z : (at + log2_z) * LN2;
+      if (a.lse) a.lse[r] = !live ? 0.0f : empty ? ninf : m + log_z;
       if (a.logp) a.logp[r] = !live ? 0.0f : empty ? ninf : lp(x_t);
-      if (ENT && a.entropy) a.entropy[r] = !live || empty ? 0.0f : (log2_z - u / z) * LN2;
+      if (ENT && a.entropy) a.entropy[r] = !live || empty ? 0.0f : fmaf(-(u / z), LN2, ln_z);
     }
     if constexpr (TOP) {
       // The row's lanes find the largest of their largest logits, `top` times, of equal ones the lane with the lowest place; it goes on to its next.

@@ -421,3 +421,31 @@ def test_two_threads_with_rows_of_different_lengths():
     torch.cuda.synchronize()
     assert not failed, failed[:5]
     assert all(torch.equal(want, got) for _, _, want, got, _ in jobs)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(40, 3), (40, 10), (40, 100), (40, 1000), (3000, 2500), (40, 2500), (40, 10007), (40, 50257), (3, 128256)])
+def test_log_probabilities_are_rounded_as_the_definition_has_them(rows, vocab, dtype):
+    """Whole logits, one of them 40 or more above all others: lse is that one, and the others' log probabilities their distances from it, to the bit. (The
+    others weigh less than 1e-12; the sum is 1 to the 2^-22 of an exponential and the rounding of its shift, which is taken off again, so that its logarithm
+    is below 2^-21, less than half a step of a number from 16 on.)"""
+    from oxidized_neural_orchestra_b200.ops.token_loss import token_logprobs, token_loss
+
+    torch.manual_seed(vocab)
+    most = torch.randint(20, 101, (rows,), device="cuda")
+    least = torch.randint(40, 101, (rows, vocab), device="cuda")
+    at = torch.randint(0, vocab, (rows,), device="cuda")
+    least[torch.arange(rows, device="cuda"), at] = 0
+    x = (most.unsqueeze(1) - least).to(dtype)
+    targets = torch.randint(0, vocab, (rows,), device="cuda")
+    targets = torch.where(targets == at, (at + 1) % vocab, targets)
+    want = -least.gather(1, targets.unsqueeze(1)).squeeze(1).float()
+    k = min(4, vocab)
+    logp, lse, top, tid = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda"), torch.empty(rows, k, device="cuda"), torch.empty(rows, k, device="cuda", dtype=torch.int32)
+    for kw in (dict(), dict(entropy=torch.empty(rows, device="cuda")), dict(top_logp=top, top_id=tid)):
+        token_logprobs(x, targets, logp=logp, lse=lse, **kw)
+        assert torch.equal(lse, most.float()) and torch.equal(logp, want)
+    assert torch.equal(top[:, 1:], -least.gather(1, tid[:, 1:].long()).float()) and torch.equal(tid[:, 0].long(), at)
+    lse.zero_(), logp.zero_()
+    token_loss(x, targets, out=torch.empty_like(x), logp=logp, lse=lse)
+    assert torch.equal(lse, most.float()) and torch.equal(logp, want)
