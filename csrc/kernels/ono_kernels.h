@@ -533,6 +533,7 @@ typedef struct OnoTokens {
   const float* weight;       // [R], optional (ones)
   float scale;
   int* status;
+  float* lse_low;            // [R], optional beside lse and without out: what rounding to f32 took off it
 } OnoTokens;
 int ono_tokens(const OnoTokens* t, ono_stream_t stream);
 // out = d_logp (1[target] - p) - d_entropy p (ln p + entropy): the logits' gradient from those of ono_tokens' results.
@@ -544,6 +545,7 @@ typedef struct OnoTokensGrad {
   const float *lse, *entropy, *d_logp, *d_entropy;   // [R]; d_logp optional; entropy and d_entropy both or none
   void* out; int out_bf16;   // [R, ld_out], may be x (same type)
   int* status;
+  const float* lse_low;      // [R], optional: ono_tokens' of that name. Without it half a step of lse is a relative error of the row's p.
 } OnoTokensGrad;
 int ono_tokens_grad(const OnoTokensGrad* t, ono_stream_t stream);
 

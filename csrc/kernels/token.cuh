@@ -12,24 +12,24 @@ namespace ono {
 void set_error(const char* fmt, const char* a, long long b, long long c);
 
 // What a launch computes: log probabilities, with entropy, with entropy and alternatives, the token loss's gradient, the gradient from
-// those of log probability and entropy.
-enum TokMode : int { TOK_LOGP, TOK_ENTROPY, TOK_TOP, TOK_LOSS, TOK_GRAD };
+// those of log probability and entropy (of short rows, with lse_low too).
+enum TokMode : int { TOK_LOGP, TOK_ENTROPY, TOK_TOP, TOK_LOSS, TOK_GRAD, TOK_GRAD_LOW };
 
 struct TokDev {
   const void* x; const void* targets;
   long long R, ld, ld_out, ignore_id;
   int V, targets64, top, per, staged;      // per: 16-byte groups of a row that a CTA takes; staged: they are kept in shared memory
-  float *logp, *lse, *entropy, *top_logp;
+  float *logp, *lse, *lse_low, *entropy, *top_logp;
   int* top_id;
   void* out;
   const float* weight;
   float scale;
-  const float *lse_in, *entropy_in, *d_logp, *d_entropy;
+  const float *lse_in, *lse_low_in, *entropy_in, *d_logp, *d_entropy;
   int* status;
 };
 
-// lse comes rounded to f32: half a step of it is an error relative in p. Beyond this (2^-17 there) the gradient takes the row's maximum and sum
-// again; a row that is masked by the type's lowest value would have no sum at all beside it.
+// lse comes rounded to f32: half a step of it is an error relative in p (2^-21 from 8 on), which lse_low takes away where it is given. Beyond this (2^-17 there)
+// the gradient takes the row's maximum and sum again; a row that is masked by the type's lowest value would have no sum at all beside it.
 constexpr float LSE_EXACT = 128.0f;
 constexpr int TOK_CTAS = 8;      // of a cluster, at most
 
@@ -64,6 +64,10 @@ constexpr float TOK_FAR = 1e6f;
 // What exponents are taken relative to, in units of log2: the maximum's, of any size, rounded; a logit is then one multiply-add, and its error
 // that of the difference. Zero where there is nothing but far negative ones (all exponentials are zero then).
 __device__ __forceinline__ float shift_of(float m) { return m < -TOK_FAR ? 0.0f : m * LOG2E; }
+
+// What rounding took off `lse`, of a sum z relative to the shift `at`: to the bits of z, so in 64. With it p = 2^(x log2 e - at) / z, as if neither had been
+// joined to the other; log2 e is the one that the exponents are made with. Out of line: few calls ask for it.
+static __device__ __noinline__ float low_of(float at, float z, float lse) { return (float)(((double)at + log2((double)z)) / (double)LOG2E - (double)lse); }
 
 __device__ __forceinline__ uint4 load16(const void* p) {
   uint4 v;

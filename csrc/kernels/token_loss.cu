@@ -318,6 +318,7 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
         if (gt == 0) {
           if (a.logp) a.logp[r] = 0.0f;
           if (a.lse) a.lse[r] = 0.0f;
+          if (FWD && a.lse_low) a.lse_low[r] = 0.0f;
           if (ENT && a.entropy) a.entropy[r] = 0.0f;
         }
         if (TOP && gt < K) { a.top_logp[r * K + gt] = ninf; a.top_id[r * K + gt] = -1; }
@@ -326,11 +327,12 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
       if (staged && r + stride < a.R && target(raw_next) >= 0) fetch(r + stride);
       continue;
     }
-    float x_t = 0.0f, i0 = 1.0f, i1 = 0.0f, i2 = 0.0f, i3 = 0.0f;
+    float x_t = 0.0f, i0 = 1.0f, i1 = 0.0f, i2 = 0.0f, i3 = 0.0f, low = 0.0f;
     if (MODE != TOK_GRAD && gt == 0 && a.targets) x_t = to_f32(x[t]);
     if (MODE == TOK_LOSS && a.weight) i0 = __ldg(a.weight + r);
     if (MODE == TOK_GRAD) {
       i0 = __ldg(a.lse_in + r);
+      if (a.lse_low_in) low = __ldg(a.lse_low_in + r);
       if (a.d_logp) i1 = __ldg(a.d_logp + r);
       if (a.d_entropy) { i2 = __ldg(a.d_entropy + r); i3 = __ldg(a.entropy_in + r); }
     }
@@ -450,7 +452,9 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
       // ln p of a logit: the distance from the maximum first, which is rounded once if at all
       auto lp = [&](float v) { return (v - g.m) - log_z; };
       if (MODE != TOK_GRAD && gt == 0 && rank == 0) {
-        if (a.lse) a.lse[r] = empty ? ninf : g.m + log_z;
+        const float lse = empty ? ninf : g.m + log_z;
+        if (a.lse) a.lse[r] = lse;
+        if (FWD && a.lse_low) a.lse_low[r] = empty || far ? 0.0f : low_of(shift_of(g.m), g.z, lse);
         if (a.logp) a.logp[r] = empty ? ninf : lp(x_t);
         if (ENT && a.entropy) a.entropy[r] = empty ? 0.0f : fmaf(-(g.u / g.z), LN2, ln_z);
       }
@@ -551,8 +555,8 @@ __global__ void __launch_bounds__(NT, tok_resident(MODE, W, NT)) tok_kernel(cons
       }
     } else if (MODE == TOK_GRAD) {
       if (fabsf(i0) <= LSE_EXACT) {
-        // -p (g + h (ln p + H)) with ln p = ln 2 (q - off): q = x log2 e - c, c the product lse log2 e rounded, off what that took off
-        const float c = i0 * LOG2E, off = fmaf(i0, LOG2E, -c), f = -exp2_of(-off);
+        // -p (g + h (ln p + H)) with ln p = ln 2 (q - off): q = x log2 e - c, c the product lse log2 e rounded, off what that and lse's own rounding took off
+        const float c = i0 * LOG2E, off = fmaf(low, LOG2E, fmaf(i0, LOG2E, -c)), f = -exp2_of(-off);
         const float2 at = both(-c), A = both(f * (i1 + i2 * (i3 - LN2 * off))), B = both(f * LN2 * i2);
         if (a.d_entropy)
           write(xh, xt, i1, [&](float2 v) {
@@ -650,7 +654,7 @@ using namespace ono;
 
 extern "C" int ono_tokens(const OnoTokens* t, ono_stream_t stream) {
   if (!t || t->R < 0 || t->V <= 0 || t->V > ONO_DIM_MAX || t->ld < t->V || (t->R && !t->x) || t->top < 0 || t->top > ONO_TOP_MAX || t->top > t->V ||
-      (t->top > 0 && t->R && (!t->top_logp || !t->top_id)) || (t->out && (t->ld_out < t->V || t->entropy || t->top)) || (!t->targets && (t->logp || t->out))) {
+      (t->top > 0 && t->R && (!t->top_logp || !t->top_id)) || (t->out && (t->ld_out < t->V || t->entropy || t->top || t->lse_low)) || (t->lse_low && !t->lse) || (!t->targets && (t->logp || t->out))) {
     set_error("bad tokens args%s", "", 0, 0);
     return -1;
   }
@@ -658,7 +662,7 @@ extern "C" int ono_tokens(const OnoTokens* t, ono_stream_t stream) {
   if (t->R == 0) return 0;
   TokDev d = {};
   d.x = t->x; d.targets = t->targets; d.R = t->R; d.ld = t->ld; d.ld_out = t->ld_out; d.ignore_id = t->ignore_id;
-  d.V = t->V; d.targets64 = t->targets64; d.top = t->top; d.logp = t->logp; d.lse = t->lse; d.entropy = t->entropy;
+  d.V = t->V; d.targets64 = t->targets64; d.top = t->top; d.logp = t->logp; d.lse = t->lse; d.lse_low = t->lse_low; d.entropy = t->entropy;
   d.top_logp = t->top_logp; d.top_id = t->top_id; d.out = t->out; d.weight = t->weight; d.scale = t->scale; d.status = t->status;
   cudaStream_t st = (cudaStream_t)stream;
   using B = __nv_bfloat16;
@@ -681,7 +685,7 @@ extern "C" int ono_tokens_grad(const OnoTokensGrad* t, ono_stream_t stream) {
   TokDev d = {};
   d.x = t->x; d.targets = t->targets; d.R = t->R; d.ld = t->ld; d.ld_out = t->ld_out; d.ignore_id = t->ignore_id;
   d.V = t->V; d.targets64 = t->targets64; d.out = t->out; d.status = t->status;
-  d.lse_in = t->lse; d.entropy_in = t->entropy; d.d_logp = t->d_logp; d.d_entropy = t->d_entropy;
+  d.lse_in = t->lse; d.lse_low_in = t->lse_low; d.entropy_in = t->entropy; d.d_logp = t->d_logp; d.d_entropy = t->d_entropy;
   cudaStream_t st = (cudaStream_t)stream;
   using B = __nv_bfloat16;
   if (t->x_bf16) return t->out_bf16 ? tok_run<B, B, TOK_GRAD>(d, st) : tok_run<B, float, TOK_GRAD>(d, st);

@@ -12,7 +12,7 @@ namespace ono {
 template <typename T, typename O, int MODE, int NV>
 __global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const __grid_constant__ TokDev a, int lg) {
   constexpr int E = TokVec<T>::E;
-  constexpr bool TOP = MODE == TOK_TOP, ENT = MODE == TOK_ENTROPY || MODE == TOK_TOP, FWD = MODE <= TOK_TOP;
+  constexpr bool TOP = MODE == TOK_TOP, ENT = MODE == TOK_ENTROPY || MODE == TOK_TOP, FWD = MODE <= TOK_TOP, LOW = MODE == TOK_GRAD_LOW, GRAD = MODE == TOK_GRAD || LOW;
   const float ninf = __int_as_float(0xff800000);
   const unsigned int full = 0xffffffffu;
   const int lane = threadIdx.x & 31, G = NV == 1 ? 1 << lg : 32, gl = lane & (G - 1);
@@ -44,10 +44,11 @@ __global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const 
       for (int k = 0; k < E; ++k) if (j + k >= 0 && j + k < a.V) o[k] = x[j + k];
     }
   }
-  float i0 = 1.0f, i1 = 0.0f, i2 = 0.0f, i3 = 0.0f;
+  float i0 = 1.0f, i1 = 0.0f, i2 = 0.0f, i3 = 0.0f, low = 0.0f;
   if (MODE == TOK_LOSS && a.weight) i0 = __ldg(a.weight + rr);
-  if (MODE == TOK_GRAD) {
+  if (GRAD) {
     i0 = __ldg(a.lse_in + rr);
+    if (LOW) low = __ldg(a.lse_low_in + rr);
     if (a.d_logp) i1 = __ldg(a.d_logp + rr);
     if (a.d_entropy) { i2 = __ldg(a.d_entropy + rr); i3 = __ldg(a.entropy_in + rr); }
   }
@@ -58,7 +59,7 @@ __global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const 
   }
   const bool live = t >= 0;
   float x_t = 0.0f;
-  if (MODE != TOK_GRAD && live && gl == 0) x_t = to_f32(x[t]);
+  if (!GRAD && live && gl == 0) x_t = to_f32(x[t]);
   auto group = [&](float v, auto join) {      // over the row's lanes
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) if (o < G) v = join(v, __shfl_xor_sync(full, v, o));
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const 
   };
   float m = 0.0f, z = 1.0f, u = 0.0f, log_z = 0.0f;
   bool far = false;
-  if (MODE != TOK_GRAD || __any_sync(full, live && fabsf(i0) > LSE_EXACT)) {
+  if (!GRAD || __any_sync(full, live && fabsf(i0) > LSE_EXACT)) {
     m = fmaxf(xh, xt);
 #pragma unroll
     for (int q = 0; q < NV; ++q) m = fmaxf(m, TokVec<T>::most(w[q]));
@@ -107,8 +108,10 @@ __global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const 
     const float ln_z = empty ? 0.0f : logf(z);
     log_z = fabsf(m) <= TOK_FAR ? fmaf(-fmaf(m, LOG2E, -at), LN2, ln_z) : ln_z;
     auto lp = [&](float v) { return (v - m) - log_z; };
-    if (MODE != TOK_GRAD && in && gl == 0) {
-      if (a.lse) a.lse[r] = !live ? 0.0f : empty ? ninf : m + log_z;
+    if (!GRAD && in && gl == 0) {
+      const float lse = empty ? ninf : m + log_z;
+      if (a.lse) a.lse[r] = !live ? 0.0f : lse;
+      if (FWD && a.lse_low) a.lse_low[r] = !live || empty || far ? 0.0f : low_of(at, z, lse);
       if (a.logp) a.logp[r] = !live ? 0.0f : empty ? ninf : lp(x_t);
       if (ENT && a.entropy) a.entropy[r] = !live || empty ? 0.0f : fmaf(-(u / z), LN2, ln_z);
     }
@@ -195,7 +198,7 @@ __global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const 
       B = -i2 * LN2;
     } else {      // see token_loss.cu
       c = i0 * LOG2E;
-      const float off = fmaf(i0, LOG2E, -c), f = -exp2_of(-off);
+      const float off = LOW ? fmaf(low, LOG2E, fmaf(i0, LOG2E, -c)) : fmaf(i0, LOG2E, -c), f = -exp2_of(-off);
       A = f * (i1 + i2 * (i3 - LN2 * off));
       B = f * LN2 * i2;
     }
@@ -274,9 +277,14 @@ int tok_short(const TokDev& d, int mode, int x_bf16, int out_bf16, cudaStream_t 
     case TOK_LOSS:
       if (x_bf16) return out_bf16 ? tok_short_go<B, B, TOK_LOSS>(d, st) : tok_short_go<B, float, TOK_LOSS>(d, st);
       return out_bf16 ? tok_short_go<float, B, TOK_LOSS>(d, st) : tok_short_go<float, float, TOK_LOSS>(d, st);
-    default:
-      if (x_bf16) return out_bf16 ? tok_short_go<B, B, TOK_GRAD>(d, st) : tok_short_go<B, float, TOK_GRAD>(d, st);
-      return out_bf16 ? tok_short_go<float, B, TOK_GRAD>(d, st) : tok_short_go<float, float, TOK_GRAD>(d, st);
+    default: {      // (a form of its own with lse_low: one more value a row spills, gradient of 16384 x 1000 f32 19.6 us, so 20.6)
+      auto grad = [&](auto mode) {
+        constexpr int M = mode.value;
+        if (x_bf16) return out_bf16 ? tok_short_go<B, B, M>(d, st) : tok_short_go<B, float, M>(d, st);
+        return out_bf16 ? tok_short_go<float, B, M>(d, st) : tok_short_go<float, float, M>(d, st);
+      };
+      return d.lse_low_in ? grad(std::integral_constant<int, TOK_GRAD_LOW>{}) : grad(std::integral_constant<int, TOK_GRAD>{});
+    }
   }
 }
 }  // namespace ono

@@ -210,6 +210,7 @@ class OnoTokens(C.Structure):
         ("V", C.c_int), ("x_bf16", C.c_int), ("targets64", C.c_int), ("top", C.c_int),
         ("logp", C.c_void_p), ("lse", C.c_void_p), ("entropy", C.c_void_p), ("top_logp", C.c_void_p), ("top_id", C.c_void_p),
         ("out", C.c_void_p), ("out_bf16", C.c_int), ("weight", C.c_void_p), ("scale", C.c_float), ("status", C.c_void_p),
+        ("lse_low", C.c_void_p),
     ]
 
 
@@ -219,7 +220,7 @@ class OnoTokensGrad(C.Structure):
         ("R", C.c_longlong), ("ld", C.c_longlong), ("ld_out", C.c_longlong), ("ignore_id", C.c_longlong),
         ("V", C.c_int), ("x_bf16", C.c_int), ("targets64", C.c_int),
         ("lse", C.c_void_p), ("entropy", C.c_void_p), ("d_logp", C.c_void_p), ("d_entropy", C.c_void_p),
-        ("out", C.c_void_p), ("out_bf16", C.c_int), ("status", C.c_void_p),
+        ("out", C.c_void_p), ("out_bf16", C.c_int), ("status", C.c_void_p), ("lse_low", C.c_void_p),
     ]
 
 

@@ -56,7 +56,7 @@ def _out(out: torch.Tensor, logits: torch.Tensor) -> int:
     return pitch
 
 
-def _tokens(logits, targets, ignore_id, status, stream, *, logp=None, lse=None, entropy=None, top_logp=None, top_id=None, out=None, ld_out=0,
+def _tokens(logits, targets, ignore_id, status, stream, *, logp=None, lse=None, lse_low=None, entropy=None, top_logp=None, top_id=None, out=None, ld_out=0,
             weight=None, scale=1.0) -> None:
     ld = _logits(logits)
     rows, vocab = logits.shape
@@ -71,12 +71,12 @@ def _tokens(logits, targets, ignore_id, status, stream, *, logp=None, lse=None, 
         if top > min(TOP_MAX, vocab):
             raise ValueError(f"at most {min(TOP_MAX, vocab)} alternatives")
     ignore_id = id_or_none(ignore_id)
-    one_device(logits, targets, status, logp, lse, entropy, top_logp, top_id, out, weight)
+    one_device(logits, targets, status, logp, lse, lse_low, entropy, top_logp, top_id, out, weight)
     a = _lib.OnoTokens(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, ld, ld_out, ignore_id,
                        vocab, logits.dtype == torch.bfloat16, wide, top, _column(logp, rows, "logp"), _column(lse, rows, "lse"),
                        _column(entropy, rows, "entropy"), top_logp.data_ptr() if top else None, top_id.data_ptr() if top else None,
                        None if out is None else out.data_ptr(), out is not None and out.dtype == torch.bfloat16, _column(weight, rows, "weight"),
-                       scale, status_ptr(status))
+                       scale, status_ptr(status), _column(lse_low, rows, "lse_low"))
     if rows == 0:
         return
     if vocab == 0:
@@ -85,15 +85,17 @@ def _tokens(logits, targets, ignore_id, status, stream, *, logp=None, lse=None, 
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None, *, logp: torch.Tensor | None = None, lse: torch.Tensor | None = None,
-                   entropy: torch.Tensor | None = None, top_logp: torch.Tensor | None = None, top_id: torch.Tensor | None = None,
-                   ignore_id: int | None = -1, status: torch.Tensor | None = None, stream=None) -> None:
+                   lse_low: torch.Tensor | None = None, entropy: torch.Tensor | None = None, top_logp: torch.Tensor | None = None,
+                   top_id: torch.Tensor | None = None, ignore_id: int | None = -1, status: torch.Tensor | None = None, stream=None) -> None:
     """With ``lse = ln sum_v exp(x_v)``: ``logp[r] = x[r, targets[r]] - lse[r]``, ``entropy[r] = -sum_v p_v ln p_v`` (natural logarithms, f32), and
     the ``top_id.shape[1]`` (at most ``TOP_MAX``) largest logits' tokens and log probabilities, the largest first and among equal ones
     the lowest token first. Where a row has fewer logits above -inf, id -1 and -inf follow. The logits are read once. Without ``targets`` every row
-    counts and there is no ``logp``."""
+    counts and there is no ``logp``. ``lse_low``: what rounding to f32 took off ``lse``, for ``token_logprobs_grad``."""
     if targets is None and logp is not None:
         raise ValueError("logp needs targets")
-    _tokens(logits, targets, ignore_id, status, stream, logp=logp, lse=lse, entropy=entropy, top_logp=top_logp, top_id=top_id)
+    if lse_low is not None and lse is None:
+        raise ValueError("lse_low needs lse")
+    _tokens(logits, targets, ignore_id, status, stream, logp=logp, lse=lse, lse_low=lse_low, entropy=entropy, top_logp=top_logp, top_id=top_id)
 
 
 def token_loss(logits: torch.Tensor, targets: torch.Tensor, *, out: torch.Tensor, logp: torch.Tensor | None = None,
@@ -108,9 +110,12 @@ def token_loss(logits: torch.Tensor, targets: torch.Tensor, *, out: torch.Tensor
 
 def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, *, lse: torch.Tensor, out: torch.Tensor,
                         d_logp: torch.Tensor | None = None, entropy: torch.Tensor | None = None, d_entropy: torch.Tensor | None = None,
-                        ignore_id: int | None = -1, status: torch.Tensor | None = None, stream=None) -> None:
+                        lse_low: torch.Tensor | None = None, ignore_id: int | None = -1, status: torch.Tensor | None = None, stream=None) -> None:
     """The logits' gradient from those of ``token_logprobs``' results, ``lse`` and ``entropy`` being what it returned:
-    ``out = d_logp (1[v = target] - p) - d_entropy p (ln p + entropy)``. ``out`` may be ``logits``."""
+    ``out = d_logp (1[v = target] - p) - d_entropy p (ln p + entropy)``. ``out`` may be ``logits``.
+
+    p is ``exp(logits - lse)``, so that half a step of ``lse`` is a relative error of a row's p: 4.8e-7 where ``lse`` is from 8 to 16, 3.8e-6 from 64 to 128 (beyond that
+    the row's sum is taken again). A gradient in bf16 does not show it; for one in f32 give ``lse_low`` too, and p is as exact as ``token_loss`` has it."""
     ld = _logits(logits)
     rows, vocab = logits.shape
     wide = _targets(targets, rows)
@@ -122,11 +127,11 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor | None, *, l
     if (entropy is None) != (d_entropy is None):
         raise ValueError("d_entropy needs the entropy, which has no other use")
     ignore_id = id_or_none(ignore_id)
-    one_device(logits, targets, status, lse, entropy, d_logp, d_entropy, out)
+    one_device(logits, targets, status, lse, lse_low, entropy, d_logp, d_entropy, out)
     a = _lib.OnoTokensGrad(logits.data_ptr(), None if targets is None else targets.data_ptr(), rows, ld, ld_out, ignore_id,
                            vocab, logits.dtype == torch.bfloat16, wide, _column(lse, rows, "lse"), _column(entropy, rows, "entropy"),
                            _column(d_logp, rows, "d_logp"), _column(d_entropy, rows, "d_entropy"), out.data_ptr(), out.dtype == torch.bfloat16,
-                           status_ptr(status))
+                           status_ptr(status), _column(lse_low, rows, "lse_low"))
     if rows == 0 or vocab == 0:
         return
     launch(logits, stream, "ono_tokens_grad", C.byref(a))

@@ -449,3 +449,65 @@ def test_log_probabilities_are_rounded_as_the_definition_has_them(rows, vocab, d
     lse.zero_(), logp.zero_()
     token_loss(x, targets, out=torch.empty_like(x), logp=logp, lse=lse)
     assert torch.equal(lse, most.float()) and torch.equal(logp, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(64, 3), (64, 10), (64, 100), (64, 1000), (3000, 1100), (64, 2500), (64, 10007)])
+def test_gradient_with_what_rounding_took_off_lse(rows, vocab, dtype):
+    """Rows of equal logits, p = 1 / V, whose lse is from 64 to 128 and rounded by up to 3.8e-6. With lse_low none of that is left: two exponentials of 2^-22 (one
+    in the sum), at most 22 additions and ten other roundings of half a step. (A thread has at most 16 logits an accumulator at these sizes.)"""
+    from oxidized_neural_orchestra_b200.ops.token_loss import token_logprobs, token_logprobs_grad
+
+    torch.manual_seed(vocab)
+    c = (torch.rand(rows, 1, device="cuda") * 50 + 64).to(dtype)
+    x = c.expand(rows, vocab).contiguous()
+    targets = torch.randint(0, vocab, (rows,), device="cuda")
+    lse, low, ent, g = (torch.empty(rows, device="cuda") for _ in range(4))
+    g.normal_()
+    tol = 2 * 2.0 ** -22 + 32 * 2.0 ** -24
+    want = (torch.zeros(rows, vocab, device="cuda", dtype=torch.float64).scatter_(1, targets.unsqueeze(1), 1.0) - 1.0 / vocab) * g.double().unsqueeze(1)
+    for kw in (dict(), dict(entropy=ent), dict(entropy=ent, top_logp=torch.empty(rows, 2, device="cuda"), top_id=torch.empty(rows, 2, device="cuda", dtype=torch.int32))):
+        low.fill_(SENTINEL)
+        token_logprobs(x, targets, lse=lse, lse_low=low, **kw)
+        # (log2 e as f32 has it is 1.4e-8 off)
+        assert ((lse.double() + low.double() - c.double().squeeze(1) - math.log(vocab)).abs() <= tol + 1.4e-8 * math.log(vocab)).all()
+        assert (low.abs() <= 2.0 ** -18 + tol).all()
+        d = torch.empty(rows, vocab, device="cuda")
+        token_logprobs_grad(x, targets, lse=lse, lse_low=low, d_logp=g, out=d)
+        assert ((d.double() - want).abs() <= g.double().abs().unsqueeze(1) * (tol / vocab + 2.0 ** -24 * (want != 0))).all()
+        other = torch.ones(rows, vocab, device="cuda") * SENTINEL
+        token_logprobs_grad(x, targets, lse=lse, lse_low=low, d_logp=g, entropy=ent, d_entropy=torch.zeros_like(g), out=other)
+        assert torch.equal(other.isnan(), d.isnan()) and ((other - d).abs() <= 4 * 2.0 ** -24 * d.abs() + 2.0 ** -24 * g.abs().unsqueeze(1)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(12, 50), (12, 1030), (2400, 1030), (12, 30011)])
+def test_what_rounding_took_off_of_rows_of_every_kind(rows, vocab, dtype):
+    """None where there is no sum or a gradient takes it again: the gradient is the one without it there, and within its bounds elsewhere."""
+    from oxidized_neural_orchestra_b200.ops.token_loss import token_logprobs, token_logprobs_grad
+
+    torch.manual_seed(vocab)
+    x, _ = _logits(rows, vocab, dtype, vocab + 3)
+    x[1] = -math.inf
+    x[2], x[3] = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x[4, 0], x[5, 1] = math.nan, math.inf
+    x[6] *= 1e30
+    x[7] += 500.0
+    targets = torch.randint(0, vocab, (rows,), device="cuda")
+    targets[0] = -1
+    lse, low, ent, g, h = (torch.full((rows,), SENTINEL, device="cuda") for _ in range(5))
+    g.normal_(), h.normal_()
+    token_logprobs(x, targets, lse=lse, lse_low=low, entropy=ent)
+    assert (low[[0, 1, 2, 3, 6]] == 0).all() and low[[4, 5]].isnan().logical_or(low[[4, 5]] == 0).all()
+    ok = torch.isfinite(lse)
+    assert (low[ok].abs() <= 2.0 ** -23 * lse[ok].abs().clamp_min(1.0)).all()
+    a, b = torch.empty(rows, vocab, device="cuda"), torch.empty(rows, vocab, device="cuda")
+    token_logprobs_grad(x, targets, lse=lse, entropy=ent, d_logp=g, d_entropy=h, out=a)
+    token_logprobs_grad(x, targets, lse=lse, lse_low=low, entropy=ent, d_logp=g, d_entropy=h, out=b)
+    assert torch.equal(a[:8].isnan(), b[:8].isnan())
+    again = [0, 1, 2, 3, 6, 7]
+    assert torch.equal(a[again], b[again])
+    _, _, rlse, H, _, _ = _ref(x, targets, vocab)
+    size = g.abs() + h.abs() * (2 * H.clamp_min(1.0) + 30).float()
+    rest = slice(8, None)
+    assert ((a - b).abs()[rest] <= (size * 2.0 ** -22 * rlse.float().abs().clamp_min(1.0))[rest].unsqueeze(1)).all()

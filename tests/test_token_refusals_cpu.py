@@ -188,3 +188,18 @@ def test_powers_that_the_gpu_cannot_read():
 
     with pytest.raises(RuntimeError, match="CUDA"):
         ew.adam_tick(torch.ones(2), 0.9, 0.999)
+
+
+def test_what_rounding_took_off_lse():
+    from oxidized_neural_orchestra_b200.ops.token_loss import token_logprobs, token_logprobs_grad
+
+    x, t, v = torch.zeros(3, 9), torch.zeros(3, dtype=torch.int64), torch.zeros(3)
+    with pytest.raises(ValueError, match="lse_low needs lse"):
+        token_logprobs(x, t, logp=v, lse_low=v)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        token_logprobs(x, t, lse=v, lse_low=v)
+    for bad in (torch.zeros(4), v.double(), torch.zeros(6)[::2], torch.zeros(3, 1)):
+        with pytest.raises((ValueError, RuntimeError)):
+            token_logprobs(x, t, lse=v, lse_low=bad)
+        with pytest.raises((ValueError, RuntimeError)):
+            token_logprobs_grad(x, t, lse=v, lse_low=bad, d_logp=v, out=x)
