@@ -14,6 +14,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "chain.cuh"
 #include "ono_kernels.h"
@@ -334,6 +335,38 @@ __global__ void __launch_bounds__(SMALL_THREADS) clip_small_kernel(const __grid_
   }
 }
 
+static cudaLaunchConfig_t small_launch(cudaLaunchAttribute& attr, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(SMALL_CTAS);
+  cfg.blockDim = dim3(SMALL_THREADS);
+  cfg.stream = st;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = SMALL_CTAS; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+// Clusters of that size that the current device has room for, asked for once: 16 blocks are more than every device, or part of one, has to take.
+static int clip_clusters() {
+  constexpr int DEVICES = 64;
+  static std::atomic<int> known[DEVICES];      // one more than there are
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= DEVICES) return 0;
+  int k = known[device].load();
+  if (k == 0) {
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = small_launch(attr, nullptr);
+    int clusters = 0;
+    if (cudaFuncSetAttribute(clip_small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, clip_small_kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    known[device].store(k = clusters + 1);
+  }
+  return k - 1;
+}
+
 template <int G>
 static cudaError_t clip_go(const OnoClip* c, cudaStream_t st) {
   constexpr int CLIP_CHUNK = 8 * CLIP_THREADS * G;
@@ -368,6 +401,10 @@ static cudaError_t clip_go(const OnoClip* c, cudaStream_t st) {
 
 using namespace ono;
 
+extern "C" int ono_clip_one_launch(int n_tensors, long long values, int clusters) {
+  return clusters > 0 && n_tensors <= SMALL_TENSORS && values <= SMALL_CHUNKS * 8ll * SMALL_THREADS;
+}
+
 extern "C" long long ono_clip_scratch(void) { return CLIP_MAX_BLOCKS * 8; }
 
 extern "C" int ono_clip(const OnoClip* c, ono_stream_t stream) {
@@ -388,23 +425,14 @@ extern "C" int ono_clip(const OnoClip* c, ono_stream_t stream) {
     }
   }
   cudaStream_t st = (cudaStream_t)stream;
-  if (c->n_tensors <= SMALL_TENSORS && values <= SMALL_CHUNKS * 8ll * SMALL_THREADS) {
+  if (ono_clip_one_launch(c->n_tensors, values, clip_clusters())) {
     ClipSmall b;
     int next = 0;
     if (clip_fill(b, c, next, 8 * SMALL_THREADS) && b.end[b.count - 1] <= SMALL_CHUNKS) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(SMALL_CTAS);
-      cfg.blockDim = dim3(SMALL_THREADS);
-      cfg.stream = st;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = SMALL_CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      cudaError_t e = cudaFuncSetAttribute(clip_small_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, clip_small_kernel, b, c->scale, c->max_norm, c->norm, c->coef, (int)(c->out != nullptr));
-      if (e != cudaSuccess) { set_error("clip launch: %s", cudaGetErrorString(e), 0, 0); return -7; }
-      return 0;
+      cudaLaunchAttribute attr;
+      const cudaLaunchConfig_t cfg = small_launch(attr, st);
+      if (cudaLaunchKernelEx(&cfg, clip_small_kernel, b, c->scale, c->max_norm, c->norm, c->coef, (int)(c->out != nullptr)) == cudaSuccess) return 0;
+      cudaGetLastError();      // (fewer multiprocessors than were asked about: the form below runs on any)
     }
   }
   // Two groups a thread, or four. (Us, two, four: 101 k f32 values 5.0, 6.8; 8 M bf16 15.4, 17.6, 17 M 27.9, 25.3, 90 M 137, 119; 30 M f32 71, 69, 90 M 209, 185;

@@ -566,6 +566,8 @@ typedef struct OnoClip {
   void* scratch; long long scratch_bytes;
 } OnoClip;
 long long ono_clip_scratch(void);
+// Whether one cluster takes them all, on a device with room for so many of its size (at most: tensors that begin anywhere may need one chunk more than it has).
+int ono_clip_one_launch(int n_tensors, long long values, int clusters);
 int ono_clip(const OnoClip* c, ono_stream_t stream);
 
 #ifdef __cplusplus

@@ -107,6 +107,8 @@ def _declare(lib) -> None:
     lib.ono_sizeof.argtypes = [ci]
     lib.ono_sizeof.restype = ci
     lib.ono_embedding_grad_scratch.argtypes = [ll, ci, ci]
+    lib.ono_clip_one_launch.argtypes = [ci, ll, ci]
+    lib.ono_clip_one_launch.restype = ci
     lib.ono_embedding_grad_scratch.restype = lib.ono_clip_scratch.restype = ll
     for i, st in enumerate((OnoGemm, OnoLoss, OnoOptim, OnoRows, OnoSync, OnoPsAsync, OnoRing, OnoStagePull, OnoRingEmu, OnoFeed, OnoColsum, OnoDenseStep)):
         if lib.ono_sizeof(i) != C.sizeof(st):

@@ -203,3 +203,12 @@ def test_what_rounding_took_off_lse():
             token_logprobs(x, t, lse=v, lse_low=bad)
         with pytest.raises((ValueError, RuntimeError)):
             token_logprobs_grad(x, t, lse=v, lse_low=bad, d_logp=v, out=x)
+
+
+def test_a_cluster_is_taken_only_where_there_is_room_for_it():
+    """A device, or a part of one, that has no room for a cluster of 16 clips in two launches."""
+    from oxidized_neural_orchestra_b200.ops import _lib
+
+    one = _lib.load().ono_clip_one_launch
+    assert one(4, 101770, 1) == 1 and one(32, 131072, 9) == 1
+    assert one(4, 101770, 0) == 0 and one(33, 1000, 1) == 0 and one(4, 131073, 1) == 0
