@@ -51,7 +51,7 @@ def _out(out: torch.Tensor, logits: torch.Tensor) -> int:
     pitch = rows_of(out, "out")
     if out.shape != logits.shape:
         raise ValueError("out must have the logits' shape")
-    if out.data_ptr() == logits.data_ptr() and (out.dtype != logits.dtype or out.stride(0) != logits.stride(0)):
+    if out.data_ptr() == logits.data_ptr() and (out.dtype != logits.dtype or pitch != rows_of(logits, "logits")):
         raise ValueError("out over the logits needs the same type and rows")
     return pitch
 

@@ -212,3 +212,16 @@ def test_a_cluster_is_taken_only_where_there_is_room_for_it():
     one = _lib.load().ono_clip_one_launch
     assert one(4, 101770, 1) == 1 and one(32, 131072, 9) == 1
     assert one(4, 101770, 0) == 0 and one(33, 1000, 1) == 0 and one(4, 131073, 1) == 0
+
+
+def test_one_row_in_place_whatever_its_pitch():
+    """A single row has no next one: a view of it that says otherwise is the same place."""
+    from oxidized_neural_orchestra_b200.ops.token_loss import token_logprobs_grad, token_loss
+
+    buf, t, v = torch.zeros(1, 16), torch.zeros(1, dtype=torch.int64), torch.zeros(1)
+    x, out = buf[:, :9], buf[0, :9].unsqueeze(0).as_strided((1, 9), (9, 1))
+    assert x.stride(0) != out.stride(0)
+    with pytest.raises(RuntimeError, match="CUDA"):      # (nothing else is wrong with it)
+        token_loss(x, t, out=out)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        token_logprobs_grad(x, t, lse=v, d_logp=v, out=out)
