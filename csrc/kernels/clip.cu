@@ -384,7 +384,9 @@ static cudaError_t clip_go(const OnoClip* c, cudaStream_t st) {
     clip_norm_kernel<G><<<grid, CLIP_THREADS, 0, st>>>(b, part, parts == 0);
     parts = std::max(parts, grid);
   }
-  if (!c->out || parts == 0) {
+  if (parts == 0) {      // no values
+    clip_finish_kernel<<<1, CLIP_THREADS, 0, st>>>(part, 0, c->scale, c->max_norm, c->norm, c->coef);
+  } else if (!c->out) {
     const cudaError_t e = launch_behind(clip_finish_kernel, 1u, CLIP_THREADS, st, (const double*)part, parts, c->scale, c->max_norm, c->norm, c->coef);
     if (e != cudaSuccess) return e;
   } else {
