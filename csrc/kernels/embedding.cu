@@ -607,10 +607,14 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) embedding_join_kernel(const _
 
 // Places to a chunk: as many as leave enough warps to fill the GPU (a lane has U rows in flight whatever the chunk), fewer warps for short chunks.
 // Us, 64 a multiprocessor for every length: 131072 x 2048 268 against 255, 16384 x 1024 of 500 tokens 31 against 28; 128: 131072 x 256 79 against 62.
+constexpr int CHUNK_MIN = 8, CHUNK_MAX = 512;
+static long long chunk_least(int L, int width) {      // the fewest places that take chunks of L, or longer ones
+  const long long tiles = (width + 127) / 128, warps = (L > 64 ? 128 : L > 32 ? 64 : 32) * 148;
+  return L == CHUNK_MIN ? 0 : (warps + tiles - 1) / tiles * L;
+}
 static int grad_chunk(long long n, int width) {
-  const long long tiles = (width + 127) / 128;
-  int L = 512;
-  while (L > 8 && n / L * tiles < (L > 64 ? 128ll : L > 32 ? 64 : 32) * 148) L >>= 1;
+  int L = CHUNK_MAX;
+  while (n < chunk_least(L, width)) L >>= 1;
   return L;
 }
 
@@ -628,6 +632,20 @@ static GradScratch grad_scratch(long long n, int width) {
   g.part = g.runs + ((2 + 2 * chunks) * 4 + 15) / 16 * 16;
   g.bytes = g.part + chunks * 2 * g.pitch * 4;
   return g;
+}
+
+// Enough for n places and for any fewer: shorter chunks, and shorter tiles of the sort, of fewer places may be more of them.
+static long long grad_scratch_up_to(long long n, int width) {
+  const GradScratch g = grad_scratch(n, width);
+  long long chunks = 0, most = n;
+  for (int L = CHUNK_MAX; L >= CHUNK_MIN; L >>= 1) {
+    const long long least = chunk_least(L, width);
+    if (most < least || most < 0) continue;
+    chunks = std::max(chunks, (most + L - 1) / L);
+    most = least - 1;
+  }
+  const long long tiles = n > RANK_MAX ? std::min<long long>(SORT_TILES, (n + SORT_TILE - 1) / SORT_TILE) : 0;
+  return 2 * g.items + 3 * tiles * SORT_RADIX * 4 + ((2 + 2 * chunks) * 4 + 15) / 16 * 16 + chunks * 2 * g.pitch * 4;
 }
 
 template <typename TI, typename TO, int VEC, typename I>
@@ -667,7 +685,7 @@ extern "C" int ono_embedding(const OnoEmbedding* e, ono_stream_t stream) {
 }
 
 extern "C" long long ono_embedding_grad_scratch(long long n, int vocab, int width) {
-  return n < 0 || vocab <= 0 || vocab > ONO_DIM_MAX || width <= 0 || width > ONO_DIM_MAX ? -1 : n == 0 || grad_few(n, vocab) ? 0 : grad_scratch(n, width).bytes;
+  return n < 0 || vocab <= 0 || vocab > ONO_DIM_MAX || width <= 0 || width > ONO_DIM_MAX ? -1 : n == 0 || grad_few(n, vocab) ? 0 : grad_scratch_up_to(n, width);
 }
 
 extern "C" int ono_embedding_grad(const OnoEmbeddingGrad* e, ono_stream_t stream) {

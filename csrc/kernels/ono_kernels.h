@@ -498,7 +498,7 @@ typedef struct OnoEmbedding {
 int ono_embedding(const OnoEmbedding* e, ono_stream_t stream);
 // grad[v] = (accumulate ? grad[v] : 0) + scale * sum of d[i] over the i with ids[i] == v, in an order that the sizes and ids give: that of i, in parts where
 // there are many (the same bits every time). scratch: ono_embedding_grad_scratch bytes (0 for few
-// tokens), 16-byte aligned; calls that overlap on the device need one each.
+// tokens; enough for any fewer tokens of the same table), 16-byte aligned; calls that overlap on the device need one each.
 typedef struct OnoEmbeddingGrad {
   const void* d;             // [n, ld_d]
   const void* ids;           // [n]

@@ -53,7 +53,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, *, scal
 
 
 def embedding_grad_scratch(n: int, vocab: int, width: int) -> int:
-    """Bytes of scratch that ``embedding_grad`` wants for ``n`` tokens (0 for few; more tokens may want less)."""
+    """Bytes of scratch that ``embedding_grad`` wants for ``n`` tokens (0 for few), and no more for any fewer of them."""
     _sizes(vocab, width)
     return _lib.load().ono_embedding_grad_scratch(n, vocab, width)
 

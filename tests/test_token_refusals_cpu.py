@@ -225,3 +225,23 @@ def test_one_row_in_place_whatever_its_pitch():
         token_loss(x, t, out=out)
     with pytest.raises(RuntimeError, match="CUDA"):
         token_logprobs_grad(x, t, lse=v, d_logp=v, out=out)
+
+
+def test_scratch_for_many_tokens_does_for_fewer():
+    """One tensor, of what the most tokens want, serves all calls: wherever shorter chunks or other tiles begin, and everywhere between."""
+    import random
+
+    from oxidized_neural_orchestra_b200.ops.embedding import embedding_grad_scratch
+
+    rng = random.Random(1)
+    edges = {1, 511, 512, 513, 2048, 2049, 131072, 131073, 262144, 262145, 1000000}
+    for width in (1, 24, 128, 129, 517, 1024, 2048, 4096, 16384, 130000):
+        tiles = (width + 127) // 128
+        for L, warps in ((16, 32), (32, 32), (64, 64), (128, 128), (256, 128), (512, 128)):
+            least = -(-warps * 148 // tiles) * L
+            edges |= {least - L, least - 1, least, least + 1, least + L}
+    edges = sorted(edges | {int(2 ** rng.uniform(0, 27)) for _ in range(300)})
+    for width in (1, 24, 128, 129, 517, 1024, 2048, 4096, 16384, 130000):
+        for vocab in (5, 50257):
+            wanted = [embedding_grad_scratch(n, vocab, width) for n in edges if n > 0]
+            assert wanted == sorted(wanted), width
