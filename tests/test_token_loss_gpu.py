@@ -511,3 +511,22 @@ def test_what_rounding_took_off_of_rows_of_every_kind(rows, vocab, dtype):
     size = g.abs() + h.abs() * (2 * H.clamp_min(1.0) + 30).float()
     rest = slice(8, None)
     assert ((a - b).abs()[rest] <= (size * 2.0 ** -22 * rlse.float().abs().clamp_min(1.0))[rest].unsqueeze(1)).all()
+
+
+@pytest.mark.parametrize("vocab,dtype", [(210011, F32), (420013, BF16)])
+def test_loss_of_rows_too_long_to_be_kept(vocab, dtype):
+    """Rows that do not fit into the shared memory of a cluster: their logits are read again, in place as well, wherever rows and outputs begin."""
+    torch.manual_seed(vocab)
+    for ld, lead in ((vocab // 16 * 16 + 16, 0), (vocab + 2, 3)):
+        x, whole = _logits(6, vocab, dtype, ld, lead)
+        _special("huge", x)
+        x[3] = -math.inf
+        x[4, ::2] = torch.finfo(dtype).min
+        targets = torch.tensor([vocab - 1, 7, vocab // 2, 0, 4, -1], device="cuda")
+        for out_dtype in (F32, BF16):
+            _check_loss(x, whole, targets, out_dtype)
+        _check_loss(x, whole, targets, dtype, in_place=True)
+        x.copy_((torch.randn(6, vocab, device="cuda") * 3).to(dtype))
+        for out_dtype in (F32, BF16):
+            _check_loss(x, whole, targets, out_dtype)
+        _check_loss(x, whole, targets, dtype, in_place=True)
