@@ -4,7 +4,8 @@
 //
 // Either is bound by memory: the rows read and written, and for the gradient the whole table where it is not added to. Sums go over the tokens
 // in the order of their places, so that a gradient is the same to the bit from run to run: the places are sorted by token (stable), and
-// one warp adds up a run of equal tokens, or a long one's part in a chunk of the sorted places.
+// one warp adds up a run of equal tokens, or a long one's part in a chunk of the sorted places. A few hundred places are not sorted: a warp looks for those
+// of its token.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -112,7 +113,8 @@ __global__ void __launch_bounds__(256) embedding_kernel(const OnoEmbedding e, in
 }
 
 // ------------------------------------------------------------------------------------------------
-// Gradient. The places are sorted by token (stable), while other CTAs of the same launches fill the table with zeros.
+// Gradient. The places are sorted by token (stable), while other CTAs of the same launches fill the table with zeros. One launch ranks them, or one counts digits and
+// one to four sort by them; then embedding_sum_kernel, and embedding_join_kernel for runs of several chunks. For very few places embedding_few_kernel does all of it.
 // ------------------------------------------------------------------------------------------------
 struct GradDev {
   OnoEmbeddingGrad e;
@@ -126,7 +128,8 @@ struct GradDev {
   int zero;                            // values of a CTA that fills the table with zeros (a multiple of 4)
 };
 
-// Zeros for the CTAs behind the first ones of a launch: of the table's values, `zero` to a CTA, or of whole rows that many values long.
+// Zeros for the CTAs behind the first ones of a launch: of the table's values, `zero` to a CTA, or of whole rows that many values long, value by value, where
+// the table does not begin at 16 bytes (gradient of 16384 x 1024 of 50257: 68.5 us against 67.6).
 constexpr int ZERO_VALUES = 1 << 16, ZERO_LEAST = 2048;
 __device__ __forceinline__ void fill_zeros(const GradDev& p, long long cta) {
   const OnoEmbeddingGrad& e = p.e;
@@ -300,9 +303,9 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_scatter_kernel(const _
   }
 }
 
-// Second launch: a warp adds up the rows of a chunk of `chunk` sorted places, 32 * VEC columns of them. A run of equal tokens belongs to
+// embedding_sum_kernel: a warp adds up the rows of a chunk of `chunk` sorted places, 32 * VEC columns of them. A run of equal tokens belongs to
 // the chunk it starts in, whose warp follows it into the next chunk if it ends there. A longer run is summed chunk by chunk: part[c][1]
-// has the sum of what starts in c, part[c][0] of what comes from before; the third launch adds them in order.
+// has the sum of what starts in c, part[c][0] of what comes from before; embedding_join_kernel adds them in order.
 // A lane's values of a row: VEC of them, one behind the other (STEP 1, where rows are aligned) or every 32nd (STEP 32). `left`: columns from the first
 // of them on.
 template <typename T, int VEC, int STEP>
@@ -363,7 +366,8 @@ struct GradVec {      // the same of an f32 row; 16-byte accesses where it is al
 
 // U rows are in flight; with ACC those of the table that they are added to as well. (Eight values a lane are many registers: fewer rows, more warps. Us,
 // eight rows, four: 131072 x 512 of 200 tokens 58.0, 53.3, 16384 x 1024 58.9, 57.1, 131072 x 2048 318, 321; with ACC four, two in four blocks:
-// 131072 x 2048 257.6, 251.4, 131072 x 512 73.6, 62.9. Four values: 60000 x 1024 f32 with ACC four, two 105.8, 112.3, without eight, four 122.0, 124.2.)
+// 131072 x 2048 257.6, 251.4, 131072 x 512 73.6, 62.9, although the four blocks' 64 registers spill 64 bytes: of many tokens three blocks, without, take 262 against 253
+// and 101 against 95. Four values: 60000 x 1024 f32 with ACC four, two 105.8, 112.3, without eight, four 122.0, 124.2.)
 template <typename T, int VEC, int STEP, bool ACC, int U>
 __global__ void __launch_bounds__(256, U == 2 ? 4 : 1) embedding_sum_kernel(const __grid_constant__ GradDev p, int tiles) {
   const OnoEmbeddingGrad& e = p.e;
@@ -560,7 +564,7 @@ __global__ void __launch_bounds__(256) embedding_few_kernel(const OnoEmbeddingGr
   GradVec<VEC, STEP>::store(g, acc, left, aligned);
 }
 
-// Third launch: a block takes a long run's sums, 32 * VEC columns of them; its warps every JOIN_WARPS-th, then one adds up theirs.
+// embedding_join_kernel: a block takes a long run's sums, 32 * VEC columns of them; its warps every JOIN_WARPS-th, then one adds up theirs.
 // (Eight of them: 60000 x 256 of 1000 tokens 45.8 us against 42.6; 32: 9916 x 3509 58.0 against 56.2, but 600000 x 64 132 against 136.)
 constexpr int JOIN_WARPS = 16;
 template <int VEC>

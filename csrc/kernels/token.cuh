@@ -142,8 +142,9 @@ __device__ __forceinline__ void store_group(O* o, const float (&w)[E]) {
   }
 }
 
-// Rows of up to TOK_SHORT_ROW bytes, TOK_TOP of up to TOK_SHORT_TOP (token_short.cu). (Us, this against the other form: entropy and its gradient of 30000 x 800
-// f32 48, 56; loss of 8192 x 1900 bf16 17.7, 20.4; five alternatives of 65536 x 100 f32 59.6, 66.4, of 65536 x 300 bf16 148, 77.)
+// Rows of up to TOK_SHORT_ROW bytes, TOK_TOP of up to TOK_SHORT_TOP (token_short.cu). (Us, this against the other form: entropy of 30000 x 800 f32 16.9, 21.8, its gradient in
+// bf16 21.1, 23.5; loss of 8192 x 1900 bf16 13.8, 18.1; entropy of 47107 x 123 bf16 18.4, 25.6; five alternatives of 65536 x 100 f32 55, 65, of 65536 x 300 bf16 148, 77; twenty
+// of 65536 x 100 f32 135, 94, for which the rule has no case of its own.)
 constexpr int TOK_SHORT_ROW = 4096, TOK_SHORT_TOP = 512;
 int tok_short(const TokDev& d, int mode, int x_bf16, int out_bf16, cudaStream_t st);
 // 16-byte groups that a row takes wherever it begins.

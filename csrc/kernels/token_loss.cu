@@ -4,7 +4,9 @@
 //   z = sum exp(x - m), m = max x      lse = m + ln z      logp = (x_t - m) - ln z      entropy = ln z - sum exp(x - m) (x - m) / z
 //   d logp / dx_v = 1[v = t] - p_v      d entropy / dx_v = -p_v (ln p_v + entropy)
 //
-// All of it is f32 whatever the logits' type; x - m before the multiplication by log2 e, so that logits of any size keep their distances.
+// All of it is f32 whatever the logits' type. An exponential is one multiply-add and 2^: x log2 e less the maximum's, rounded once, so that logits keep
+// their distances; those of rows far from zero, which the product would take out of f32 or round too much, are subtracted first. lse, logp and the alternatives'
+// are differences from the maximum less the logarithm of the sum.
 //
 // Bound by memory, so a row is read once, by a warp, a CTA or a cluster of up to eight: a thread keeps a running maximum and sum of what it has seen,
 // the warps hand theirs to each other, and for the loss's gradient the row waits in shared memory meanwhile. Instructions are the next
@@ -187,7 +189,9 @@ __device__ __noinline__ void zero_write(O* d, int j0, int j1, int gt) {
 }
 
 // CTAs of an SM that the registers have to allow: 64 registers a thread, a few more where a row is gone through twice in one form or another (us, 1024
-// threads to an SM against this: loss of 4096 x 50257 bf16 175.4 -> 165.9, gradient of 4096 x 128256 362.6 -> 357.6).
+// threads to an SM against this: loss of 4096 x 50257 bf16 175.4 -> 165.9, gradient of 4096 x 128256 362.6 -> 357.6). A warp to a row in 64 registers spills 44 to 60
+// bytes for the gradient and up to 88 for alternatives; in 80 it does not and is faster or slower by the row (us, 64 and 80: gradient of 30000 x 2500
+// bf16 54, 59, of 4000 x 8000 f32 to bf16 32, 39, but of 16000 x 5000 f32 118, 111; five alternatives of 16000 x 5000 bf16 49, 52, f32 77, 71).
 constexpr int tok_resident(int mode, int warps, int threads) {
   return (warps == 1 || mode <= TOK_TOP ? 1024 : mode == TOK_LOSS ? 896 : 768) / threads;
 }
@@ -590,9 +594,14 @@ static TokShape tok_shape(long long rows, int V, int esz, int mode, int top) {
   // entropy of 47005 x 2322 f32 123.8, 69.9, of 8000 x 15000 bf16 51.2, 45.3; loss of 16000 x 5000 bf16 79.4, 67.7, but of 8000 x 8000 57.1, 60.7;
   // entropy of 300 x 5000 4.8, 7.7).
   s.warps = rows >= 16ll * ono_num_sms() && bytes <= (mode == TOK_LOSS ? 12288 : 32768) ? 1 : 4;
+  // Longer rows are shared out among CTAs where there are few. (Us, one CTA a row, CTAs by these limits, twice the CTAs allowed: entropy of 20 x 50257 bf16 6.2, 4.4, 4.3, of 150
+  // 7.7, 6.6, 7.7, of 333 10.7, 9.6, 10.1, of 600 14.7, 14.7, 13.5; five alternatives of 4 x 50257 f32 11.9, 7.1, 7.1, of 333 22.2, 18.1, 22.1, of 600 33, 33, 43; half as
+  // many CTAs are between. Not below 8 KB a CTA: 4 KB and 16 KB are within a tenth for 300 x 50257, 16 KB better by that for 300 x 5000.)
   if (s.warps > 1) {
     while (s.ctas < TOK_CTAS && ((mode == TOK_LOSS && bytes > (long long)TOK_SLICE * s.ctas) || (rows * s.ctas <= 4 * ono_num_sms() && bytes > 8192ll * s.ctas))) s.ctas *= 2;
   }
+  // Eight warps up to two CTAs an SM. (Us, four, eight up to here, eight for four times as many: twenty alternatives of 4 x 128256 bf16 12.5, 10.3, 10.3; entropy of
+  // 20 x 50257 4.1, 4.4, 4.3, of 100 5.3, 5.4, 7.9; five alternatives of 4 x 50257 f32 7.8, 7.1, 7.1, of 100 11.2, 11.2, 15.2.)
   if (s.warps > 1 && mode != TOK_LOSS && rows * s.ctas <= 2 * ono_num_sms()) s.warps = 8;
   s.per = (int)((groups + s.ctas - 1) / s.ctas);
   // A warp whose lanes have fewer logits than its share of the alternatives bounds nothing, and every logit would be a candidate (us, five of

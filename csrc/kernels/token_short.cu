@@ -1,6 +1,7 @@
 // The operators of token_loss.cu on short rows: a row lies in the registers of one warp, or of a few lanes of it, which load all of it at once.
 // Nothing is looped over and nothing goes through shared memory; a row costs its loads, a handful of shuffles and its stores, so that
-// what bounds it is memory or, of rows of a few logits, the launch and the latency of its one chain of loads.
+// what bounds it is memory or, of rows of a few logits, the launch and the latency of its one chain of loads. (The gradient of the longest bf16 rows spills 52 bytes in
+// the 64 registers of eight CTAs; seven without take longer: 16384 x 2000 25.0 us against 22.5.)
 #include <type_traits>
 
 #include "token.cuh"
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(128, NV == 1 ? 12 : 8) tok_short_kernel(const 
     if constexpr (TOP) {
       // The row's lanes find the largest of their largest logits, `top` times, of equal ones the lane with the lowest place; it goes on to its next.
       // A lane's logits are in the order of their places: of the row's beginning, its group, of the row's end. 0: none left. (65536 rows of 100 f32: five take
-      // 60 us, twenty 154; with the place as the lower half of 64-bit keys, and shuffles for all of it, 84 and 244.)
+      // 55 us, twenty 135; with the place as the lower half of 64-bit keys, and shuffles for all of it, 1.4 and 1.6 times as long.)
       static_assert(NV == 1, "one group to a lane");
       unsigned int key[E + 2], best, slot;
       auto key_of = [&](float v) { return v > ninf ? order_of(v) : 0u; };

@@ -52,9 +52,9 @@ def test_runs_at_the_edges_of_the_longest_chunks(L, d_dtype):
     _check_grad(ids, len(counts), _width(ids.numel(), L, 0), d_dtype, accumulate=d_dtype == F32)
 
 
-@pytest.mark.parametrize("n", [131072, 131073, 131072 + 1500, 262144, 262145, 400003])
-@pytest.mark.parametrize("vocab", [300, 511, 512, 70000, 300000])
-def test_more_places_than_a_batch_to_each_warp_of_the_sort(n, vocab):
+@pytest.mark.parametrize("vocab,n", [(v, n) for v in (300, 511, 512) for n in (131072, 131073, 131072 + 1500, 262144, 262145, 400003)] +
+                         [(70000, 131073), (70000, 262144), (70000, 400003), (270000, 132572), (270000, 400003)])
+def test_more_places_than_a_batch_to_each_warp_of_the_sort(vocab, n):
     """One to three passes; a CTA of the sort has one, two or four batches of the places, the last of them fewer."""
     torch.manual_seed(n % 1000 + vocab)
     for ids in (torch.randint(-1, vocab, (n,), device="cuda"), (torch.rand(n, device="cuda").pow(6) * vocab).to(torch.int32)):
