@@ -13,26 +13,27 @@ class DynBarrier {
  public:
   explicit DynBarrier(size_t size) : size_(size) {}
 
-  // Blocks until `size` participants arrived; the last one runs `leader` first. Returns true for
-  // the leader.
+  // Blocks until `size` participants arrived; the last one runs `leader` first, or, where a member's
+  // leaving has made them enough, one of those that wait. Returns true for the leader.
   bool wait_with(const std::function<void()>& leader) {
     std::unique_lock<std::mutex> lk(mu_);
     const size_t gen = generation_;
     ++arrived_;
-    if (arrived_ >= size_) {
-      release(leader);
-      return true;
-    }
-    cv_.wait(lk, [&] { return generation_ != gen; });
-    return false;
+    cv_.wait(lk, [&] { return generation_ != gen || arrived_ >= size_; });
+    if (generation_ != gen) return false;
+    if (leader) leader();
+    arrived_ = 0;
+    ++generation_;
+    cv_.notify_all();
+    return true;
   }
 
   // A participant leaves for good: the expected count drops by one, and if everyone else is already
-  // waiting they are released (the leader section runs on the leaving thread).
-  void leave(const std::function<void()>& leader) {
+  // waiting they are released.
+  void leave() {
     std::unique_lock<std::mutex> lk(mu_);
     if (size_ > 0) --size_;
-    if (size_ > 0 && arrived_ >= size_) release(leader);
+    cv_.notify_all();
   }
 
   size_t size() const {
@@ -41,12 +42,6 @@ class DynBarrier {
   }
 
  private:
-  void release(const std::function<void()>& leader) {
-    if (leader) leader();
-    arrived_ = 0;
-    ++generation_;
-    cv_.notify_all();
-  }
   mutable std::mutex mu_;
   std::condition_variable cv_;
   size_t size_, arrived_ = 0, generation_ = 0;

@@ -78,9 +78,7 @@ void BarrierSync::step(Store& store, const float* grad, size_t n, float* params_
   store.pull_params(params_out);
 }
 
-void BarrierSync::leave(Store& store) {
-  barrier_.leave([&] { store.update_params(); });
-}
+void BarrierSync::leave(Store&) { barrier_.leave(); }
 
 void NonBlockingSync::step(Store& store, const float* grad, size_t n, float* params_out) {
   store.accumulate(grad, n);
@@ -499,7 +497,7 @@ void LocalCluster::run_all() {
             failed.store(true);
             ClusterEvent ev; ev.kind = "error"; ev.worker = w; ev.text = e.what(); emit(std::move(ev));
             request_stop();
-            ring_barrier_->leave(nullptr);
+            ring_barrier_->leave();
           }
         });
       for (auto& t : threads_) t.join();

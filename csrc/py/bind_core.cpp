@@ -104,7 +104,7 @@ void bind_core(py::module_& m) {
   py::class_<DynBarrier>(m, "DynBarrier")
       .def(py::init<size_t>())
       .def("wait", [](DynBarrier& b) { py::gil_scoped_release rel; return b.wait_with(nullptr); })
-      .def("leave", [](DynBarrier& b) { b.leave(nullptr); })
+      .def("leave", [](DynBarrier& b) { b.leave(); })
       .def("size", &DynBarrier::size);
 
   // ---- codecs ----

@@ -48,6 +48,20 @@ def test_dyn_barrier_survivors_pass_when_a_member_leaves():
     assert sum(leaders) == 3 and len(passed) == 7       # one leader per generation, 3 + 3 + 1 passages
 
 
+def test_dyn_barrier_a_survivor_leads_when_a_member_leaves():
+    """All others wait already when the last member leaves: one of them runs the section that belongs to the passage, not the one that is gone."""
+    b, leaders = core.DynBarrier(3), []
+    ts = [threading.Thread(target=lambda: leaders.append(bool(b.wait()))) for _ in range(2)]
+    for t in ts:
+        t.start()
+    time.sleep(0.3)
+    assert not leaders and all(t.is_alive() for t in ts)
+    b.leave()
+    for t in ts:
+        t.join(timeout=20)
+    assert sorted(leaders) == [False, True] and b.size() == 2
+
+
 def test_a_node_that_dies_mid_run_ends_the_session_with_an_error():
     procs, addrs = spawn_nodes(3, "cpu", once=True)
     try:
