@@ -437,7 +437,6 @@ static void colsum_any(const T* d, int M, int N, int ld, float* out, float beta,
 // ------------------------------------------------------------------------------------------------
 struct OptimScalars {
   float lr, mu, b1, b2, eps, gs, adam_step, ob1, ob2;
-  bool once;
 };
 
 // An average moved towards x by the share of ob, whose weights add up to one: with ob rounded once beside 1 - ob as f32 has it, those of v would be 1.3e-5 too
@@ -446,6 +445,7 @@ __device__ __forceinline__ float toward(float old, float ob, float difference) {
   return fabsf(old) <= 3.402823466e38f ? fmaf(ob, difference, old) : old;
 }
 
+template <bool ONCE>
 __device__ __forceinline__ float optim_one(int kind, const OptimScalars& s, float p, float g, float* m, float* v) {
   g *= s.gs;
   if (kind == 0) return p - s.lr * g;  // gradient_descent.rs:45-47
@@ -455,16 +455,17 @@ __device__ __forceinline__ float optim_one(int kind, const OptimScalars& s, floa
     return p - s.lr * vel;
   }
   // adam.rs:75-91: step = lr*sqrt(1-b2^t)/(1-b1^t); p -= step * m / (sqrt(v) + eps)
-  const float mm = s.once ? toward(*m, s.ob1, g - *m) : s.b1 * (*m) + (1.0f - s.b1) * g;
-  const float vv = s.once ? toward(*v, s.ob2, fmaf(g, g, -*v)) : s.b2 * (*v) + (1.0f - s.b2) * g * g;
+  const float mm = ONCE ? toward(*m, s.ob1, g - *m) : s.b1 * (*m) + (1.0f - s.b1) * g;
+  const float vv = ONCE ? toward(*v, s.ob2, fmaf(g, g, -*v)) : s.b2 * (*v) + (1.0f - s.b2) * g * g;
   *m = mm;
   *v = vv;
   return p - s.adam_step * mm / (sqrtf(vv) + s.eps);
 }
 
+// ONCE: with ob1 and ob2. A kernel of its own, in which kind is 2: beside it the compiler would round the steps of the other kinds in another order.
+template <bool ONCE>
 __global__ void optim_kernel(const OnoOptim o) {
-  OptimScalars s{o.lr, o.mu, o.b1, o.b2, o.eps, o.grad_coef ? o.grad_scale * *o.grad_coef : o.grad_scale, 0.0f, o.ob1, o.ob2,
-                 o.ob1 != 0.0f || o.ob2 != 0.0f};
+  OptimScalars s{o.lr, o.mu, o.b1, o.b2, o.eps, o.grad_coef ? o.grad_scale * *o.grad_coef : o.grad_scale, 0.0f, o.ob1, o.ob2};
   if (o.kind == 2) {
     const float b1t = o.adam_pows[0], b2t = o.adam_pows[1];
     s.adam_step = o.lr * sqrtf(1.0f - b2t) / (1.0f - b1t);
@@ -482,10 +483,10 @@ __global__ void optim_kernel(const OnoOptim o) {
     const float4 g = g4[i];
     float4 m = o.kind >= 1 ? m4[i] : make_float4(0, 0, 0, 0);
     float4 v = o.kind == 2 ? v4[i] : make_float4(0, 0, 0, 0);
-    p.x = optim_one(o.kind, s, p.x, g.x, &m.x, &v.x);
-    p.y = optim_one(o.kind, s, p.y, g.y, &m.y, &v.y);
-    p.z = optim_one(o.kind, s, p.z, g.z, &m.z, &v.z);
-    p.w = optim_one(o.kind, s, p.w, g.w, &m.w, &v.w);
+    p.x = optim_one<ONCE>(o.kind, s, p.x, g.x, &m.x, &v.x);
+    p.y = optim_one<ONCE>(o.kind, s, p.y, g.y, &m.y, &v.y);
+    p.z = optim_one<ONCE>(o.kind, s, p.z, g.z, &m.z, &v.z);
+    p.w = optim_one<ONCE>(o.kind, s, p.w, g.w, &m.w, &v.w);
     p4[i] = p;
     if (o.kind >= 1) m4[i] = m;
     if (o.kind == 2) v4[i] = v;
@@ -500,7 +501,7 @@ __global__ void optim_kernel(const OnoOptim o) {
   }
   for (long long i = (n4 << 2) + tid; i < o.n; i += stride) {
     float m = o.kind >= 1 ? o.m[i] : 0.0f, v = o.kind == 2 ? o.v[i] : 0.0f;
-    const float p = optim_one(o.kind, s, o.p[i], o.g[i], &m, &v);
+    const float p = optim_one<ONCE>(o.kind, s, o.p[i], o.g[i], &m, &v);
     o.p[i] = p;
     if (o.kind >= 1) o.m[i] = m;
     if (o.kind == 2) o.v[i] = v;
@@ -728,7 +729,8 @@ extern "C" int ono_optim(const OnoOptim* o, ono_stream_t st) {
   }
   if (o->p_bf16 && ((uintptr_t)o->p_bf16 & 7)) { set_error("bf16 shadow must be 8-byte aligned%s", "", 0, 0); return -1; }
   if (o->n == 0) return 0;
-  optim_kernel<<<grid_for(o->n, 256, 8), 256, 0, (cudaStream_t)st>>>(*o);
+  const auto kern = o->kind == 2 && (o->ob1 != 0.0f || o->ob2 != 0.0f) ? optim_kernel<true> : optim_kernel<false>;
+  kern<<<grid_for(o->n, 256, 8), 256, 0, (cudaStream_t)st>>>(*o);
   return launch_ok("optim");
 }
 

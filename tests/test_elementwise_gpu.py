@@ -157,3 +157,16 @@ def test_powers_in_pinned_host_memory(own_stream):
         got.append((pows.cpu(), p, m, v))
     assert all(torch.equal(a, b) for a, b in zip(*got))
     assert not torch.equal(got[0][0], torch.ones(2))
+
+
+def test_sgd_rounds_its_update_once():
+    """p - lr g with g = grad_scale * gradient rounded: product and difference in one rounding (64 bits hold the product; their sum rounded to f32 is that one)."""
+    from oxidized_neural_orchestra_b200.ops import elementwise as ew
+
+    torch.manual_seed(6)
+    n = 100003
+    p, g = torch.randn(n, device="cuda"), torch.randn(n, device="cuda")
+    want = (p.double() - torch.tensor(0.01, device="cuda").double() * (g * torch.tensor(0.7, device="cuda")).double()).float()
+    assert not torch.equal(want, p - 0.01 * (g * 0.7))
+    ew.optim_step(p, g, kind="sgd", lr=0.01, grad_scale=0.7)
+    assert torch.equal(p, want)
