@@ -1,7 +1,7 @@
 """Python entries to the rows-by-token kernels (``csrc/kernels/embedding.cu``): a table's rows looked up by token, and its gradient.
 
 Like the other ops each call launches on the current (or given) stream, can be captured into a graph and returns nothing. Tables and
-rows are 2-D with unit inner stride, f32 or bf16; ids are int32 or int64, of any shape."""
+rows are 2-D with unit inner stride, f32 or bf16; ids are int32 or int64, of any shape. What is written lies in none of the inputs."""
 from __future__ import annotations
 
 import ctypes as C

@@ -1,7 +1,8 @@
 """Python entries to the softmax over a vocabulary with one given token per row (``csrc/kernels/token_loss.cu``): log probabilities,
 entropy, most likely alternatives, and the logits' gradients. ``elementwise.loss_backward`` is the form for one-hot (or soft) label rows.
 
-Logits are 2-D rows with unit inner stride, f32 or bf16; targets int32 or int64, one a row. Each call launches on the current (or given)
+Logits are 2-D rows with unit inner stride, f32 or bf16; targets int32 or int64, one a row. A gradient's ``out`` is the logits themselves or nowhere in them;
+no other result lies in an input or in another result. Each call launches on the current (or given)
 stream, can be captured into a graph and returns nothing.
 
 A logit of -inf has probability zero. A row of nothing else has log probability and ``lse`` of -inf, entropy 0 and a gradient of zeros; a
